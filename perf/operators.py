@@ -246,7 +246,8 @@ def _run_own(state):
     if case["kind"] == "quantize":
         return list(ops.quantize_fp8(state["x"], block_rows=case["block_rows"]))
     if case["kind"] == "linear":
-        return ops.linear_fp8(state["x"], state["xs"], state["w"], state["ws"], out_dtype=getattr(torch, case["out"]))
+        return ops.linear_fp8(state["x"], state["xs"], state["w"], state["ws"], out_dtype=getattr(torch, case["out"]),
+                              w_is_parameter=True)
     rule = case["rule"]
     return ops.moe_layer(state["h"], state["router"], state["correction"], case["groups"], case["keep"], case["top"],
                          2.5 if rule == "sigmoid" else 1.0, state["up"], state["down"], up_scale=state["up_scale"],
