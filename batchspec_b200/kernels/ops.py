@@ -128,6 +128,10 @@ _SIGNATURES = {
                             c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
                             c_void_p, c_void_p],
     "bspec_gate_heads": [c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "bspec_quantize_fp8": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_int,
+                           c_int, c_void_p],
+    "bspec_gemm_fp8": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
+                       c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "bspec_moe_route": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                         c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p],
     "bspec_moe_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
@@ -239,7 +243,7 @@ _TRACE_SETTERS = ["bspec_trace_set_attention_tcgen05", "bspec_trace_set_elementw
                   "bspec_trace_set_gemm_fp32", "bspec_trace_set_sampling", "bspec_trace_set_gemm_tcgen05", "bspec_trace_set_latent",
                   "bspec_trace_set_moe", "bspec_trace_set_latent_mma", "bspec_trace_set_latent_prompt", "bspec_trace_set_delta",
                   "bspec_trace_set_state_mixers", "bspec_trace_set_streams", "bspec_trace_set_joins",
-                  "bspec_trace_set_gated_states"]
+                  "bspec_trace_set_gated_states", "bspec_trace_set_fp8", "bspec_trace_set_gemm_fp8"]
 TRACE_KERNEL_NAMES = {1: "embed", 2: "add_rmsnorm", 3: "gather_rows_add", 4: "silu_mul", 5: "rope_kv_append",
                       6: "rope_inplace", 7: "attn_generic", 8: "attn_decode", 9: "attn_prefill", 10: "sgemm",
                       11: "sample_threshold", 12: "sample_pick", 13: "sample_final", 14: "add_layernorm", 15: "clamped_glu",
@@ -247,7 +251,8 @@ TRACE_KERNEL_NAMES = {1: "embed", 2: "add_rmsnorm", 3: "gather_rows_add", 4: "si
                       61: "delta_recurrence", 62: "gated_rmsnorm", 63: "bigram_add", 64: "scale", 65: "lightning_recurrence",
                       66: "scan_conv", 67: "selective_scan", 70: "stream_expand", 71: "stream_norm", 72: "stream_gather", 73: "branch_join", 74: "state_space", 75: "matrix_memory", 21: "pool_append", 20: "gemm_tcgen05", 30: "attn_prefill_tc", 40: "latent_prepare",
                       41: "latent_attn_generic", 42: "gate_heads", 43: "latent_attn_mma", 44: "latent_attn_join",
-                      50: "moe_route", 51: "moe_plan", 52: "moe_grouped", 53: "moe_gather", 54: "moe_combine", 55: "moe_skinny", 56: "moe_skinny_mma", 57: "moe_rank", 58: "moe_offsets", 59: "moe_place"}
+                      50: "moe_route", 51: "moe_plan", 52: "moe_grouped", 53: "moe_gather", 54: "moe_combine", 55: "moe_skinny", 56: "moe_skinny_mma", 57: "moe_rank", 58: "moe_offsets", 59: "moe_place",
+                      80: "quantize_rows", 81: "quantize_blocks", 82: "gemm_fp8_few", 83: "gemm_fp8_many"}
 
 
 def set_trace(buf: Optional[torch.Tensor], count: Optional[torch.Tensor]) -> None:
@@ -1242,7 +1247,8 @@ WAIT_CODES = ((1, 1, "GEMM: stage never freed"), (2, 2, "GEMM: operands never ar
               (64, 68, "latent attention of long portions: operands, weights or a free accumulator never came"),
               (69, 71, "latent attention of long portions: scores or sums never completed"),
               (91, 91, "float32 product of few rows: stage never freed"),
-              (92, 92, "float32 product of few rows: operands never arrived"))
+              (92, 92, "float32 product of few rows: operands never arrived"),
+              (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"))
 
 
 def wait_meaning(code: int) -> str:
@@ -1462,6 +1468,102 @@ def _sgemm(x, w, out, M: int, N: int, K: int, lda: int, ldw: int, sa: int, sw: i
                                       _ptr(scratch), int(w_is_parameter), _status_word(x.device).data_ptr(), _stream()), "sgemm_tn")
     if need:
         count_launches(1)
+
+
+# ---------------------------------------------------------------------------- 8-bit floating point
+
+FP8_BLOCK = 128                   # numbers of a row that share a scale; weights share one per 128 x 128
+
+
+def _stream_of(*tensors) -> int:
+    """The current stream of the device that all tensors are on, which has to be the current device."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise KernelError(f"tensors on {dev} and {t.device}: one launch takes tensors of one device")
+    if dev.type != "cuda":
+        raise KernelError("batchspec_b200 kernels run on a CUDA device only; got a tensor on " + str(dev))
+    if dev.index != torch.cuda.current_device():
+        raise KernelError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
+    """``x`` [..., R, K] (float32 or bfloat16) in 8-bit floating point with a scale per block: (q, scale) with x ~ q * scale.
+
+    Blocks are 128 numbers of a row (``block_rows`` 1: activations) or 128 x 128 numbers (``block_rows`` 128: weights); the last ones
+    may be shorter.  ``q`` float8_e4m3fn [..., R, K], each row on a 16-byte boundary (the row stride is K rounded up to 16);
+    ``scale`` float8_e8m0fnu [..., ceil(R / block_rows), ceil(K / 128)]: the smallest power of two, 2^-127 at least, with which no
+    number of the block exceeds 448, 1 for a block of zeros.  A block with an infinity or a NaN becomes NaN, scale and numbers.
+    A matrix may have strided rows (its numbers dense); more dimensions have to be contiguous."""
+    stream = _stream_of(x)
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"quantize_fp8 takes float32 or bfloat16, got {x.dtype}")
+    if block_rows not in (1, FP8_BLOCK):
+        raise KernelError(f"quantize_fp8: blocks of {block_rows} rows are not supported (1 or {FP8_BLOCK})")
+    if x.dim() < 2 or x.shape[-1] < 1:
+        raise KernelError(f"quantize_fp8 takes matrices of at least one column, got shape {tuple(x.shape)}")
+    R, K = x.shape[-2:]
+    if x.dim() == 2:
+        if K > 1 and x.stride(1) != 1:
+            raise KernelError("quantize_fp8: the numbers of a row have to be dense")
+        batch, ldx = 1, (x.stride(0) if R > 1 else K)
+    else:
+        if not x.is_contiguous():
+            raise KernelError("quantize_fp8: a tensor of more than two dimensions has to be contiguous")
+        batch, ldx = x.shape[:-2].numel(), K
+    lib = load_library(features=("fp8",))
+    pitch, KB = (K + 15) // 16 * 16, (K + FP8_BLOCK - 1) // FP8_BLOCK
+    q = torch.empty(x.shape[:-1] + (pitch,), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-2] + ((R + block_rows - 1) // block_rows, KB), dtype=torch.float8_e8m0fnu, device=x.device)
+    if batch * R:
+        _check(lib.bspec_quantize_fp8(x.data_ptr(), _dtype_code(x.dtype), ldx, R * ldx, q.data_ptr(), pitch, scale.data_ptr(), batch, R,
+                                      K, block_rows, stream), "quantize_fp8")
+    return (q if pitch == K else q[..., :K]), scale
+
+
+def _fp8_rows(t: torch.Tensor, name: str) -> int:
+    """Bytes from row to row of an e4m3 matrix that a tensor map can describe."""
+    rows, K = t.shape
+    if t.dtype != torch.float8_e4m3fn or (K > 1 and t.stride(1) != 1):
+        raise KernelError(f"linear_fp8: {name} has to be float8_e4m3fn with dense rows, got {t.dtype} with strides {t.stride()}")
+    ld = t.stride(0) if rows > 1 else (K + 15) // 16 * 16
+    if ld % 16 or ld < K or t.data_ptr() % 16:
+        raise KernelError(f"linear_fp8: the rows of {name} have to start on 16-byte boundaries (as quantize_fp8 lays them out), "
+                          f"got a row stride of {ld} bytes")
+    return ld
+
+
+def _fp8_scales(t: torch.Tensor, shape, name: str):
+    """(scales from row to row, whether they are 8-bit exponents) of a matrix of scales."""
+    if t.dtype not in (torch.float32, torch.float8_e8m0fnu) or tuple(t.shape) != tuple(shape):
+        raise KernelError(f"{name} has to be float32 or float8_e8m0fnu of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise KernelError(f"{name} has to have dense rows")
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[1]), int(t.dtype == torch.float8_e8m0fnu)
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               out_dtype: torch.dtype = torch.bfloat16, w_is_parameter: bool = False) -> torch.Tensor:
+    """(x * x_scale) [M, K] @ (w * w_scale)[N, K]^T -> [M, N] in ``out_dtype`` (bfloat16 or float32), the products of 8-bit numbers
+    (float8_e4m3fn) with a scale per block of 128: ``x_scale`` [M, ceil(K / 128)], ``w_scale`` [ceil(N / 128), ceil(K / 128)], float32 or
+    float8_e8m0fnu each.  ``quantize_fp8`` makes all four; the sums are float32.  ``w_is_parameter`` as in ``linear``."""
+    stream = _stream_of(x, x_scale, w, w_scale)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1:
+        raise KernelError(f"linear_fp8: x {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"linear_fp8 gives bfloat16 or float32, not {out_dtype}")
+    (M, K), N = x.shape, w.shape[0]
+    KB = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    ldx, ldw = _fp8_rows(x, "x"), _fp8_rows(w, "w")
+    ldxs, xe = _fp8_scales(x_scale, (M, KB), "linear_fp8: x_scale")
+    ldws, we = _fp8_scales(w_scale, ((N + FP8_BLOCK - 1) // FP8_BLOCK, KB), "linear_fp8: w_scale")
+    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    if M and N:
+        _check(load_library(features=("fp8",)).bspec_gemm_fp8(
+            x.data_ptr(), ldx, x_scale.data_ptr(), ldxs, xe, w.data_ptr(), ldw, w_scale.data_ptr(), ldws, we, out.data_ptr(),
+            int(out_dtype == torch.float32), M, N, K, int(w_is_parameter), _status_word(x.device).data_ptr(), stream), "gemm_fp8")
+    return out
 
 
 # ---------------------------------------------------------------------------- latent attention
