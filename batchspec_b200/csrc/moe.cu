@@ -21,26 +21,19 @@
 //
 // Nothing here reads a count on the host: grids are sized by upper bounds and surplus blocks leave at once, so the
 // kernels can be captured in a graph.
-#include "common.cuh"
+#include "moe_choose.cuh"
 #include <math.h>
 using namespace bspec;
 
 namespace {
 
 constexpr int ROUTE_THREADS = 128;
-// the router's rule: bits 0-1 what the scores are, then options
-constexpr int ROUTE_SIGMOID = 0, ROUTE_SOFTMAX_TOP = 1, ROUTE_SOFTMAX = 2, ROUTE_SCORES = 3;
-constexpr int ROUTE_GROUP_MAX = 4, ROUTE_RENORMALISE = 8;
-constexpr int MAX_EXPERTS = 1024;
-
 template <typename T>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 moe_route_kernel(const T* __restrict__ h, int d, const T* __restrict__ wr, const void* __restrict__ corr,
                  int corr_dtype, int E, int G, int keep, int top, float scale, int* __restrict__ ids,
                  float* __restrict__ wts, const float* __restrict__ logits, long long ld_logits, int rule) {
   bspec::pdl_prologue(50);
-  const int scores = rule & ROUTE_SCORES;
-  const bool softmax_top = scores == ROUTE_SOFTMAX_TOP;
   extern __shared__ float sm[];
   float* hs = sm;                 // [d]
   float* sc = hs + d;             // [E] sigmoid scores
@@ -48,10 +41,8 @@ moe_route_kernel(const T* __restrict__ h, int d, const T* __restrict__ wr, const
   const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (logits != nullptr) {            // the logits were formed by a matrix product (many tokens)
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
-      const float z = logits[(size_t)t * ld_logits + e], b = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
-      const float s = softmax_top ? z + b : (scores == ROUTE_SOFTMAX ? z : 1.f / (1.f + expf(-z)));
-      sc[e] = s;
-      ch[e] = softmax_top ? s : s + b;
+      const float b = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
+      route_score(rule, logits[(size_t)t * ld_logits + e], b, sc + e, ch + e);
     }
   } else {
     for (int i = threadIdx.x; i < d; i += blockDim.x) hs[i] = to_f32(h[(size_t)t * d + i]);
@@ -63,87 +54,14 @@ moe_route_kernel(const T* __restrict__ h, int d, const T* __restrict__ wr, const
       z = warp_sum(z);
       if (lane == 0) {
         const float b = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
-        const float s = softmax_top ? z + b : (scores == ROUTE_SOFTMAX ? z : 1.f / (1.f + expf(-z)));
-        sc[e] = s;
-        ch[e] = softmax_top ? s : s + b;
+        route_score(rule, z, b, sc + e, ch + e);
       }
     }
   }
   __syncthreads();
   if (warp != 0) return;
-  if (scores == ROUTE_SOFTMAX) {
-    float mx = -INFINITY, sum = 0.f;
-    for (int i = lane; i < E; i += 32) mx = fmaxf(mx, sc[i]);
-    mx = warp_max(mx);
-    for (int i = lane; i < E; i += 32) sum += expf(sc[i] - mx);
-    sum = warp_sum(sum);
-    // without a correction the logits themselves choose (the softmax keeps their order)
-    for (int i = lane; i < E; i += 32) {
-      sc[i] = expf(sc[i] - mx) / sum;
-      if (corr != nullptr) ch[i] = sc[i] + load_as_f32(corr, corr_dtype, i);
-    }
-    __syncwarp();
-  }
-  // The choice is made by warp 0: every lane scans its share of the candidates, a shuffle tree finds the best
-  // (the larger value, the lower index among equals), lane 0 marks it as taken (NaN).
-  auto best_of = [&](const float* v, int n) -> int {
-    float bv = 0.f;
-    int bi = 0x7fffffff;
-    for (int i = lane; i < n; i += 32) {
-      const float x = v[i];
-      if (!isnan(x) && (bi == 0x7fffffff || x > bv)) { bv = x; bi = i; }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
-    }
-    return bi;
-  };
-  if (G > 1 && keep < G) {
-    const int per = E / G;
-    for (int g = lane; g < G; g += 32) {          // group scores into the start of hs (no longer needed)
-      float a = -INFINITY, b = -INFINITY;         // the two largest
-      for (int j = 0; j < per; ++j) {
-        const float v = ch[g * per + j];
-        if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
-      }
-      hs[g] = per > 1 && !(rule & ROUTE_GROUP_MAX) ? a + b : a;
-    }
-    __syncwarp();
-    for (int k = 0; k < keep; ++k) {
-      const int best = best_of(hs, G);
-      if (lane == 0 && best != 0x7fffffff) hs[best] = NAN;      // NaN marks a kept group
-      __syncwarp();
-    }
-    for (int i = lane; i < E; i += 32)
-      if (!isnan(hs[i / per])) ch[i] = -INFINITY;
-    __syncwarp();
-  }
-  for (int k = 0; k < top; ++k) {
-    int best = best_of(ch, E);
-    if (best == 0x7fffffff) best = 0;
-    if (lane == 0) {
-      ids[(size_t)t * top + k] = best;
-      wts[(size_t)t * top + k] = sc[best] * scale;
-      ch[best] = NAN;                             // taken
-    }
-    __syncwarp();
-  }
-  if ((rule & ROUTE_RENORMALISE) && !softmax_top && lane == 0) {
-    float* w = wts + (size_t)t * top;
-    float sum = 0.f;
-    for (int k = 0; k < top; ++k) sum += sc[ids[(size_t)t * top + k]];
-    for (int k = 0; k < top; ++k) w[k] = sc[ids[(size_t)t * top + k]] / (sum + 1e-20f) * scale;
-  }
-  if (softmax_top && lane == 0) {                 // the weights: softmax over the chosen logits alone
-    float* w = wts + (size_t)t * top;
-    float mx = -INFINITY, sum = 0.f;
-    for (int k = 0; k < top; ++k) mx = fmaxf(mx, sc[ids[(size_t)t * top + k]]);
-    for (int k = 0; k < top; ++k) sum += expf(sc[ids[(size_t)t * top + k]] - mx);
-    for (int k = 0; k < top; ++k) w[k] = expf(sc[ids[(size_t)t * top + k]] - mx) / sum * scale;
-  }
+  // the choice is made by warp 0; the group scores take the start of hs (no longer needed)
+  choose_experts<false>(sc, ch, hs, corr, corr_dtype, E, G, keep, top, scale, rule, ids + (size_t)t * top, wts + (size_t)t * top);
 }
 
 // Numbers E and above are choices without rows of their own in the grouped products (identity experts): they are sorted
@@ -250,8 +168,6 @@ moe_place_kernel(const int* __restrict__ ids, const int* __restrict__ rank, cons
   perm[r] = s;
   inv[s] = r;
 }
-
-__device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752440f)); }
 
 // A gated operand (``gated_a`` in the kernels below): the rows of A are [gate | up], 2 K numbers, and the product's
 // operand is silu(gate) * up, formed while a tile's rows are staged and rounded to A's type, as a kernel of its own
@@ -419,13 +335,6 @@ moe_skinny_kernel(const __nv_bfloat16* __restrict__ A, const int* __restrict__ p
 // contiguous bytes of two weight rows straight from global memory (no staging: every weight is used once) and 16
 // bytes of a token row from shared memory; both sides number the 32 k of a step in the same permuted order
 // (lane l % 4 holds k = 8 (l % 4) .. + 7), which a sum over k does not notice.  Eight loads are in flight per lane.
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 template <typename TO, bool GELU, int RT>          // RT: token rows a tile may hold, 8 or 16
 __global__ void __launch_bounds__(256)
 moe_skinny_mma_kernel(const __nv_bfloat16* __restrict__ A, const int* __restrict__ perm, int top,

@@ -1,0 +1,121 @@
+// The router's choice of experts from their scores, by one warp: shared by the router kernel and by the kernels of a whole layer.
+#pragma once
+#include "common.cuh"
+
+namespace bspec {
+
+// the router's rule: bits 0-1 what the scores are, then options
+constexpr int ROUTE_SIGMOID = 0, ROUTE_SOFTMAX_TOP = 1, ROUTE_SOFTMAX = 2, ROUTE_SCORES = 3;
+constexpr int ROUTE_GROUP_MAX = 4, ROUTE_RENORMALISE = 8;
+constexpr int MAX_EXPERTS = 1024;
+
+// What a logit z and an expert's correction b make of its score and of its choice score (before a softmax over all).
+__device__ __forceinline__ void route_score(int rule, float z, float b, float* score, float* choice) {
+  const int scores = rule & ROUTE_SCORES;
+  const bool softmax_top = scores == ROUTE_SOFTMAX_TOP;
+  const float s = softmax_top ? z + b : (scores == ROUTE_SOFTMAX ? z : 1.f / (1.f + expf(-z)));
+  *score = s;
+  *choice = softmax_top ? s : s + b;
+}
+
+// One warp chooses the `top` experts of a token and their weights.  sc, ch [E]: scores and choice scores of route_score, in
+// shared memory (changed); hs: room for G numbers.  DISTINCT: where no number is left to compare (NaN logits), the lowest
+// expert not taken yet instead of expert 0, so that a token never has an expert twice.
+template <bool DISTINCT>
+__device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, const void* __restrict__ corr, int corr_dtype, int E,
+                                               int G, int keep, int top, float scale, int rule, int* __restrict__ ids,
+                                               float* __restrict__ w) {
+  const int lane = threadIdx.x & 31;
+  const int scores = rule & ROUTE_SCORES;
+  const bool softmax_top = scores == ROUTE_SOFTMAX_TOP;
+  if (scores == ROUTE_SOFTMAX) {
+    float mx = -INFINITY, sum = 0.f;
+    for (int i = lane; i < E; i += 32) mx = fmaxf(mx, sc[i]);
+    mx = warp_max(mx);
+    for (int i = lane; i < E; i += 32) sum += expf(sc[i] - mx);
+    sum = warp_sum(sum);
+    // without a correction the logits themselves choose (the softmax keeps their order)
+    for (int i = lane; i < E; i += 32) {
+      sc[i] = expf(sc[i] - mx) / sum;
+      if (corr != nullptr) ch[i] = sc[i] + load_as_f32(corr, corr_dtype, i);
+    }
+    __syncwarp();
+  }
+  // Every lane scans its share of the candidates, a shuffle tree finds the best
+  // (the larger value, the lower index among equals), lane 0 marks it as taken (NaN).
+  auto best_of = [&](const float* v, int n) -> int {
+    float bv = 0.f;
+    int bi = 0x7fffffff;
+    for (int i = lane; i < n; i += 32) {
+      const float x = v[i];
+      if (!isnan(x) && (bi == 0x7fffffff || x > bv)) { bv = x; bi = i; }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
+    }
+    return bi;
+  };
+  if (G > 1 && keep < G) {
+    const int per = E / G;
+    for (int g = lane; g < G; g += 32) {          // group scores
+      float a = -INFINITY, b = -INFINITY;         // the two largest
+      for (int j = 0; j < per; ++j) {
+        const float v = ch[g * per + j];
+        if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
+      }
+      hs[g] = per > 1 && !(rule & ROUTE_GROUP_MAX) ? a + b : a;
+    }
+    __syncwarp();
+    for (int k = 0; k < keep; ++k) {
+      const int best = best_of(hs, G);
+      if (lane == 0 && best != 0x7fffffff) hs[best] = NAN;      // NaN marks a kept group
+      __syncwarp();
+    }
+    for (int i = lane; i < E; i += 32)
+      if (!isnan(hs[i / per])) ch[i] = -INFINITY;
+    __syncwarp();
+  }
+  for (int k = 0; k < top; ++k) {
+    int best = best_of(ch, E);
+    if (best == 0x7fffffff) {
+      best = 0;
+      if (DISTINCT && lane == 0) {
+        for (int j = 0; j < k;) {
+          if (ids[j] == best) { ++best; j = 0; } else ++j;
+        }
+      }
+    }
+    if (lane == 0) {
+      ids[k] = best;
+      w[k] = sc[best] * scale;
+      ch[best] = NAN;                             // taken
+    }
+    __syncwarp();
+  }
+  if ((rule & ROUTE_RENORMALISE) && !softmax_top && lane == 0) {
+    float sum = 0.f;
+    for (int k = 0; k < top; ++k) sum += sc[ids[k]];
+    for (int k = 0; k < top; ++k) w[k] = sc[ids[k]] / (sum + 1e-20f) * scale;
+  }
+  if (softmax_top && lane == 0) {                 // the weights: softmax over the chosen logits alone
+    float mx = -INFINITY, sum = 0.f;
+    for (int k = 0; k < top; ++k) mx = fmaxf(mx, sc[ids[k]]);
+    for (int k = 0; k < top; ++k) sum += expf(sc[ids[k]] - mx);
+    for (int k = 0; k < top; ++k) w[k] = expf(sc[ids[k]] - mx) / sum * scale;
+  }
+}
+
+__device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752440f)); }
+
+// D += A B, 16 x 8 x 16, bfloat16 with float32 sums: lane l holds rows l / 4 and l / 4 + 8 of A and column l / 4 of B
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+}  // namespace bspec

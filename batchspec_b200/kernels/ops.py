@@ -132,6 +132,10 @@ _SIGNATURES = {
                            c_int, c_void_p],
     "bspec_gemm_fp8": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "bspec_moe_layer_route": [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "bspec_moe_layer_experts": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                                c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "bspec_moe_route": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                         c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p],
     "bspec_moe_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
@@ -243,7 +247,8 @@ _TRACE_SETTERS = ["bspec_trace_set_attention_tcgen05", "bspec_trace_set_elementw
                   "bspec_trace_set_gemm_fp32", "bspec_trace_set_sampling", "bspec_trace_set_gemm_tcgen05", "bspec_trace_set_latent",
                   "bspec_trace_set_moe", "bspec_trace_set_latent_mma", "bspec_trace_set_latent_prompt", "bspec_trace_set_delta",
                   "bspec_trace_set_state_mixers", "bspec_trace_set_streams", "bspec_trace_set_joins",
-                  "bspec_trace_set_gated_states", "bspec_trace_set_fp8", "bspec_trace_set_gemm_fp8"]
+                  "bspec_trace_set_gated_states", "bspec_trace_set_fp8", "bspec_trace_set_gemm_fp8",
+                  "bspec_trace_set_moe_layer"]
 TRACE_KERNEL_NAMES = {1: "embed", 2: "add_rmsnorm", 3: "gather_rows_add", 4: "silu_mul", 5: "rope_kv_append",
                       6: "rope_inplace", 7: "attn_generic", 8: "attn_decode", 9: "attn_prefill", 10: "sgemm",
                       11: "sample_threshold", 12: "sample_pick", 13: "sample_final", 14: "add_layernorm", 15: "clamped_glu",
@@ -252,7 +257,8 @@ TRACE_KERNEL_NAMES = {1: "embed", 2: "add_rmsnorm", 3: "gather_rows_add", 4: "si
                       66: "scan_conv", 67: "selective_scan", 70: "stream_expand", 71: "stream_norm", 72: "stream_gather", 73: "branch_join", 74: "state_space", 75: "matrix_memory", 21: "pool_append", 20: "gemm_tcgen05", 30: "attn_prefill_tc", 40: "latent_prepare",
                       41: "latent_attn_generic", 42: "gate_heads", 43: "latent_attn_mma", 44: "latent_attn_join",
                       50: "moe_route", 51: "moe_plan", 52: "moe_grouped", 53: "moe_gather", 54: "moe_combine", 55: "moe_skinny", 56: "moe_skinny_mma", 57: "moe_rank", 58: "moe_offsets", 59: "moe_place",
-                      80: "quantize_rows", 81: "quantize_blocks", 82: "gemm_fp8_few", 83: "gemm_fp8_many"}
+                      80: "quantize_rows", 81: "quantize_blocks", 82: "gemm_fp8_few", 83: "gemm_fp8_many",
+                      84: "moe_layer_route", 85: "moe_layer_experts"}
 
 
 def set_trace(buf: Optional[torch.Tensor], count: Optional[torch.Tensor]) -> None:
@@ -1248,7 +1254,8 @@ WAIT_CODES = ((1, 1, "GEMM: stage never freed"), (2, 2, "GEMM: operands never ar
               (69, 71, "latent attention of long portions: scores or sums never completed"),
               (91, 91, "float32 product of few rows: stage never freed"),
               (92, 92, "float32 product of few rows: operands never arrived"),
-              (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"))
+              (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"),
+              (111, 111, "routed layer of a few tokens: the up products never completed"))
 
 
 def wait_meaning(code: int) -> str:
@@ -1887,6 +1894,86 @@ def moe_experts(h: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_up: tor
                                  out.data_ptr(), _dtype_code(out_dtype), n, d, _ptr(add), ids.data_ptr() if identity else None,
                                  E, h.data_ptr() if identity else None, _ptr(add_gate),
                                  add_gate.stride(0) if add_gate is not None else 0, _stream()), "moe_combine")
+    return out
+
+
+MOE_LAYER_MAX = 64               # tokens that moe_layer takes
+
+
+def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.Tensor], n_groups: int, keep: int, top: int,
+              scale: float, w_up: torch.Tensor, w_down: torch.Tensor, up_scale: Optional[torch.Tensor] = None,
+              down_scale: Optional[torch.Tensor] = None, glu: bool = False, softmax_top: bool = False, softmax: bool = False,
+              group_max: bool = False, renormalise: bool = False, add: Optional[torch.Tensor] = None, add_gated: bool = False,
+              identity: int = 0) -> torch.Tensor:
+    """A whole routed feed-forward for at most ``MOE_LAYER_MAX`` tokens in two kernels: ``moe_route`` and ``moe_experts`` on its result
+    (their arguments of the same names have the same meaning), [n, d] in bfloat16 for bfloat16 ``h`` [n, d].
+
+    ``router`` [E + identity (+ 1)] rows: the experts, then ``identity`` experts whose result is h itself, then, with ``add_gated``, the row
+    whose logit's sigmoid multiplies ``add``.  ``w_up`` [E, ff, d] (``glu``: [E, 2 ff, d], gates first), ``w_down`` [E, d, ff]: bfloat16,
+    or float8_e4m3fn with ``up_scale`` / ``down_scale``, a float32 or float8_e8m0fnu scale per 128 x 128 block of every expert (both of one
+    type; what ``quantize_fp8`` makes of the stacked matrices).  8-bit weights have to be finite numbers (a NaN shows through its block's
+    scale, as ``quantize_fp8`` leaves it).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps: ``moe_route`` and
+    ``moe_experts``."""
+    stream = _stream_of(h, router, correction, w_up, w_down, up_scale, down_scale, add)
+    if h.dim() != 2 or w_up.dim() != 3 or w_down.dim() != 3 or router.dim() != 2:
+        raise KernelError("moe_layer takes h and router as matrices, w_up and w_down as stacks of matrices")
+    (n, d), (E, ff_up, _) = h.shape, w_up.shape
+    ff = ff_up // 2 if glu else ff_up
+    fp8 = w_up.dtype == torch.float8_e4m3fn
+    many = E + int(identity)
+    if h.dtype != torch.bfloat16 or router.dtype != h.dtype or w_down.dtype != w_up.dtype or not (fp8 or w_up.dtype == torch.bfloat16):
+        raise KernelError(f"moe_layer takes bfloat16 tokens and router, experts in bfloat16 or float8_e4m3fn; got {h.dtype}, {router.dtype}, "
+                          f"{w_up.dtype}, {w_down.dtype}")
+    if n > MOE_LAYER_MAX:
+        raise KernelError(f"moe_layer takes at most {MOE_LAYER_MAX} tokens, got {n}: longer steps go through moe_route and moe_experts")
+    unit = 16 if fp8 else 8
+    if E < 1 or many > 1024 or identity < 0 or d < 1 or ff < 1 or d % unit or ff % unit or (glu and ff_up % 2):
+        raise KernelError(f"moe_layer: {E} experts (+ {identity}) of {d} x {ff} are not supported: at most 1024, sizes multiples of {unit}")
+    if tuple(w_up.shape) != (E, ff_up, d) or tuple(w_down.shape) != (E, d, ff) or tuple(router.shape) != (many + int(add_gated), d):
+        raise KernelError(f"moe_layer: h {tuple(h.shape)}, router {tuple(router.shape)}, w_up {tuple(w_up.shape)} and w_down "
+                          f"{tuple(w_down.shape)} do not fit each other")
+    if not (0 < top <= many and n_groups > 0 and many % n_groups == 0 and 0 < keep <= n_groups and keep * (many // n_groups) >= top):
+        raise KernelError(f"moe_layer: routing of {top} of {many} experts in {n_groups} groups keeping {keep} is not possible")
+    if (softmax and softmax_top) or (add_gated and add is None):
+        raise KernelError("moe_layer: softmax and softmax_top exclude each other; add_gated needs add")
+    for name, t in (("h", h), ("router", router), ("w_up", w_up), ("w_down", w_down)):
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"moe_layer: {name} has to be contiguous and to start on a 16-byte boundary")
+    if correction is not None and (tuple(correction.shape) != (many,) or not correction.is_contiguous()):
+        raise KernelError(f"moe_layer: correction has to be a dense vector of {many} numbers")
+    if add is not None and (add.shape != h.shape or add.dtype != h.dtype or not add.is_contiguous()):
+        raise KernelError("moe_layer: add has to be a dense bfloat16 matrix like h")
+    e8m0 = 0
+    if fp8:
+        if up_scale is None or down_scale is None:
+            raise KernelError("moe_layer: 8-bit experts need up_scale and down_scale")
+        b = [(v + FP8_BLOCK - 1) // FP8_BLOCK for v in (ff_up, d, ff)]
+        for name, t, shape in (("up_scale", up_scale, (E, b[0], b[1])), ("down_scale", down_scale, (E, b[1], b[2]))):
+            if t.dtype not in (torch.float32, torch.float8_e8m0fnu) or tuple(t.shape) != shape or not t.is_contiguous():
+                raise KernelError(f"moe_layer: {name} has to be dense float32 or float8_e8m0fnu of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+        if up_scale.dtype != down_scale.dtype:
+            raise KernelError("moe_layer: up_scale and down_scale have to be of one type")
+        e8m0 = int(up_scale.dtype == torch.float8_e8m0fnu)
+    elif up_scale is not None or down_scale is not None:
+        raise KernelError("moe_layer: bfloat16 experts take no scales")
+    out = torch.empty((n, d), dtype=h.dtype, device=h.device)
+    if n == 0:
+        return out
+    lib = load_library(features=("moe",))
+    # counters, expert numbers, weights and gate logits of this call, then u: a buffer of its own, so that calls on other streams or in
+    # other graphs share nothing
+    slots = n * top
+    head = (4 + 2 * slots + n + 3) // 4 * 16
+    scratch = torch.empty((head + 2 * slots * ff,), dtype=torch.uint8, device=h.device)
+    at = scratch.data_ptr()
+    ids, wts, gate, u = at + 16, at + 16 + 4 * slots, at + 16 + 8 * slots, at + head
+    rule = (1 if softmax_top else 2 if softmax else 0) + (4 if group_max else 0) + (8 if renormalise else 0)
+    _check(lib.bspec_moe_layer_route(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),
+                                     _dtype_code(correction.dtype) if correction is not None else F32, many, int(n_groups), int(keep),
+                                     int(top), float(scale), rule, ids, wts, gate, at, stream), "moe_layer_route")
+    _check(lib.bspec_moe_layer_experts(h.data_ptr(), n, d, w_up.data_ptr(), w_down.data_ptr(), _ptr(up_scale), _ptr(down_scale), e8m0, E, ff,
+                                       int(bool(glu)), ids, wts, int(top), gate if add_gated else None, _ptr(add), u, out.data_ptr(), at,
+                                       _status_word(h.device).data_ptr(), stream), "moe_layer_experts")
     return out
 
 
