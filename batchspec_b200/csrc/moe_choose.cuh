@@ -41,22 +41,18 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
     }
     __syncwarp();
   }
-  // Every lane scans its share of the candidates, a shuffle tree finds the best
-  // (the larger value, the lower index among equals), lane 0 marks it as taken (NaN).
+  // Every lane scans its share of the candidates; the best (the larger value, the lower index among equals) is found by two
+  // reductions over the lanes, of the values in the order of their bits and of the indices that hold the largest.  NaN: taken.
   auto best_of = [&](const float* v, int n) -> int {
-    float bv = 0.f;
+    unsigned bv = 0u;
     int bi = 0x7fffffff;
     for (int i = lane; i < n; i += 32) {
-      const float x = v[i];
-      if (!isnan(x) && (bi == 0x7fffffff || x > bv)) { bv = x; bi = i; }
+      const float x = v[i] + 0.f;                  // one zero
+      const unsigned b = __float_as_uint(x), key = isnan(x) ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
+      if (key > bv) { bv = key; bi = i; }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
-    }
-    return bi;
+    const unsigned most = __reduce_max_sync(0xffffffffu, bv);
+    return most == 0u ? 0x7fffffff : __reduce_min_sync(0xffffffffu, bv == most ? bi : 0x7fffffff);
   };
   if (G > 1 && keep < G) {
     const int per = E / G;
@@ -78,29 +74,51 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
       if (!isnan(hs[i / per])) ch[i] = -INFINITY;
     __syncwarp();
   }
+  // Lane k keeps choice k (and k + 32 ...: `top` beyond the lanes goes through memory); sums run over the choices in their order.
+  int mine = 0;
   for (int k = 0; k < top; ++k) {
     int best = best_of(ch, E);
     if (best == 0x7fffffff) {
       best = 0;
-      if (DISTINCT && lane == 0) {
-        for (int j = 0; j < k;) {
-          if (ids[j] == best) { ++best; j = 0; } else ++j;
-        }
+      if (DISTINCT) {
+        if (lane == 0)
+          for (int j = 0; j < k;) {
+            if (ids[j] == best) { ++best; j = 0; } else ++j;
+          }
+        best = __shfl_sync(0xffffffffu, best, 0);
       }
     }
+    if (lane == (k & 31)) mine = best;
     if (lane == 0) {
       ids[k] = best;
-      w[k] = sc[best] * scale;
+      if (top > 32) w[k] = sc[best] * scale;
       ch[best] = NAN;                             // taken
     }
     __syncwarp();
   }
-  if ((rule & ROUTE_RENORMALISE) && !softmax_top && lane == 0) {
+  const bool renormalise = (rule & ROUTE_RENORMALISE) && !softmax_top;
+  if (top <= 32) {
+    const float s = lane < top ? sc[mine] : -INFINITY;
+    float v = s * scale;
+    if (renormalise) {
+      float sum = 0.f;
+      for (int k = 0; k < top; ++k) sum += __shfl_sync(0xffffffffu, s, k);
+      v = s / (sum + 1e-20f) * scale;
+    } else if (softmax_top) {                     // the weights: softmax over the chosen logits alone
+      const float e = expf(s - warp_max(s));
+      float sum = 0.f;
+      for (int k = 0; k < top; ++k) sum += __shfl_sync(0xffffffffu, e, k);
+      v = e / sum * scale;
+    }
+    if (lane < top) w[lane] = v;
+    return;
+  }
+  if (renormalise && lane == 0) {
     float sum = 0.f;
     for (int k = 0; k < top; ++k) sum += sc[ids[k]];
     for (int k = 0; k < top; ++k) w[k] = sc[ids[k]] / (sum + 1e-20f) * scale;
   }
-  if (softmax_top && lane == 0) {                 // the weights: softmax over the chosen logits alone
+  if (softmax_top && lane == 0) {
     float mx = -INFINITY, sum = 0.f;
     for (int k = 0; k < top; ++k) mx = fmaxf(mx, sc[ids[k]]);
     for (int k = 0; k < top; ++k) sum += expf(sc[ids[k]] - mx);

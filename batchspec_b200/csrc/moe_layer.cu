@@ -5,11 +5,10 @@
 // Experts in bfloat16, or in 8-bit floating point (e4m3) with a scale per 128 x 128 block; activations stay bfloat16 either
 // way (u is rounded to bfloat16 between the products: it is the operand of a bfloat16 product), sums are float32.
 //
-// Bound by the read of the chosen experts' weights, each of which is used once per step: a weight is fetched once, by
-// cp.async into a ring of its warp's own (a lane reads back the 16 bytes it fetched itself, so the ring needs no barriers, and
-// several KB per warp are in flight whatever the registers hold), and meets up to 64 token columns on mma.sync m16n8k16.  The
-// WEIGHT rows take the 16 rows of the product, the expert's tokens its columns, 8 at a time; both operands number the k of a
-// step in the same permuted order (lane l % 4 holds neighbouring k), which a sum over k does not notice.
+// Bound by the read of the chosen experts' weights.  A weight is fetched once per 16 tokens of its expert, by bulk copies into a ring
+// of its warp's own (several KB per warp are in flight, whatever the registers hold), and meets its tokens on mma.sync m16n8k16: the
+// WEIGHT rows take the 16 rows of the product, the expert's tokens its columns, 8 at a time.  Both operands number the k of a step in
+// the same permuted order (lane l % 4 holds neighbouring k), which a sum over k does not notice.
 //
 //   route    one cluster of 8 CTAs per 8 tokens: 64 warps share the router's rows and k, partial sums meet in the first CTA's
 //            shared memory, whose warps choose for a token each.  It also clears the counters of the second kernel.
@@ -18,6 +17,7 @@
 //            all been drawn by CTAs that run and wait for nothing, so it ends however many CTAs the device can hold.  A column's
 //            sum runs over the experts in a fixed order: no atomic adds numbers.
 #include "moe_choose.cuh"
+#include "tma.cuh"
 #include <math.h>
 
 using namespace bspec;
@@ -27,12 +27,10 @@ namespace {
 constexpr int LAYER_TOKENS = 64;             // most tokens of a step
 constexpr int ROUTE_CLUSTER = 8, ROUTE_WARPS = 8, ROUTE_TOKENS = 8;
 constexpr int WARPS = 16, LAYER_THREADS = 32 * WARPS;
-constexpr int SMEM_BUDGET = 220 * 1024;
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+constexpr int SMEM_BUDGET = 225 * 1024;
 
 // ------------------------------------------------------------------------------------------------ the router
-// z partials: [unit = (16 rows of the router, slice of k)][16 rows][8 tokens] in the first CTA of the cluster.
+// z partials: [unit = (16 rows of the router, slice of k)][8 tokens][16 rows] in the first CTA of the cluster.
 __global__ void __cluster_dims__(ROUTE_CLUSTER, 1, 1) __launch_bounds__(32 * ROUTE_WARPS)
 moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const __nv_bfloat16* __restrict__ wr, int rows, int slices,
                        const void* __restrict__ corr, int corr_dtype, int C, int G, int keep, int top, float scale, int rule,
@@ -40,14 +38,14 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   bspec::pdl_prologue(84);
   extern __shared__ float sm[];
   const int tiles = (rows + 15) / 16, units = tiles * slices;
-  float* part = sm;                                            // [units][16][8]
+  float* part = sm;                                            // [units][8][16]
   const int rank = blockIdx.x % ROUTE_CLUSTER, t0 = blockIdx.x / ROUTE_CLUSTER * ROUTE_TOKENS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   if (blockIdx.x == 0 && threadIdx.x < 4) counters[threadIdx.x] = 0;
   // every CTA of the cluster runs before another one writes to its memory
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   uint32_t first;                                              // the first CTA's partials
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(first) : "r"(smem_addr(part)), "r"(0));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(first) : "r"(s32(part)), "r"(0));
   const int steps = (d + 31) / 32, per = (steps + slices - 1) / slices;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const bool token = t0 + g < n;
@@ -75,23 +73,28 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = (unit * 16 + g + 8 * (i >> 1)) * ROUTE_TOKENS + 2 * q + (i & 1);
+      const int at = (unit * ROUTE_TOKENS + 2 * q + (i & 1)) * 16 + g + 8 * (i >> 1);
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(first + 4u * (uint32_t)at), "f"(acc[i]) : "memory");
     }
   }
+  float* bias = part + (size_t)units * 16 * ROUTE_TOKENS;      // [C]
+  if (rank == 0)
+    for (int e = threadIdx.x; e < C; e += 32 * ROUTE_WARPS) bias[e] = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int t = t0 + warp;
   if (rank != 0 || t >= n) return;
-  float* sc = part + (size_t)units * 16 * ROUTE_TOKENS + (size_t)warp * 3 * C;
+  float* sc = bias + C + (size_t)warp * 3 * C;
   float* ch = sc + C;
   for (int e = lane; e < rows; e += 32) {
+    const float* from = part + ((size_t)(e / 16 * slices) * ROUTE_TOKENS + warp) * 16 + e % 16;
     float z = 0.f;
-    for (int s = 0; s < slices; ++s) z += part[((e / 16 * slices + s) * 16 + e % 16) * ROUTE_TOKENS + warp];
-    if (e < C) route_score(rule, z, corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f, sc + e, ch + e);
+#pragma unroll 8
+    for (int s = 0; s < slices; ++s) z += from[s * ROUTE_TOKENS * 16];
+    if (e < C) route_score(rule, z, bias[e], sc + e, ch + e);
     else gate[t] = z;                                          // the row behind the experts' rows
   }
   __syncwarp();
-  choose_experts<true>(sc, ch, ch + C, corr, corr_dtype, C, G, keep, top, scale, rule, ids + (size_t)t * top, wts + (size_t)t * top);
+  choose_experts<true>(sc, ch, ch + C, corr != nullptr ? bias : nullptr, BSPEC_F32, C, G, keep, top, scale, rule, ids + (size_t)t * top, wts + (size_t)t * top);
 }
 
 // ------------------------------------------------------------------------------------------------ the experts
@@ -111,27 +114,17 @@ struct LayerParams {
   int* counters;                             // {pieces drawn, up pieces done, output pieces drawn}, zero
   int* status;
   int n, d, ff, E, top;
-  int stages, ring_tiles;                    // of a warp's ring: stages, and column tiles whose tokens are fetched through it
+  int stages;                                // of a warp's ring
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp16_l1(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but the newest `left` groups have landed
-__device__ __forceinline__ void cp_wait(int left) {
-  if (left <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
-}
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
+}
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // Four e4m3 numbers -> bfloat16, two to a register.  Sign, exponent and fraction move to their places, which leaves a number 2^120 times
 // too small (the exponents' biases differ by 120; numbers below e4m3's normal ones become bfloat16 numbers below its normal ones); the
@@ -152,371 +145,339 @@ __device__ __forceinline__ float block_scale(const void* p, int e8m0, size_t i) 
   return __uint_as_float(code == 0u ? 0x00400000u : (code == 255u ? 0x7fc00000u : code << 23));
 }
 
-// A stage of a warp's ring: 16 weight rows of DEPTH k (2 KB), then for each column tile 8 tokens' numbers.
-template <bool FP8> struct Ring;
-template <> struct Ring<false> { static constexpr int DEPTH = 64, ESZ = 2, STEP = 32, B_PIECES = 2; };
-template <> struct Ring<true> { static constexpr int DEPTH = 128, ESZ = 1, STEP = 64, B_PIECES = 4; };
-constexpr int A_BYTES = 2048;
-
-// the weights of a stage: rows `lo` and `hi` of this lane (null: zeros), k from k0
-template <bool FP8>
-__device__ __forceinline__ void fetch_weights(uint32_t at, const unsigned char* lo, const unsigned char* hi, const unsigned char* any,
-                                              int k0, int K) {
-  using R = Ring<FP8>;
-  const int q = threadIdx.x & 3;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int k = k0 + R::STEP * s + (16 / R::ESZ) * q;
-    const bool in = k < K;
-    cp16(at + (2 * s) * 512, in && lo ? lo + (size_t)k * R::ESZ : any, in && lo);
-    cp16(at + (2 * s + 1) * 512, in && hi ? hi + (size_t)k * R::ESZ : any, in && hi);
-  }
-}
-// the k of piece p of a token's numbers in a stage
-template <bool FP8>
-__device__ __forceinline__ int token_k(int k0, int p) {
-  const int q = threadIdx.x & 3;
-  return FP8 ? k0 + 64 * (p >> 1) + 16 * q + 8 * (p & 1) : k0 + 32 * p + 8 * q;
-}
-template <bool FP8, bool L1>
-__device__ __forceinline__ void fetch_tokens(uint32_t at, const __nv_bfloat16* row, const void* any, int k0, int K) {
-#pragma unroll
-  for (int p = 0; p < Ring<FP8>::B_PIECES; ++p) {
-    const int k = token_k<FP8>(k0, p);
-    const bool live = row != nullptr && k < K;
-    if (L1) cp16_l1(at + p * 512, live ? (const void*)(row + k) : any, live);
-    else cp16(at + p * 512, live ? (const void*)(row + k) : any, live);
-  }
-}
-
-// The products of one stage: acc[t] += the 16 rows x column tile t, for the first `nt` tiles.  `b_at`: the tokens' numbers in the
-// ring (T column tiles of them), or 0: they are read from `rows`.  8-bit weights: s_lo, s_hi are the scales of this lane's two rows.
-template <bool FP8, int T>
-__device__ __forceinline__ void multiply(uint32_t a_at, uint32_t b_at, const __nv_bfloat16* const* rows, int k0, int K, int nt,
-                                         float s_lo, float s_hi, float (&acc)[T][4]) {
-  using R = Ring<FP8>;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  auto token = [&](int t, int p) -> uint4 {
-    if (b_at != 0u) return lds16(b_at + (uint32_t)(t * R::B_PIECES + p) * 512u);
-    const int k = token_k<FP8>(k0, p);
-    return rows[t] != nullptr && k < K ? __ldcg(reinterpret_cast<const uint4*>(rows[t] + k)) : zero;
-  };
-  if (FP8) {
-    float sum[T][4];
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint4 lo = lds16(a_at + (2 * s) * 512), hi = lds16(a_at + (2 * s + 1) * 512);
-      const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
-      uint32_t wl[8], wh[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        widen4(l[j], wl[2 * j], wl[2 * j + 1]);
-        widen4(h[j], wh[2 * j], wh[2 * j + 1]);
-      }
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-        if (t < nt) {
-          const uint4 x = token(t, 2 * s), y = token(t, 2 * s + 1);
-          mma_bf16_16816(sum[t], wl[0], wh[0], wl[1], wh[1], x.x, x.y);
-          mma_bf16_16816(sum[t], wl[2], wh[2], wl[3], wh[3], x.z, x.w);
-          mma_bf16_16816(sum[t], wl[4], wh[4], wl[5], wh[5], y.x, y.y);
-          mma_bf16_16816(sum[t], wl[6], wh[6], wl[7], wh[7], y.z, y.w);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      acc[t][0] = fmaf(sum[t][0], s_lo, acc[t][0]);
-      acc[t][1] = fmaf(sum[t][1], s_lo, acc[t][1]);
-      acc[t][2] = fmaf(sum[t][2], s_hi, acc[t][2]);
-      acc[t][3] = fmaf(sum[t][3], s_hi, acc[t][3]);
-    }
-  } else {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint4 lo = lds16(a_at + (2 * s) * 512), hi = lds16(a_at + (2 * s + 1) * 512);
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-        if (t < nt) {
-          const uint4 x = token(t, s);
-          mma_bf16_16816(acc[t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-          mma_bf16_16816(acc[t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
-        }
-    }
-  }
-}
+// A stage of a warp's ring: 256 bytes of each of 16 weight rows, fetched row by row by bulk copies.  Lanes 8 i .. 8 i + 7 read the rows
+// 2 i and 2 i + 1 together, 64 bytes of each: an odd row begins 64 bytes further round the 128 bytes that the banks span.
+constexpr int ROW_BYTES = 256, STAGE_BYTES = 8 * 576;
+__device__ __forceinline__ uint32_t row_at(int r) { return (uint32_t)((r >> 1) * 576 + (r & 1) * 320); }
+// k of a stage, and of a step of the products; tokens' numbers are read 128 k (a scale's block) at a time
+template <bool FP8> struct Depth { static constexpr int ESZ = FP8 ? 1 : 2, STAGE = ROW_BYTES / ESZ, STEP = FP8 ? 64 : 32, STEPS = 128 / STEP; };
 
 // What all pieces of a CTA know of the step, in shared memory.
 struct Lists {
-  int* active;                               // chosen experts, ascending
-  int* first;                                // [active + 1] where an expert's entries begin
+  int* active;                               // chosen experts, ascending; one with more than 16 tokens stands here once for every 16
+  int* first;                                // [active + 1] where their entries begin
   int* slot;                                 // entries: (token, choice) numbers by expert
   int* count;                                // [E] scratch
-  float* total;                              // [WARPS][8 tiles][16 rows] sums of a warp; before that its partial tiles
-  uint32_t ring;                             // this warp's
+  float* total;                              // this warp's sums [tokens][16 rows]; before that its partial tiles
 };
 struct Block {
   int drawn[WARPS];                          // a team's next piece
-  int base, n_active, most, done, piece, stop;
+  int base, n_active, most, done, piece;
+  int stop;                                  // a wait ran out
+};
+constexpr int MOST_COLUMNS = 16;             // tokens that meet a weight at a time
+__host__ __device__ inline int most_active(int n, int E, int top) { return E + n * top / MOST_COLUMNS; }
+// A warp's ring: `stages` slots; running slot and phase of the next stage to fill and to use.
+struct Ring {
+  uint32_t at, bars;
+  uint64_t* bar;
+  int stages, fill, use;
+  uint32_t phase;
 };
 
-template <bool FP8, bool GLU, int T>
-__device__ __forceinline__ void run_layer(const LayerParams& p, const Lists& L, Block& B) {
-  using R = Ring<FP8>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const bool ringed = T <= p.ring_tiles;
-  const uint32_t stage_bytes = A_BYTES + (uint32_t)p.ring_tiles * R::B_PIECES * 512u;
-  const uint32_t my_ring = L.ring + 16u * lane;
-  const int A = B.n_active, ffu = GLU ? 2 * p.ff : p.ff;
-  const int stages = p.stages;
-  const __nv_bfloat16* rows[T];
+// Streams the stages [begin, begin + count) of the weight rows row_lo + 0 .. 7, row_hi + 0 .. 7 of the chosen experts, one expert's
+// after the other's (`per` stages each), through this warp's ring, and multiplies them with the experts' tokens.  `done(a, acc)` is called
+// when the last stage of expert a's share has been added to acc[column tile][4]; acc is cleared afterwards.  `ready()` is called when the
+// first stages have been asked for and before any token is read, `ending()` before the last stage is waited for.
+template <bool FP8, int T, bool DOWN, typename Ready, typename Ending, typename Done>
+__device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Block& B, Ring& R, int begin, int count, int per, int row_lo,
+                                       int row_hi, int rows_all, int K, Ready ready, Ending ending, Done done) {
+  using D = Depth<FP8>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const unsigned char* weights = DOWN ? p.wd : p.wu;
+  const __nv_bfloat16* tokens = DOWN ? p.u : p.h;
+  const void* scales = DOWN ? p.sd : p.su;
+  const int KB = (K + 127) / 128, RB = (rows_all + 127) / 128;
 
-  // ---- up products: a piece is 16 rows of one expert (GLU: 8 gate rows and their 8 up rows), shared by the warps of a team
-  {
-    constexpr int OUT = GLU ? 8 : 16;
-    const int tiles = (p.ff + OUT - 1) / OUT, pieces = A * tiles, depth = (p.d + R::DEPTH - 1) / R::DEPTH;
-    // fewer pieces than warps: a team of 2, 4 or 8 warps cuts a piece's k, as long as each has four stages
-    int team_size = 1;
-    while (team_size < 8 && (long long)pieces * team_size * 2 <= (long long)gridDim.x * WARPS && depth >= 8 * team_size) team_size *= 2;
-    const int team = warp / team_size, member = warp % team_size;
-    const int per = (depth + team_size - 1) / team_size, from = min(depth, member * per), to = min(depth, from + per);
-    if (threadIdx.x == 0) B.base = atomicAdd(p.counters, WARPS / team_size);
-    __syncthreads();
-    int piece = B.base + team, mine = 0;
-    while (piece < pieces) {
-      int next = 0;
-      if (member == 0 && lane == 0) next = atomicAdd(p.counters, 1);
-      const int a = piece / tiles, i0 = (piece - a * tiles) * OUT, e = L.active[a];
-      const int c0 = L.first[a], cnt = L.first[a + 1] - c0, nt = (cnt + 7) / 8;
-      const int r_lo = i0 + g, r_hi = GLU ? p.ff + i0 + g : i0 + 8 + g;
-      const unsigned char* we = p.wu + (size_t)e * ffu * p.d * R::ESZ;
-      const unsigned char* lo = i0 + g < p.ff ? we + (size_t)r_lo * p.d * R::ESZ : nullptr;
-      const unsigned char* hi = (GLU ? i0 + g : i0 + 8 + g) < p.ff ? we + (size_t)r_hi * p.d * R::ESZ : nullptr;
+  // filling: lane r copies row r
+  const int my_row = lane < 8 ? row_lo + lane : row_hi + (lane & 7);
+  const bool copies = lane < 16 && my_row < rows_all;
+  const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies));
+  int fa = begin / per, fs = begin - fa * per, filled = 0;
+  auto fill = [&]() {
+    if (filled < count && !B.stop) {
+      const uint32_t bytes = (uint32_t)min(ROW_BYTES, K * D::ESZ - fs * ROW_BYTES);
+      const uint32_t bar = R.bars + 8u * R.fill;
+      if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * n_copies) : "memory");
+      if (copies)
+        copy_bulk(R.at + (uint32_t)R.fill * STAGE_BYTES + row_at(lane),
+                  weights + ((size_t)L.active[fa] * rows_all + my_row) * (size_t)K * D::ESZ + (size_t)fs * ROW_BYTES, bytes, bar);
+      if (++R.fill == R.stages) R.fill = 0;
+      ++filled;
+      if (++fs == per) { fs = 0; ++fa; }
+    }
+  };
+  // the tokens' numbers: a cursor of its own, one block of 128 k ahead of the products
+  uint4 b[T][4];
+  int rows[T];
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto enter = [&](int a) {                   // rows of expert a's tokens, column g of every tile
+    const int c0 = L.first[a], cnt = L.first[a + 1] - c0;
 #pragma unroll
-      for (int t = 0; t < T; ++t) rows[t] = 8 * t + g < cnt ? p.h + (size_t)(L.slot[c0 + 8 * t + g] / p.top) * p.d : nullptr;
-      float acc[T][4];
+    for (int t = 0; t < T; ++t) {
+      const int slot = 8 * t + g < cnt ? L.slot[c0 + 8 * t + g] : -1;
+      rows[t] = DOWN || slot < 0 ? slot : slot / p.top;
+    }
+  };
+  // piece i of a block: bfloat16 weights meet k 32 i + 8 q, 8-bit ones 64 (i / 2) + 16 q + 8 (i % 2)
+  auto piece = [&](int t, int k0, int i) -> uint4 {
+    const int k = FP8 ? k0 + 64 * (i >> 1) + 16 * q + 8 * (i & 1) : k0 + 32 * i + 8 * q;
+    if (rows[t] < 0 || k >= K) return zero;
+    const uint4* from = reinterpret_cast<const uint4*>(tokens + (size_t)rows[t] * K + k);
+    return DOWN ? __ldcg(from) : __ldg(from);
+  };
+  float acc[T][4];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+
+  for (int i = 0; i < R.stages; ++i) fill();
+  ready();
+  int a = begin / per, s = begin - a * per;
+  if (count > 0) {
+    enter(a);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[t][i] = piece(t, s * D::STAGE, i);
+  }
+  float s_lo = 1.f, s_hi = 1.f;
+  for (int j = 0; j < count; ++j) {
+    const int c0 = L.first[a], nt = (L.first[a + 1] - c0 + 7) / 8;
+    const bool last_stage = s + 1 == per;
+    if (j + 1 == count) ending();
+    bool ok = !B.stop;
+    if (ok) ok = mbar_wait(R.bar + R.use, R.phase, &B.stop, p.status, 112);
+    const uint32_t at = R.at + (uint32_t)R.use * STAGE_BYTES + row_at(g) + 16u * q;
+    if (++R.use == R.stages) { R.use = 0; R.phase ^= 1u; }
+#pragma unroll
+    for (int blk = 0; blk < D::STAGE / 128; ++blk) {
+      const int k0 = s * D::STAGE + 128 * blk;
+      if (k0 >= K) break;
+      if (FP8) {
+        s_lo = block_scale(scales, p.e8m0, ((size_t)L.active[a] * RB + min(row_lo + g, rows_all - 1) / 128) * KB + k0 / 128);
+        s_hi = block_scale(scales, p.e8m0, ((size_t)L.active[a] * RB + min(row_hi + g, rows_all - 1) / 128) * KB + k0 / 128);
+      }
+      // where the next block's tokens lie; each piece is asked for when the one before it in its registers has been used
+      int next_k = -1;
+      if (blk + 1 < D::STAGE / 128 && k0 + 128 < K) {
+        next_k = k0 + 128;
+      } else if (j + 1 < count) {
+        next_k = last_stage ? 0 : (s + 1) * D::STAGE;
+        if (last_stage) enter(a + 1);
+      }
+      float sum[FP8 ? T : 1][4];
+      if (FP8) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
+      }
+#pragma unroll
+      for (int st = 0; st < D::STEPS; ++st) {
+        const int ks = k0 + st * D::STEP;
+        if (ks < K) {
+          uint4 lo = lds16(at + (uint32_t)(blk * D::STEPS + st) * 64u), hi = lds16(at + (uint32_t)(blk * D::STEPS + st) * 64u + 4 * 576);
+          if (ks + D::STEP > K && ks + (16 / D::ESZ) * q >= K) lo = hi = zero;    // behind the rows' ends: what an earlier stage left
+          if (FP8) {
+            const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
+            uint32_t wl[8], wh[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              widen4(l[i], wl[2 * i], wl[2 * i + 1]);
+              widen4(h[i], wh[2 * i], wh[2 * i + 1]);
+            }
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+              if (t < nt) {
+                const uint4 x = b[t][2 * st];
+                const uint4 y = b[t][2 * st + 1];
+                mma_bf16_16816(sum[t], wl[0], wh[0], wl[1], wh[1], x.x, x.y);
+                mma_bf16_16816(sum[t], wl[2], wh[2], wl[3], wh[3], x.z, x.w);
+                mma_bf16_16816(sum[t], wl[4], wh[4], wl[5], wh[5], y.x, y.y);
+                mma_bf16_16816(sum[t], wl[6], wh[6], wl[7], wh[7], y.z, y.w);
+              }
+          } else {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+              if (t < nt) {
+                const uint4 x = b[t][st];
+                mma_bf16_16816(acc[t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+                mma_bf16_16816(acc[t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+              }
+          }
+        }
+        if (next_k >= 0) {
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4 / D::STEPS; ++i) b[t][4 / D::STEPS * st + i] = piece(t, next_k, 4 / D::STEPS * st + i);
+        }
+      }
+      if (FP8) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          acc[t][0] = fmaf(sum[t][0], s_lo, acc[t][0]);
+          acc[t][1] = fmaf(sum[t][1], s_lo, acc[t][1]);
+          acc[t][2] = fmaf(sum[t][2], s_hi, acc[t][2]);
+          acc[t][3] = fmaf(sum[t][3], s_hi, acc[t][3]);
+        }
+      }
+    }
+    __syncwarp();                             // every lane has read the stage
+    fill();
+    if (last_stage || j + 1 == count) {
+      done(a, acc);
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-      const int KB = (p.d + 127) / 128, RB = (ffu + 127) / 128;
-      const size_t s_lo_at = ((size_t)e * RB + min(r_lo, ffu - 1) / 128) * KB, s_hi_at = ((size_t)e * RB + min(r_hi, ffu - 1) / 128) * KB;
-      auto fetch = [&](int j) {
-        if (j < to) {
-          const uint32_t at = my_ring + (uint32_t)((j - from) % stages) * stage_bytes;
-          fetch_weights<FP8>(at, lo, hi, we, j * R::DEPTH, p.d);
-          if (ringed) {
+    }
+    ++s;
+    if (last_stage) { s = 0; ++a; }
+  }
+}
+
+template <bool FP8, bool GLU, int T>
+__device__ __forceinline__ void run_layer(const LayerParams& p, const Lists& L, Block& B, Ring& R) {
+  using D = Depth<FP8>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int A = B.n_active, ffu = GLU ? 2 * p.ff : p.ff, warp_total = (p.n + 7) / 8 * 128;
+
+  // ---- up products: a piece is 16 rows of one expert (GLU: 8 gate rows and their 8 up rows), shared by the warps of a team
+  constexpr int OUT = GLU ? 8 : 16;
+  const int tiles = (p.ff + OUT - 1) / OUT, pieces = A * tiles, depth = (p.d + D::STAGE - 1) / D::STAGE;
+  // a team of 2 or 4 warps cuts a piece's k, as long as each has four stages: short pieces end at about the same time everywhere
+  const int team_size = depth >= 16 ? 4 : (depth >= 8 ? 2 : 1);
+  const int team = warp / team_size, member = warp % team_size;
+  const int per = (depth + team_size - 1) / team_size, from = min(depth, member * per), to = min(depth, from + per);
+  if (threadIdx.x == 0) B.base = atomicAdd(p.counters, WARPS / team_size);
+  __syncthreads();
+  int piece = B.base + team, mine = 0;
+  while (piece < pieces) {
+    int next = 0;
+    const int a = piece / tiles, i0 = (piece - a * tiles) * OUT, c0 = L.first[a], cnt = L.first[a + 1] - c0, nt = (cnt + 7) / 8;
+    float part[T][4];
 #pragma unroll
-            for (int t = 0; t < T; ++t)
-              if (t < nt) fetch_tokens<FP8, true>(at + A_BYTES + t * R::B_PIECES * 512, rows[t], we, j * R::DEPTH, p.d);
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[t][i] = 0.f;
+    stream<FP8, T, false>(p, L, B, R, a * depth + from, to - from, depth, i0, GLU ? p.ff + i0 : i0 + 8, ffu, p.d, []() {},
+                          [&]() {             // not earlier: a CTA that starts first would take the others' first pieces
+                            if (member == 0 && lane == 0) next = atomicAdd(p.counters, 1);
+                          },
+                          [&](int, float (&acc)[T][4]) {
+#pragma unroll
+                            for (int t = 0; t < T; ++t)
+#pragma unroll
+                              for (int i = 0; i < 4; ++i) part[t][i] = acc[t][i];
+                          });
+    if (team_size > 1) {
+      if (member != 0) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+          if (t < nt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) L.total[(t * 4 + i) * 32 + lane] = part[t][i];
           }
-        }
-        cp_commit();
-      };
-      float s_lo = 1.f, s_hi = 1.f;
-      if (FP8 && from < to) {
-        s_lo = block_scale(p.su, p.e8m0, s_lo_at + from);
-        s_hi = block_scale(p.su, p.e8m0, s_hi_at + from);
       }
-      for (int j = 0; j < stages - 1; ++j) fetch(from + j);
-      for (int j = from; j < to; ++j) {
-        fetch(j + stages - 1);
-        cp_wait(stages - 1);
-        float n_lo = 1.f, n_hi = 1.f;
-        if (FP8 && j + 1 < to) {
-          n_lo = block_scale(p.su, p.e8m0, s_lo_at + j + 1);
-          n_hi = block_scale(p.su, p.e8m0, s_hi_at + j + 1);
-        }
-        const uint32_t at = my_ring + (uint32_t)((j - from) % stages) * stage_bytes;
-        multiply<FP8, T>(at, ringed ? at + A_BYTES : 0u, rows, j * R::DEPTH, p.d, nt, s_lo, s_hi, acc);
-        s_lo = n_lo;
-        s_hi = n_hi;
-      }
-      cp_wait(0);
-      if (team_size > 1) {
-        float* red = L.total + (size_t)warp * T * 128;
-        if (member != 0) {
+      if (member == 0 && lane == 0) B.drawn[team] = next;
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
+      if (member == 0) {
+        for (int m = 1; m < team_size; ++m)
 #pragma unroll
           for (int t = 0; t < T; ++t)
             if (t < nt) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) red[(t * 4 + i) * 32 + lane] = acc[t][i];
+              for (int i = 0; i < 4; ++i) part[t][i] += L.total[m * warp_total + (t * 4 + i) * 32 + lane];
             }
-        }
-        if (member == 0 && lane == 0) B.drawn[team] = next;
-        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
-        if (member == 0) {
-          for (int m = 1; m < team_size; ++m)
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-              if (t < nt) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][i] += red[(size_t)m * T * 128 + (t * 4 + i) * 32 + lane];
-              }
-        }
-        next = B.drawn[team];
-        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
-      } else {
-        next = __shfl_sync(0xffffffffu, next, 0);
       }
-      if (member == 0) {
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int c = 8 * t + 2 * q + i;
-            if (c >= cnt) continue;
-            __nv_bfloat16* u = p.u + (size_t)L.slot[c0 + c] * p.ff + i0 + g;
-            if (GLU) {
-              const float gv = acc[t][i];
-              if (i0 + g < p.ff) *u = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * acc[t][2 + i]);
-            } else {
-              if (i0 + g < p.ff) u[0] = __float2bfloat16_rn(gelu_erf(acc[t][i]));
-              if (i0 + 8 + g < p.ff) u[8] = __float2bfloat16_rn(gelu_erf(acc[t][2 + i]));
-            }
-          }
-        ++mine;
-      }
-      piece = next;
+      next = B.drawn[team];
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
+    } else {
+      next = __shfl_sync(0xffffffffu, next, 0);
     }
-    if (member == 0 && lane == 0 && mine) atomicAdd(&B.done, mine);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      if (B.done) {
-        __threadfence();
-        atomicAdd(p.counters + 1, B.done);
-      }
-      B.piece = atomicAdd(p.counters + 2, 1);
-    }
-    __syncthreads();
-    // ---- down products: a piece is 16 output columns over all chosen experts; the warps take equal shares of the (expert, k) stages
-    const int out_pieces = (p.d + 15) / 16, per_expert = (p.ff + R::DEPTH - 1) / R::DEPTH;
-    const int all = A * per_expert, w0 = (int)((long long)all * warp / WARPS), w1 = (int)((long long)all * (warp + 1) / WARPS);
-    const int KB = (p.ff + 127) / 128, RB = (p.d + 127) / 128;
-    float* total = L.total + (size_t)warp * 8 * T * 16;          // [tokens][16]
-    bool first = true;
-    while (B.piece < out_pieces) {
-      const int n0 = B.piece * 16;
-      for (int i = lane; i < p.n * 16; i += 32) total[i] = 0.f;
-      __syncwarp();
-      const bool live_lo = n0 + g < p.d, live_hi = n0 + 8 + g < p.d;
-      auto fetch_w = [&](int j) {
-        const int a = j / per_expert, k0 = (j - a * per_expert) * R::DEPTH;
-        const unsigned char* we = p.wd + (size_t)L.active[a] * p.d * p.ff * R::ESZ;
-        const unsigned char* lo = live_lo ? we + (size_t)(n0 + g) * p.ff * R::ESZ : nullptr;
-        const unsigned char* hi = live_hi ? we + (size_t)(n0 + 8 + g) * p.ff * R::ESZ : nullptr;
-        fetch_weights<FP8>(my_ring + (uint32_t)((j - w0) % stages) * stage_bytes, lo, hi, we, k0, p.ff);
-      };
-      auto fetch_u = [&](int j) {
-        if (!ringed) return;
-        const int a = j / per_expert, k0 = (j - a * per_expert) * R::DEPTH;
-        const int c0 = L.first[a], cnt = L.first[a + 1] - c0;
-        const uint32_t at = my_ring + (uint32_t)((j - w0) % stages) * stage_bytes + A_BYTES;
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-          if (8 * t < cnt)
-            fetch_tokens<FP8, false>(at + t * R::B_PIECES * 512, 8 * t + g < cnt ? p.u + (size_t)L.slot[c0 + 8 * t + g] * p.ff : nullptr,
-                                     p.u, k0, p.ff);
-      };
-      // the first weights are asked for before the wait for the up products
-      for (int j = w0; j < min(w1, w0 + stages - 1); ++j) fetch_w(j);
-      if (first) {
-        first = false;
-        if (threadIdx.x == 0) {
-          unsigned long long t_from = 0ull;
-          for (uint32_t i = 0;; ++i) {
-            int v;
-            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.counters + 1) : "memory");
-            if (v >= pieces) break;
-            if ((i & 255u) == 255u) {
-              const unsigned long long now = bspec::global_timer();
-              if (t_from == 0ull) t_from = now;
-              if (now - t_from > 2000000000ull || i >= (1u << 24) || *reinterpret_cast<volatile int*>(p.status) != 0) {
-                atomicCAS(p.status, 0, 111);
-                B.stop = 1;
-                break;
-              }
-            }
-          }
-          __threadfence();
-        }
-        __syncthreads();
-        if (B.stop) break;
-      }
-      for (int j = w0; j < w0 + stages - 1; ++j) {
-        if (j < w1) fetch_u(j);
-        cp_commit();
-      }
-      float acc[T][4];
+    if (member == 0) {
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-      int a = w0 < w1 ? w0 / per_expert : 0, kb = w0 - a * per_expert;
-      int c0 = 0, cnt = 0;
-      const __nv_bfloat16* at_rows[T];
-      auto enter = [&]() {
-        c0 = L.first[a];
-        cnt = L.first[a + 1] - c0;
-#pragma unroll
-        for (int t = 0; t < T; ++t) at_rows[t] = 8 * t + g < cnt ? p.u + (size_t)L.slot[c0 + 8 * t + g] * p.ff : nullptr;
-      };
-      auto scale_of = [&](int aa, int k, int row) {
-        return block_scale(p.sd, p.e8m0, ((size_t)L.active[aa] * RB + min(row, p.d - 1) / 128) * KB + k);
-      };
-      float s_lo = 1.f, s_hi = 1.f;
-      if (w0 < w1) {
-        enter();
-        if (FP8) s_lo = scale_of(a, kb, n0 + g), s_hi = scale_of(a, kb, n0 + 8 + g);
-      }
-      for (int j = w0; j < w1; ++j) {
-        if (j + stages - 1 < w1) {
-          fetch_w(j + stages - 1);
-          fetch_u(j + stages - 1);
+        for (int i = 0; i < 2; ++i) {
+          const int c = 8 * t + 2 * q + i;
+          if (c >= cnt) continue;
+          __nv_bfloat16* u = p.u + (size_t)L.slot[c0 + c] * p.ff + i0 + g;
+          if (GLU) {
+            const float gv = part[t][i];
+            if (i0 + g < p.ff) *u = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * part[t][2 + i]);
+          } else {
+            if (i0 + g < p.ff) u[0] = __float2bfloat16_rn(gelu_erf(part[t][i]));
+            if (i0 + 8 + g < p.ff) u[8] = __float2bfloat16_rn(gelu_erf(part[t][2 + i]));
+          }
         }
-        cp_commit();
-        cp_wait(stages - 1);
-        float n_lo = 1.f, n_hi = 1.f;
-        const bool last = kb + 1 == per_expert;
-        if (FP8 && j + 1 < w1) {
-          n_lo = scale_of(last ? a + 1 : a, last ? 0 : kb + 1, n0 + g);
-          n_hi = scale_of(last ? a + 1 : a, last ? 0 : kb + 1, n0 + 8 + g);
-        }
-        const uint32_t at = my_ring + (uint32_t)((j - w0) % stages) * stage_bytes;
-        multiply<FP8, T>(at, ringed ? at + A_BYTES : 0u, at_rows, kb * R::DEPTH, p.ff, (cnt + 7) / 8, s_lo, s_hi, acc);
-        s_lo = n_lo;
-        s_hi = n_hi;
-        ++kb;
-        if (last || j + 1 == w1) {
-          // this expert's share is complete: into the warp's sums, weighted
-#pragma unroll
-          for (int t = 0; t < T; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int c = 8 * t + 2 * q + i;
-              if (c < cnt) {
-                const int slot = L.slot[c0 + c];
-                const float w = p.wts[slot];
-                float* to = total + slot / p.top * 16 + g;
-                to[0] = fmaf(w, acc[t][i], to[0]);
-                to[8] = fmaf(w, acc[t][2 + i], to[8]);
-              }
-              acc[t][i] = acc[t][2 + i] = 0.f;
-            }
-          __syncwarp();
-          if (last && j + 1 < w1) {
-            ++a;
-            kb = 0;
-            enter();
+      ++mine;
+    }
+    piece = next;
+  }
+  if (member == 0 && lane == 0 && mine) atomicAdd(&B.done, mine);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (B.done) {
+      __threadfence();
+      atomicAdd(p.counters + 1, B.done);
+    }
+    B.piece = atomicAdd(p.counters + 2, 1);
+  }
+  __syncthreads();
+  // ---- down products: a piece is 16 output columns over all chosen experts; the warps take equal shares of the (expert, k) stages
+  const int out_pieces = (p.d + 15) / 16, per_expert = (p.ff + D::STAGE - 1) / D::STAGE;
+  const int all = A * per_expert, w0 = (int)((long long)all * warp / WARPS), w1 = (int)((long long)all * (warp + 1) / WARPS);
+  bool waited = false;
+  auto up_done = [&]() {                      // every up piece of every CTA is done
+    if (waited) return;
+    waited = true;
+    if (threadIdx.x == 0) {
+      unsigned long long t_from = 0ull;
+      for (uint32_t i = 0; !B.stop; ++i) {
+        int v;
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.counters + 1) : "memory");
+        if (v >= pieces) break;
+        if ((i & 255u) == 255u) {
+          const unsigned long long now = bspec::global_timer();
+          if (t_from == 0ull) t_from = now;
+          if (now - t_from > WAIT_NS || i >= WAIT_LIMIT || *reinterpret_cast<volatile int*>(p.status) != 0) {
+            atomicCAS(p.status, 0, 111);
+            B.stop = 1;
           }
         }
       }
-      cp_wait(0);
-      __syncthreads();
-      if (threadIdx.x == 0) B.base = atomicAdd(p.counters + 2, 1);
+      __threadfence();
+    }
+    __syncthreads();
+  };
+  while (B.piece < out_pieces) {
+    const int n0 = B.piece * 16;
+    for (int i = lane; i < p.n * 16; i += 32) L.total[i] = 0.f;
+    __syncwarp();
+    stream<FP8, T, true>(p, L, B, R, w0, w1 - w0, per_expert, n0, n0 + 8, p.d, p.ff, up_done, []() {}, [&](int a, float (&acc)[T][4]) {
+      const int c0 = L.first[a], cnt = L.first[a + 1] - c0;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = 8 * t + 2 * q + i;
+          if (c >= cnt) continue;
+          const int slot = L.slot[c0 + c];
+          const float w = p.wts[slot];
+          float* to = L.total + slot / p.top * 16 + g;
+          to[0] = fmaf(w, acc[t][i], to[0]);
+          to[8] = fmaf(w, acc[t][2 + i], to[8]);
+        }
+      __syncwarp();
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) B.base = atomicAdd(p.counters + 2, 1);
+    const float* totals = L.total - warp * warp_total;
+    if (!B.stop)
       for (int i = threadIdx.x; i < p.n * 16; i += LAYER_THREADS) {
         const int t = i >> 4, col = n0 + (i & 15);
         if (col >= p.d) continue;
@@ -526,40 +487,54 @@ __device__ __forceinline__ void run_layer(const LayerParams& p, const Lists& L, 
           if (p.gate != nullptr) v *= 1.f / (1.f + expf(-p.gate[t]));
         }
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) v += L.total[(size_t)w * 8 * T * 16 + i];
+        for (int w = 0; w < WARPS; ++w) v += totals[w * warp_total + i];
         for (int k = 0; k < p.top; ++k)
           if (p.ids[(size_t)t * p.top + k] >= p.E) v = fmaf(p.wts[(size_t)t * p.top + k], to_f32(p.h[(size_t)t * p.d + col]), v);
         p.out[(size_t)t * p.d + col] = __float2bfloat16_rn(v);
       }
-      __syncthreads();
-      if (threadIdx.x == 0) B.piece = B.base;
-      __syncthreads();
-    }
-    cp_wait(0);
+    __syncthreads();
+    if (threadIdx.x == 0) B.piece = B.base;
+    __syncthreads();
   }
+  // after a wait that ran out: copies in flight land (they take microseconds) before the shared memory is given up
+  if (B.stop)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
+
+// bytes of shared memory for the sums, the rings and the lists; a CTA's static shared memory comes on top
+__host__ __device__ inline size_t layer_smem(int n, int E, int top, int stages) {
+  return (size_t)WARPS * ((n + 7) / 8 * 128 * 4 + stages * STAGE_BYTES) + ((size_t)n * top + 2 * (size_t)most_active(n, E, top) + 1 + E) * 4;
+}
+constexpr int MAX_STAGES = 4;
 
 template <bool FP8, bool GLU>
 __global__ void __launch_bounds__(LAYER_THREADS, 1) moe_layer_experts_kernel(LayerParams p) {
-  bspec::pdl_prologue(85);
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Block B;
-  const int slots = p.n * p.top, tiles = (p.n + 7) / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int T = tiles <= 1 ? 1 : (tiles <= 2 ? 2 : 8);           // sizes of the sums: as many column tiles as the tokens can fill
+  __shared__ uint64_t bars[WARPS * MAX_STAGES];
+  const int slots = p.n * p.top, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < WARPS * MAX_STAGES) mbar_init(bars + threadIdx.x, 1);
+  if (threadIdx.x == 0) B.done = B.stop = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   Lists L;
-  L.total = reinterpret_cast<float*>(smem);
-  unsigned char* at = smem + (size_t)WARPS * 8 * T * 16 * 4;
-  const uint32_t warp_ring = (uint32_t)p.stages * (A_BYTES + (uint32_t)p.ring_tiles * Ring<FP8>::B_PIECES * 512u);
-  L.ring = smem_addr(at) + warp * warp_ring;
-  at += (size_t)WARPS * warp_ring;
+  Ring R;
+  R.at = s32(smem) + (uint32_t)(warp * p.stages) * STAGE_BYTES;
+  R.bar = bars + warp * MAX_STAGES;
+  R.bars = s32(R.bar);
+  R.stages = p.stages;
+  R.fill = R.use = 0;
+  R.phase = 0u;
+  unsigned char* at = smem + (size_t)WARPS * p.stages * STAGE_BYTES;
+  L.total = reinterpret_cast<float*>(at) + (size_t)warp * ((p.n + 7) / 8 * 128);
+  at += (size_t)WARPS * ((p.n + 7) / 8 * 128) * 4;
   L.slot = reinterpret_cast<int*>(at);
   L.active = L.slot + slots;
-  L.first = L.active + p.E;
-  L.count = L.first + p.E + 1;
-  // the entries by expert: counted, placed (in any order within an expert: a column's sums do not depend on its place)
+  L.first = L.active + most_active(p.n, p.E, p.top);
+  L.count = L.first + most_active(p.n, p.E, p.top) + 1;
   for (int e = threadIdx.x; e < p.E; e += LAYER_THREADS) L.count[e] = 0;
-  if (threadIdx.x == 0) B.done = B.stop = 0;
   __syncthreads();
+  bspec::pdl_prologue(85);
+  // the entries by expert: counted, then placed
   for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
     const int e = p.ids[s];
     if (e < p.E) atomicAdd(L.count + e, 1);
@@ -568,57 +543,46 @@ __global__ void __launch_bounds__(LAYER_THREADS, 1) moe_layer_experts_kernel(Lay
   if (warp == 0) {
     int n_active = 0, run = 0, most = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane, c = e < p.E ? L.count[e] : 0;
-      int upto = c;
+      const int e = e0 + lane, c = e < p.E ? L.count[e] : 0, groups = (c + MOST_COLUMNS - 1) / MOST_COLUMNS;
+      int upto = c, upto_g = groups;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        const int v = __shfl_up_sync(0xffffffffu, upto, o), w = __shfl_up_sync(0xffffffffu, upto_g, o);
+        if (lane >= o) upto += v, upto_g += w;
       }
-      const unsigned mask = __ballot_sync(0xffffffffu, c > 0);
-      const int at_a = n_active + __popc(mask & ((1u << lane) - 1u));
-      if (c > 0) {
-        L.active[at_a] = e;
-        L.first[at_a] = run + upto - c;
-        L.count[e] = run + upto - c;                              // where the next entry of this expert goes
+      const int from = run + upto - c;
+      for (int i = 0; i < groups; ++i) {
+        L.active[n_active + upto_g - groups + i] = e;
+        L.first[n_active + upto_g - groups + i] = from + i * MOST_COLUMNS;
       }
+      if (c > 0) L.count[e] = from;                               // where the next entry of this expert goes
       most = max(most, c);
-      n_active += __popc(mask);
+      n_active += __shfl_sync(0xffffffffu, upto_g, 31);
       run += __shfl_sync(0xffffffffu, upto, 31);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
       L.first[n_active] = run;
       B.n_active = n_active;
       B.most = most;
     }
-  }
-  __syncthreads();
-  for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
-    const int e = p.ids[s];
-    if (e < p.E) L.slot[atomicAdd(L.count + e, 1)] = s;
-  }
-  __syncthreads();
-  if (T == 1) run_layer<FP8, GLU, 1>(p, L, B);
-  else if (T == 2) run_layer<FP8, GLU, 2>(p, L, B);
-  else run_layer<FP8, GLU, 8>(p, L, B);
-}
-
-template <bool FP8>
-size_t layer_smem(int n, int E, int top, int* stages, int* ring_tiles) {
-  const int tiles = (n + 7) / 8, T = tiles <= 1 ? 1 : (tiles <= 2 ? 2 : 8);
-  const size_t fixed = (size_t)WARPS * 8 * T * 16 * 4 + ((size_t)n * top + 3 * (size_t)E + 1) * 4;
-  // the tokens' numbers ride in the ring while two stages of it fit
-  for (int rt = T < 8 ? T : 0;; rt = 0) {
-    const size_t stage = (size_t)WARPS * (A_BYTES + rt * Ring<FP8>::B_PIECES * 512);
-    const long long st = ((long long)SMEM_BUDGET - (long long)fixed) / (long long)stage;
-    if (st >= 2 || rt == 0) {
-      *ring_tiles = rt;
-      *stages = st > 4 ? 4 : (int)st;
-      return st < 2 ? 0 : fixed + (size_t)*stages * stage;
+    __syncwarp();
+    // placed in the order of their numbers, so that every CTA has the same ones in an expert's first 16
+    for (int s0 = 0; s0 < slots; s0 += 32) {
+      const int s = s0 + lane, e = s < slots ? p.ids[s] : p.E;
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      if (e < p.E) {
+        const int from = L.count[e];
+        L.slot[from + __popc(same & ((1u << lane) - 1u))] = s;
+        __syncwarp(same);
+        if (lane == __ffs(same) - 1) L.count[e] = from + __popc(same);
+      }
+      __syncwarp();
     }
   }
+  __syncthreads();
+  if (B.most <= 8) run_layer<FP8, GLU, 1>(p, L, B, R);
+  else run_layer<FP8, GLU, 2>(p, L, B, R);
 }
 
 }  // namespace
@@ -637,7 +601,7 @@ BSPEC_API int bspec_moe_layer_route(const void* h, int n, int d, const void* rou
   int slices = ROUTE_CLUSTER * ROUTE_WARPS / tiles;              // of k: as many as there are warps left
   if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;        // at least one batch of loads each
   if (slices < 1) slices = 1;
-  const size_t smem = ((size_t)tiles * slices * 16 * ROUTE_TOKENS + (size_t)ROUTE_WARPS * 3 * C) * 4;
+  const size_t smem = ((size_t)tiles * slices * 16 * ROUTE_TOKENS + (size_t)(ROUTE_WARPS * 3 + 1) * C) * 4;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(moe_layer_route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return (int)e;
@@ -664,8 +628,10 @@ BSPEC_API int bspec_moe_layer_experts(const void* h, int n, int d, const void* w
   p.su = su; p.sd = sd; p.e8m0 = e8m0; p.ids = ids; p.wts = wts; p.gate = gate; p.add = (const __nv_bfloat16*)add;
   p.u = (__nv_bfloat16*)u; p.out = (__nv_bfloat16*)out; p.counters = counters; p.status = status;
   p.n = n; p.d = d; p.ff = ff; p.E = E; p.top = top;
-  const size_t smem = fp8 ? layer_smem<true>(n, E, top, &p.stages, &p.ring_tiles) : layer_smem<false>(n, E, top, &p.stages, &p.ring_tiles);
-  if (smem == 0) return (int)cudaErrorInvalidValue;
+  p.stages = 2;
+  while (p.stages < MAX_STAGES && layer_smem(n, E, top, p.stages + 1) <= SMEM_BUDGET) ++p.stages;
+  const size_t smem = layer_smem(n, E, top, p.stages);
+  if (smem > SMEM_BUDGET) return (int)cudaErrorInvalidValue;
 #define LE(F, G)                                                                                                          \
   do {                                                                                                                    \
     static bool set_dev[bspec::kMaxDevices] = {};                                                                         \

@@ -1255,7 +1255,7 @@ WAIT_CODES = ((1, 1, "GEMM: stage never freed"), (2, 2, "GEMM: operands never ar
               (91, 91, "float32 product of few rows: stage never freed"),
               (92, 92, "float32 product of few rows: operands never arrived"),
               (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"),
-              (111, 111, "routed layer of a few tokens: the up products never completed"))
+              (111, 112, "routed layer of a few tokens: the up products never completed, or weights never arrived"))
 
 
 def wait_meaning(code: int) -> str:
