@@ -18,6 +18,22 @@ __device__ __forceinline__ void route_score(int rule, float z, float b, float* s
   *choice = softmax_top ? s : s + b;
 }
 
+// The index of the best of v[0 .. n) (the larger value, the lower index among equals; NaN: taken) or 0x7fffffff, by one warp: every lane
+// scans its share, two reductions over the lanes find the largest value, in the order of its bits, and the lowest index that holds it.
+// A function of its own: what is executed once per token costs the fetch of its instructions more than anything else.
+static __device__ __noinline__ int best_of(const float* v, int n) {
+  unsigned bv = 0u;
+  int bi = 0x7fffffff;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    const float x = v[i] + 0.f;                  // one zero
+    const unsigned b = __float_as_uint(x), key = isnan(x) ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
+    if (key > bv) { bv = key; bi = i; }
+  }
+  const unsigned most = __reduce_max_sync(0xffffffffu, bv);
+  return most == 0u ? 0x7fffffff : __reduce_min_sync(0xffffffffu, bv == most ? bi : 0x7fffffff);
+}
+
 // One warp chooses the `top` experts of a token and their weights.  sc, ch [E]: scores and choice scores of route_score, in
 // shared memory (changed); hs: room for G numbers.  DISTINCT: where no number is left to compare (NaN logits), the lowest
 // expert not taken yet instead of expert 0, so that a token never has an expert twice.
@@ -41,19 +57,6 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
     }
     __syncwarp();
   }
-  // Every lane scans its share of the candidates; the best (the larger value, the lower index among equals) is found by two
-  // reductions over the lanes, of the values in the order of their bits and of the indices that hold the largest.  NaN: taken.
-  auto best_of = [&](const float* v, int n) -> int {
-    unsigned bv = 0u;
-    int bi = 0x7fffffff;
-    for (int i = lane; i < n; i += 32) {
-      const float x = v[i] + 0.f;                  // one zero
-      const unsigned b = __float_as_uint(x), key = isnan(x) ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
-      if (key > bv) { bv = key; bi = i; }
-    }
-    const unsigned most = __reduce_max_sync(0xffffffffu, bv);
-    return most == 0u ? 0x7fffffff : __reduce_min_sync(0xffffffffu, bv == most ? bi : 0x7fffffff);
-  };
   if (G > 1 && keep < G) {
     const int per = E / G;
     for (int g = lane; g < G; g += 32) {          // group scores
@@ -65,6 +68,7 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
       hs[g] = per > 1 && !(rule & ROUTE_GROUP_MAX) ? a + b : a;
     }
     __syncwarp();
+#pragma unroll 1
     for (int k = 0; k < keep; ++k) {
       const int best = best_of(hs, G);
       if (lane == 0 && best != 0x7fffffff) hs[best] = NAN;      // NaN marks a kept group
@@ -76,6 +80,7 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
   }
   // Lane k keeps choice k (and k + 32 ...: `top` beyond the lanes goes through memory); sums run over the choices in their order.
   int mine = 0;
+#pragma unroll 1
   for (int k = 0; k < top; ++k) {
     int best = best_of(ch, E);
     if (best == 0x7fffffff) {

@@ -184,47 +184,56 @@ __device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Blo
                                        int row_hi, int rows_all, int K, Ready ready, Ending ending, Done done) {
   using D = Depth<FP8>;
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const unsigned char* weights = DOWN ? p.wd : p.wu;
-  const __nv_bfloat16* tokens = DOWN ? p.u : p.h;
-  const void* scales = DOWN ? p.sd : p.su;
+  const __nv_bfloat16* const tokens = DOWN ? p.u : p.h;
   const int KB = (K + 127) / 128, RB = (rows_all + 127) / 128;
+  const uint32_t row_bytes = (uint32_t)K * D::ESZ;
 
-  // filling: lane r copies row r
+  // filling: lane r copies row r; a running source, set anew where the next expert begins
   const int my_row = lane < 8 ? row_lo + lane : row_hi + (lane & 7);
   const bool copies = lane < 16 && my_row < rows_all;
   const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies));
-  int fa = begin / per, fs = begin - fa * per, filled = 0;
+  const uint32_t last_bytes = row_bytes - (uint32_t)(per - 1) * ROW_BYTES, my_slot = R.at + row_at(lane);
+  int a = begin / per, s = begin - a * per, fa = a, f_left = per - s, to_fill = count;
+  const unsigned char* src = nullptr;
+  auto open = [&](int from) { src = (DOWN ? p.wd : p.wu) + ((size_t)L.active[fa] * rows_all + my_row) * row_bytes + (size_t)from * ROW_BYTES; };
   auto fill = [&]() {
-    if (filled < count && !B.stop) {
-      const uint32_t bytes = (uint32_t)min(ROW_BYTES, K * D::ESZ - fs * ROW_BYTES);
-      const uint32_t bar = R.bars + 8u * R.fill;
-      if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * n_copies) : "memory");
-      if (copies)
-        copy_bulk(R.at + (uint32_t)R.fill * STAGE_BYTES + row_at(lane),
-                  weights + ((size_t)L.active[fa] * rows_all + my_row) * (size_t)K * D::ESZ + (size_t)fs * ROW_BYTES, bytes, bar);
-      if (++R.fill == R.stages) R.fill = 0;
-      ++filled;
-      if (++fs == per) { fs = 0; ++fa; }
+    if (to_fill == 0) return;
+    const uint32_t bytes = f_left == 1 ? last_bytes : (uint32_t)ROW_BYTES, bar = R.bars + 8u * R.fill;
+    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * n_copies) : "memory");
+    if (copies) copy_bulk(my_slot + (uint32_t)R.fill * STAGE_BYTES, src, bytes, bar);
+    if (++R.fill == R.stages) R.fill = 0;
+    src += ROW_BYTES;
+    --to_fill;
+    if (--f_left == 0 && to_fill > 0) {
+      ++fa;
+      f_left = per;
+      open(0);
     }
   };
-  // the tokens' numbers: a cursor of its own, one block of 128 k ahead of the products
+  // the tokens' numbers: a cursor of its own, one block of 128 k ahead of the products; a column without a token reads its neighbour's
+  constexpr int Q_STEP = FP8 ? 16 : 8;
   uint4 b[T][4];
-  int rows[T];
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  auto enter = [&](int a) {                   // rows of expert a's tokens, column g of every tile
-    const int c0 = L.first[a], cnt = L.first[a + 1] - c0;
+  const __nv_bfloat16* from[T];
+  int tiles = 0;                              // column tiles of the expert that the cursor is in
+  auto enter = [&](int at, int k) {
+    const int c0 = L.first[at], cnt = L.first[at + 1] - c0;
+    tiles = (cnt + 7) >> 3;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const int slot = 8 * t + g < cnt ? L.slot[c0 + 8 * t + g] : -1;
-      rows[t] = DOWN || slot < 0 ? slot : slot / p.top;
+      const int slot = L.slot[c0 + min(8 * t + g, cnt - 1)];
+      from[t] = tokens + (size_t)(DOWN ? slot : slot / p.top) * K + k + Q_STEP * q;
     }
   };
-  // piece i of a block: bfloat16 weights meet k 32 i + 8 q, 8-bit ones 64 (i / 2) + 16 q + 8 (i % 2)
-  auto piece = [&](int t, int k0, int i) -> uint4 {
-    const int k = FP8 ? k0 + 64 * (i >> 1) + 16 * q + 8 * (i & 1) : k0 + 32 * i + 8 * q;
-    if (rows[t] < 0 || k >= K) return zero;
-    const uint4* from = reinterpret_cast<const uint4*>(tokens + (size_t)rows[t] * K + k);
-    return DOWN ? __ldcg(from) : __ldg(from);
+  // piece i of a block: bfloat16 weights meet k 32 i + 8 q, 8-bit ones 64 (i / 2) + 16 q + 8 (i % 2); `left` k to the rows' ends
+  auto fetch = [&](int i, int left) {
+    const int off = FP8 ? 64 * (i >> 1) + 8 * (i & 1) : 32 * i;
+    const bool in = off + Q_STEP * q < left;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      if (t < tiles) {
+        const uint4* at = reinterpret_cast<const uint4*>(from[t] + off);
+        b[t][i] = !in ? make_uint4(0u, 0u, 0u, 0u) : (DOWN ? __ldcg(at) : __ldg(at));
+      }
   };
   float acc[T][4];
 #pragma unroll
@@ -232,40 +241,49 @@ __device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Blo
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
 
+  if (count > 0) open(s);
   for (int i = 0; i < R.stages; ++i) fill();
   ready();
-  int a = begin / per, s = begin - a * per;
   if (count > 0) {
-    enter(a);
+    enter(a, s * D::STAGE);
 #pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[t][i] = piece(t, s * D::STAGE, i);
+    for (int i = 0; i < 4; ++i) fetch(i, K - s * D::STAGE);
   }
-  float s_lo = 1.f, s_hi = 1.f;
+  int nt = tiles;                             // ... and of the expert of the products
+  size_t scale_lo = 0, scale_hi = 0;
+  auto scales_of = [&](int at) {
+    scale_lo = ((size_t)L.active[at] * RB + min(row_lo + g, rows_all - 1) / 128) * KB;
+    scale_hi = ((size_t)L.active[at] * RB + min(row_hi + g, rows_all - 1) / 128) * KB;
+  };
+  if (FP8 && count > 0) scales_of(a);
+  bool ok = B.stop == 0;
+#pragma unroll 1
   for (int j = 0; j < count; ++j) {
-    const int c0 = L.first[a], nt = (L.first[a + 1] - c0 + 7) / 8;
-    const bool last_stage = s + 1 == per;
-    if (j + 1 == count) ending();
-    bool ok = !B.stop;
+    const bool last_stage = s + 1 == per, more = j + 1 < count;
+    if (!more) ending();
     if (ok) ok = mbar_wait(R.bar + R.use, R.phase, &B.stop, p.status, 112);
+    if (!ok) to_fill = 0;
     const uint32_t at = R.at + (uint32_t)R.use * STAGE_BYTES + row_at(g) + 16u * q;
     if (++R.use == R.stages) { R.use = 0; R.phase ^= 1u; }
 #pragma unroll
     for (int blk = 0; blk < D::STAGE / 128; ++blk) {
-      const int k0 = s * D::STAGE + 128 * blk;
-      if (k0 >= K) break;
+      const int left = K - s * D::STAGE - 128 * blk;      // k from this block to the rows' ends
+      if (blk > 0 && left <= 0) break;
+      float s_lo = 1.f, s_hi = 1.f;
       if (FP8) {
-        s_lo = block_scale(scales, p.e8m0, ((size_t)L.active[a] * RB + min(row_lo + g, rows_all - 1) / 128) * KB + k0 / 128);
-        s_hi = block_scale(scales, p.e8m0, ((size_t)L.active[a] * RB + min(row_hi + g, rows_all - 1) / 128) * KB + k0 / 128);
+        const int kb = s * (D::STAGE / 128) + blk;
+        s_lo = block_scale(DOWN ? p.sd : p.su, p.e8m0, scale_lo + kb);
+        s_hi = block_scale(DOWN ? p.sd : p.su, p.e8m0, scale_hi + kb);
       }
-      // where the next block's tokens lie; each piece is asked for when the one before it in its registers has been used
-      int next_k = -1;
-      if (blk + 1 < D::STAGE / 128 && k0 + 128 < K) {
-        next_k = k0 + 128;
-      } else if (j + 1 < count) {
-        next_k = last_stage ? 0 : (s + 1) * D::STAGE;
-        if (last_stage) enter(a + 1);
+      // the next block's tokens; each piece is asked for when the one before it in its registers has been used
+      int next_left = 0;
+      if (left > 128 && (blk + 1 < D::STAGE / 128 || more)) {
+        next_left = left - 128;
+#pragma unroll
+        for (int t = 0; t < T; ++t) from[t] += 128;
+      } else if (left <= 128 && more) {
+        next_left = K;
+        enter(a + 1, 0);
       }
       float sum[FP8 ? T : 1][4];
       if (FP8) {
@@ -276,43 +294,39 @@ __device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Blo
       }
 #pragma unroll
       for (int st = 0; st < D::STEPS; ++st) {
-        const int ks = k0 + st * D::STEP;
-        if (ks < K) {
-          uint4 lo = lds16(at + (uint32_t)(blk * D::STEPS + st) * 64u), hi = lds16(at + (uint32_t)(blk * D::STEPS + st) * 64u + 4 * 576);
-          if (ks + D::STEP > K && ks + (16 / D::ESZ) * q >= K) lo = hi = zero;    // behind the rows' ends: what an earlier stage left
-          if (FP8) {
-            const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
-            uint32_t wl[8], wh[8];
+        const uint32_t off = (uint32_t)(blk * D::STEPS + st) * 64u;
+        uint4 lo = lds16(at + off), hi = lds16(at + off + 4 * 576);
+        if (left < 128 && st * D::STEP + (16 / D::ESZ) * q >= left) lo = hi = make_uint4(0u, 0u, 0u, 0u);   // what an earlier stage left
+        if (FP8) {
+          const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              widen4(l[i], wl[2 * i], wl[2 * i + 1]);
-              widen4(h[i], wh[2 * i], wh[2 * i + 1]);
+          for (int half = 0; half < 2; ++half) {
+            uint32_t wl[4], wh[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              widen4(l[2 * half + i], wl[2 * i], wl[2 * i + 1]);
+              widen4(h[2 * half + i], wh[2 * i], wh[2 * i + 1]);
             }
 #pragma unroll
             for (int t = 0; t < T; ++t)
               if (t < nt) {
-                const uint4 x = b[t][2 * st];
-                const uint4 y = b[t][2 * st + 1];
+                const uint4 x = b[t][2 * st + half];
                 mma_bf16_16816(sum[t], wl[0], wh[0], wl[1], wh[1], x.x, x.y);
                 mma_bf16_16816(sum[t], wl[2], wh[2], wl[3], wh[3], x.z, x.w);
-                mma_bf16_16816(sum[t], wl[4], wh[4], wl[5], wh[5], y.x, y.y);
-                mma_bf16_16816(sum[t], wl[6], wh[6], wl[7], wh[7], y.z, y.w);
-              }
-          } else {
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-              if (t < nt) {
-                const uint4 x = b[t][st];
-                mma_bf16_16816(acc[t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-                mma_bf16_16816(acc[t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
               }
           }
-        }
-        if (next_k >= 0) {
+        } else {
 #pragma unroll
           for (int t = 0; t < T; ++t)
+            if (t < nt) {
+              const uint4 x = b[t][st];
+              mma_bf16_16816(acc[t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+              mma_bf16_16816(acc[t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+            }
+        }
+        if (next_left > 0) {
 #pragma unroll
-            for (int i = 0; i < 4 / D::STEPS; ++i) b[t][4 / D::STEPS * st + i] = piece(t, next_k, 4 / D::STEPS * st + i);
+          for (int i = 0; i < 4 / D::STEPS; ++i) fetch(4 / D::STEPS * st + i, next_left);
         }
       }
       if (FP8) {
@@ -327,15 +341,18 @@ __device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Blo
     }
     __syncwarp();                             // every lane has read the stage
     fill();
-    if (last_stage || j + 1 == count) {
+    if (last_stage || !more) {
       done(a, acc);
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+      nt = tiles;
+      s = -1;
+      ++a;
+      if (FP8 && more) scales_of(a);
     }
     ++s;
-    if (last_stage) { s = 0; ++a; }
   }
 }
 
