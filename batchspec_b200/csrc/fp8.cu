@@ -11,7 +11,7 @@
 // Bound by memory: one read of x (2 or 4 bytes a number), one write of q.  A block's numbers stay in registers between the
 // maximum and the rounding, so x is read once.  Rows: 16 lanes hold a bfloat16 block as 16-byte pieces (a float32 block takes
 // 32 lanes); 128 x 128: one thread block each, 64 numbers per thread.
-#include "common.cuh"
+#include "e4m3.cuh"
 
 using namespace bspec;
 
@@ -19,26 +19,6 @@ namespace {
 
 constexpr int FP8_BLOCK = 128;
 constexpr int QUANT_THREADS = 256;
-
-// the bits of max |x| -> the e8m0 code of the block, and 1 / s
-__device__ __forceinline__ int scale_code(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return 255;
-  if (amax_bits == 0u) return 127;
-  const int code = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);   // above 1.75 x 2^e: 448 = 1.75 x 2^8
-  return code < 0 ? 0 : code;
-}
-__device__ __forceinline__ float inverse_scale(int code) {
-  return code == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(254 - code) << 23);
-}
-// two float32 numbers -> two e4m3 numbers, the first in the low byte
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t to_e4m3x4(const float* v, float inv) {
-  return to_e4m3x2(v[0] * inv, v[1] * inv) | (to_e4m3x2(v[2] * inv, v[3] * inv) << 16);
-}
 
 // A piece: 16 bytes of x as float32 numbers (8 of bfloat16, 4 of float32); numbers past `left` are 0.
 template <typename T> struct Piece;

@@ -13,6 +13,7 @@
 //     order through distributed shared memory.
 //   tokens on the rows, 256 rows of W on the columns (many tokens): one persistent CTA per SM; eight epilogue warps hold the
 //     128 x 256 sums.
+#include "e4m3.cuh"
 #include "umma.cuh"
 
 using namespace bspec;
@@ -31,12 +32,9 @@ struct Scales {
   long long ld;          // from row to row of scales
   int e8m0;              // 1: exponents in 8 bits, 0: float32
 };
-__device__ __forceinline__ float e8m0_value(uint32_t code) {
-  return __uint_as_float(code == 0u ? 0x00400000u : (code == 255u ? 0x7fc00000u : code << 23));
-}
 __device__ __forceinline__ float scale_at(const Scales& s, long long row, int kb) {
   const long long i = row * s.ld + kb;
-  return s.e8m0 ? e8m0_value(reinterpret_cast<const uint8_t*>(s.p)[i]) : reinterpret_cast<const float*>(s.p)[i];
+  return s.e8m0 ? scale_value(reinterpret_cast<const uint8_t*>(s.p)[i]) : reinterpret_cast<const float*>(s.p)[i];
 }
 
 struct Fp8Params {

@@ -2,22 +2,29 @@
 //   z = Wr h,  (ids, w) = choice(z)                      the rules of moe_choose.cuh
 //   u[t, k] = act(Wup[ids[t, k]] h[t])                   act: GELU, or silu(gate) * up with Wup = [gate; up]
 //   out[t]  = add[t] * sigmoid(gate logit) + sum over k of w[t, k] * (Wdown[ids[t, k]] u[t, k], or h[t] for an identity expert)
-// Experts in bfloat16, or in 8-bit floating point (e4m3) with a scale per 128 x 128 block; activations stay bfloat16 either
-// way (u is rounded to bfloat16 between the products: it is the operand of a bfloat16 product), sums are float32.
+// Experts in bfloat16, or in 8-bit floating point (e4m3) with a scale per 128 x 128 block; sums are float32.
 //
-// Bound by the read of the chosen experts' weights.  A weight is fetched once per 16 tokens of its expert, by bulk copies into a ring
-// of its warp's own (several KB per warp are in flight, whatever the registers hold), and meets its tokens on mma.sync m16n8k16: the
-// WEIGHT rows take the 16 rows of the product, the expert's tokens its columns, 8 at a time.  Both operands number the k of a step in
-// the same permuted order (lane l % 4 holds neighbouring k), which a sum over k does not notice.
+// Bound by the read of the chosen experts' weights, each of which is used once per step.  So the weights take the 128 rows of
+// tcgen05 products, streamed at full tile efficiency by TMA into a ring of 16 KB stages, and the tokens their 16 to 64 columns:
+// a stage costs two copies of weights and a few instructions, and what the sums cost does not grow with the weights.
+//   up     all tokens of the step are columns of every expert (no gather: the columns that did not choose it are dropped)
+//   down   an expert's tokens are its columns: u lies sorted by expert, 16 rows to a copy
+// bfloat16 weights: u is rounded to bfloat16 between the products.  8-bit weights: the activations do not lose precision to the
+// weights' format.  Every activation is the sum of two e4m3 numbers, x = s (a + b / 16): a is x / s rounded to 4 bits, b what is
+// left, times 16; s is a power of two, one for a token's h and one for 64 numbers of u.  That is 8 bits, as many as bfloat16 has (h is met
+// exactly down to 2^-22 of the token's largest number); both are columns of the same product.  A block of 128 k (of 64 in the down
+// products, for the scales of u) gets an accumulator of its own, which the epilogue warps read back and add to float32 sums.
 //
 //   route    one cluster of 8 CTAs per 8 tokens: 64 warps share the router's rows and k, partial sums meet in the first CTA's
 //            shared memory, whose warps choose for a token each.  It also clears the counters of the second kernel.
-//   experts  one CTA per SM.  First all pieces of the up products are drawn from one counter, then pieces of 16 output columns
-//            over all chosen experts.  A piece of the second kind waits until every piece of the first kind is done; those have
-//            all been drawn by CTAs that run and wait for nothing, so it ends however many CTAs the device can hold.  A column's
-//            sum runs over the experts in a fixed order: no atomic adds numbers.
+//   experts  one CTA per SM: a TMA warp that draws pieces of work, an MMA warp, four epilogue warps.  First the pieces of the up products
+//            (128 rows of one expert) are drawn from one counter, then those of the down products (128 output columns of one expert,
+//            perhaps a slice of its k).  A piece of the second kind waits until every piece of the first kind is done; those
+//            have all been drawn by CTAs that run and wait for nothing, so it ends however many CTAs the device can hold.
+//            When the last down piece is done, all CTAs add the experts' results in the order of the choices: no atomic adds numbers.
 #include "moe_choose.cuh"
-#include "tma.cuh"
+#include "e4m3.cuh"
+#include "umma.cuh"
 #include <math.h>
 
 using namespace bspec;
@@ -26,7 +33,7 @@ namespace {
 
 constexpr int LAYER_TOKENS = 64;             // most tokens of a step
 constexpr int ROUTE_CLUSTER = 8, ROUTE_WARPS = 8, ROUTE_TOKENS = 8;
-constexpr int WARPS = 16, LAYER_THREADS = 32 * WARPS;
+constexpr int LAYER_THREADS = 192;           // TMA warp, MMA warp, 4 epilogue warps
 constexpr int SMEM_BUDGET = 225 * 1024;
 
 // ------------------------------------------------------------------------------------------------ the router
@@ -34,7 +41,8 @@ constexpr int SMEM_BUDGET = 225 * 1024;
 __global__ void __cluster_dims__(ROUTE_CLUSTER, 1, 1) __launch_bounds__(32 * ROUTE_WARPS)
 moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const __nv_bfloat16* __restrict__ wr, int rows, int slices,
                        const void* __restrict__ corr, int corr_dtype, int C, int G, int keep, int top, float scale, int rule,
-                       int* __restrict__ ids, float* __restrict__ wts, float* __restrict__ gate, int* __restrict__ counters) {
+                       int* __restrict__ ids, float* __restrict__ wts, float* __restrict__ gate, int* __restrict__ counters,
+                       uint8_t* __restrict__ hq, float* __restrict__ hs) {
   bspec::pdl_prologue(84);
   extern __shared__ float sm[];
   const int tiles = (rows + 15) / 16, units = tiles * slices;
@@ -80,7 +88,42 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   float* bias = part + (size_t)units * 16 * ROUTE_TOKENS;      // [C]
   if (rank == 0)
     for (int e = threadIdx.x; e < C; e += 32 * ROUTE_WARPS) bias[e] = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // 8-bit experts: CTA `rank` brings token t0 + rank into two 8-bit numbers for each of its own, with one scale
+  if (hq != nullptr && t0 + rank < n) {
+    const int row = t0 + rank;
+    __shared__ uint32_t warp_max[ROUTE_WARPS];
+    uint32_t m = 0u;
+    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUTE_WARPS; ++i) m = max(m, warp_max[i]);
+    const int code = scale_code(m);
+    const float inv = inverse_scale(code);
+    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float v[4] = {__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
+                            __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u)};
+        two_e4m3x4(v, inv, hi[i], lo[i]);
+      }
+      *reinterpret_cast<uint2*>(hq + (size_t)row * d + k) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(hq + (size_t)(n + row) * d + k) = make_uint2(lo[0], lo[1]);
+    }
+    if (threadIdx.x == 0) hs[row] = scale_value(code);
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int t = t0 + warp;
   if (rank != 0 || t >= n) return;
   float* sc = bias + C + (size_t)warp * 3 * C;
@@ -98,524 +141,678 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
 }
 
 // ------------------------------------------------------------------------------------------------ the experts
+constexpr int TILE = 128;                    // weight rows of a piece
+constexpr int A_BYTES = TILE * 128;          // of a stage: 128 bytes of every row
+constexpr int QUEUE = 4, SLOTS = 4;          // pieces on their way through the roles; accumulators
+constexpr int MAX_STAGES = 10;
+constexpr int MAX_SPLITS = 4;                // slices of k of the down products
+
 struct LayerParams {
-  const __nv_bfloat16* h;                    // [n, d]
-  const unsigned char* wu;                   // [E, ffu, d]
-  const unsigned char* wd;                   // [E, d, ff]
-  const void* su;                            // scales of 128 x 128 blocks, or null
-  const void* sd;
+  const float* su;                           // scales of 128 x 128 blocks: float32, or 8-bit exponents (e8m0)
+  const float* sd;
   int e8m0;
   const int* ids;                            // [n, top]; E and above: the token's own h
   const float* wts;
   const float* gate;                         // [n] or null
+  const __nv_bfloat16* h;                    // [n, d]
   const __nv_bfloat16* add;                  // [n, d] or null
-  __nv_bfloat16* u;                          // [n top, ff]
+  const float* hs;                           // [n] scales of the tokens' 8-bit numbers
+  unsigned char* u;                          // entries sorted by expert: [n top, ff] bfloat16, or e4m3 [2][n top, ff]
+  float* us;                                 // [n top, blocks of 64] their scales
+  float* y;                                  // [splits][n top, d] the experts' results
   __nv_bfloat16* out;                        // [n, d]
-  int* counters;                             // {pieces drawn, up pieces done, output pieces drawn}, zero
+  int* counters;                             // zero: {up pieces drawn, up pieces done, down pieces drawn, down pieces done}
   int* status;
   int n, d, ff, E, top;
-  int stages;                                // of a warp's ring
+  int stages;
 };
 
-__device__ __forceinline__ uint4 lds16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-// Four e4m3 numbers -> bfloat16, two to a register.  Sign, exponent and fraction move to their places, which leaves a number 2^120 times
-// too small (the exponents' biases differ by 120; numbers below e4m3's normal ones become bfloat16 numbers below its normal ones); the
-// product with 2^120 is exact.
-__device__ __forceinline__ uint32_t widen(uint32_t halves) {       // each half: the number in its high byte, 0 in its low one
-  const uint32_t r = (halves & 0x80008000u) | ((halves >> 4) & 0x07f007f0u);
-  const __nv_bfloat162 big = __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80));      // 2^120
-  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&r), big);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  lo = widen(__byte_perm(w, 0u, 0x1404));
-  hi = widen(__byte_perm(w, 0u, 0x3424));
-}
-__device__ __forceinline__ float block_scale(const void* p, int e8m0, size_t i) {
-  if (!e8m0) return reinterpret_cast<const float*>(p)[i];
-  const uint32_t code = reinterpret_cast<const uint8_t*>(p)[i];
-  return __uint_as_float(code == 0u ? 0x00400000u : (code == 255u ? 0x7fc00000u : code << 23));
-}
-
-// A stage of a warp's ring: 256 bytes of each of 16 weight rows, fetched row by row by bulk copies.  Lanes 8 i .. 8 i + 7 read the rows
-// 2 i and 2 i + 1 together, 64 bytes of each: an odd row begins 64 bytes further round the 128 bytes that the banks span.
-constexpr int ROW_BYTES = 256, STAGE_BYTES = 8 * 576;
-__device__ __forceinline__ uint32_t row_at(int r) { return (uint32_t)((r >> 1) * 576 + (r & 1) * 320); }
-// k of a stage, and of a step of the products; tokens' numbers are read 128 k (a scale's block) at a time
-template <bool FP8> struct Depth { static constexpr int ESZ = FP8 ? 1 : 2, STAGE = ROW_BYTES / ESZ, STEP = FP8 ? 64 : 32, STEPS = 128 / STEP; };
-
-// What all pieces of a CTA know of the step, in shared memory.
-struct Lists {
-  int* active;                               // chosen experts, ascending; one with more than 16 tokens stands here once for every 16
-  int* first;                                // [active + 1] where their entries begin
-  int* slot;                                 // entries: (token, choice) numbers by expert
-  int* count;                                // [E] scratch
-  float* total;                              // this warp's sums [tokens][16 rows]; before that its partial tiles
-};
-struct Block {
-  int drawn[WARPS];                          // a team's next piece
-  int base, n_active, most, done, piece;
-  int stop;                                  // a wait ran out
-};
-constexpr int MOST_COLUMNS = 16;             // tokens that meet a weight at a time
-__host__ __device__ inline int most_active(int n, int E, int top) { return E + n * top / MOST_COLUMNS; }
-// A warp's ring: `stages` slots; running slot and phase of the next stage to fill and to use.
-struct Ring {
-  uint32_t at, bars;
-  uint64_t* bar;
-  int stages, fill, use;
-  uint32_t phase;
+struct Piece {
+  int down;                                  // 0: up, 1: down, -1: no more
+  int a, tile, s0, s1, split;                // place in the list of chosen experts, 128 rows, stages of k
 };
 
-// Streams the stages [begin, begin + count) of the weight rows row_lo + 0 .. 7, row_hi + 0 .. 7 of the chosen experts, one expert's
-// after the other's (`per` stages each), through this warp's ring, and multiplies them with the experts' tokens.  `done(a, acc)` is called
-// when the last stage of expert a's share has been added to acc[column tile][4]; acc is cleared afterwards.  `ready()` is called when the
-// first stages have been asked for and before any token is read, `ending()` before the last stage is waited for.
-template <bool FP8, int T, bool DOWN, typename Ready, typename Ending, typename Done>
-__device__ __forceinline__ void stream(const LayerParams& p, const Lists& L, Block& B, Ring& R, int begin, int count, int per, int row_lo,
-                                       int row_hi, int rows_all, int K, Ready ready, Ending ending, Done done) {
-  using D = Depth<FP8>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const __nv_bfloat16* const tokens = DOWN ? p.u : p.h;
-  const int KB = (K + 127) / 128, RB = (rows_all + 127) / 128;
-  const uint32_t row_bytes = (uint32_t)K * D::ESZ;
+__device__ __forceinline__ void mma_8bit(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ float block_scale(const float* p, int e8m0, size_t i) {
+  return e8m0 ? scale_value(reinterpret_cast<const uint8_t*>(p)[i]) : p[i];
+}
 
-  // filling: lane r copies row r; a running source, set anew where the next expert begins
-  const int my_row = lane < 8 ? row_lo + lane : row_hi + (lane & 7);
-  const bool copies = lane < 16 && my_row < rows_all;
-  const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies));
-  const uint32_t last_bytes = row_bytes - (uint32_t)(per - 1) * ROW_BYTES, my_slot = R.at + row_at(lane);
-  int a = begin / per, s = begin - a * per, fa = a, f_left = per - s, to_fill = count;
-  const unsigned char* src = nullptr;
-  auto open = [&](int from) { src = (DOWN ? p.wd : p.wu) + ((size_t)L.active[fa] * rows_all + my_row) * row_bytes + (size_t)from * ROW_BYTES; };
-  auto fill = [&]() {
-    if (to_fill == 0) return;
-    const uint32_t bytes = f_left == 1 ? last_bytes : (uint32_t)ROW_BYTES, bar = R.bars + 8u * R.fill;
-    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * n_copies) : "memory");
-    if (copies) copy_bulk(my_slot + (uint32_t)R.fill * STAGE_BYTES, src, bytes, bar);
-    if (++R.fill == R.stages) R.fill = 0;
-    src += ROW_BYTES;
-    --to_fill;
-    if (--f_left == 0 && to_fill > 0) {
-      ++fa;
-      f_left = per;
-      open(0);
-    }
-  };
-  // the tokens' numbers: a cursor of its own, one block of 128 k ahead of the products; a column without a token reads its neighbour's
-  constexpr int Q_STEP = FP8 ? 16 : 8;
-  uint4 b[T][4];
-  const __nv_bfloat16* from[T];
-  int tiles = 0;                              // column tiles of the expert that the cursor is in
-  auto enter = [&](int at, int k) {
-    const int c0 = L.first[at], cnt = L.first[at + 1] - c0;
-    tiles = (cnt + 7) >> 3;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int slot = L.slot[c0 + min(8 * t + g, cnt - 1)];
-      from[t] = tokens + (size_t)(DOWN ? slot : slot / p.top) * K + k + Q_STEP * q;
-    }
-  };
-  // piece i of a block: bfloat16 weights meet k 32 i + 8 q, 8-bit ones 64 (i / 2) + 16 q + 8 (i % 2); `left` k to the rows' ends
-  auto fetch = [&](int i, int left) {
-    const int off = FP8 ? 64 * (i >> 1) + 8 * (i & 1) : 32 * i;
-    const bool in = off + Q_STEP * q < left;
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-      if (t < tiles) {
-        const uint4* at = reinterpret_cast<const uint4*>(from[t] + off);
-        b[t][i] = !in ? make_uint4(0u, 0u, 0u, 0u) : (DOWN ? __ldcg(at) : __ldg(at));
-      }
-  };
-  float acc[T][4];
-#pragma unroll
-  for (int t = 0; t < T; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-
-  if (count > 0) open(s);
-  for (int i = 0; i < R.stages; ++i) fill();
-  ready();
-  if (count > 0) {
-    enter(a, s * D::STAGE);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fetch(i, K - s * D::STAGE);
-  }
-  int nt = tiles;                             // ... and of the expert of the products
-  size_t scale_lo = 0, scale_hi = 0;
-  auto scales_of = [&](int at) {
-    scale_lo = ((size_t)L.active[at] * RB + min(row_lo + g, rows_all - 1) / 128) * KB;
-    scale_hi = ((size_t)L.active[at] * RB + min(row_hi + g, rows_all - 1) / 128) * KB;
-  };
-  if (FP8 && count > 0) scales_of(a);
-  bool ok = B.stop == 0;
-#pragma unroll 1
-  for (int j = 0; j < count; ++j) {
-    const bool last_stage = s + 1 == per, more = j + 1 < count;
-    if (!more) ending();
-    if (ok) ok = mbar_wait(R.bar + R.use, R.phase, &B.stop, p.status, 112);
-    if (!ok) to_fill = 0;
-    const uint32_t at = R.at + (uint32_t)R.use * STAGE_BYTES + row_at(g) + 16u * q;
-    if (++R.use == R.stages) { R.use = 0; R.phase ^= 1u; }
-#pragma unroll
-    for (int blk = 0; blk < D::STAGE / 128; ++blk) {
-      const int left = K - s * D::STAGE - 128 * blk;      // k from this block to the rows' ends
-      if (blk > 0 && left <= 0) break;
-      float s_lo = 1.f, s_hi = 1.f;
-      if (FP8) {
-        const int kb = s * (D::STAGE / 128) + blk;
-        s_lo = block_scale(DOWN ? p.sd : p.su, p.e8m0, scale_lo + kb);
-        s_hi = block_scale(DOWN ? p.sd : p.su, p.e8m0, scale_hi + kb);
-      }
-      // the next block's tokens; each piece is asked for when the one before it in its registers has been used
-      int next_left = 0;
-      if (left > 128 && (blk + 1 < D::STAGE / 128 || more)) {
-        next_left = left - 128;
-#pragma unroll
-        for (int t = 0; t < T; ++t) from[t] += 128;
-      } else if (left <= 128 && more) {
-        next_left = K;
-        enter(a + 1, 0);
-      }
-      float sum[FP8 ? T : 1][4];
-      if (FP8) {
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
-      }
-#pragma unroll
-      for (int st = 0; st < D::STEPS; ++st) {
-        const uint32_t off = (uint32_t)(blk * D::STEPS + st) * 64u;
-        uint4 lo = lds16(at + off), hi = lds16(at + off + 4 * 576);
-        if (left < 128 && st * D::STEP + (16 / D::ESZ) * q >= left) lo = hi = make_uint4(0u, 0u, 0u, 0u);   // what an earlier stage left
-        if (FP8) {
-          const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t wl[4], wh[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              widen4(l[2 * half + i], wl[2 * i], wl[2 * i + 1]);
-              widen4(h[2 * half + i], wh[2 * i], wh[2 * i + 1]);
-            }
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-              if (t < nt) {
-                const uint4 x = b[t][2 * st + half];
-                mma_bf16_16816(sum[t], wl[0], wh[0], wl[1], wh[1], x.x, x.y);
-                mma_bf16_16816(sum[t], wl[2], wh[2], wl[3], wh[3], x.z, x.w);
-              }
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < T; ++t)
-            if (t < nt) {
-              const uint4 x = b[t][st];
-              mma_bf16_16816(acc[t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-              mma_bf16_16816(acc[t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
-            }
-        }
-        if (next_left > 0) {
-#pragma unroll
-          for (int i = 0; i < 4 / D::STEPS; ++i) fetch(4 / D::STEPS * st + i, next_left);
-        }
-      }
-      if (FP8) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-          acc[t][0] = fmaf(sum[t][0], s_lo, acc[t][0]);
-          acc[t][1] = fmaf(sum[t][1], s_lo, acc[t][1]);
-          acc[t][2] = fmaf(sum[t][2], s_hi, acc[t][2]);
-          acc[t][3] = fmaf(sum[t][3], s_hi, acc[t][3]);
-        }
+// Waits until *counter reaches `target` (a bounded wait, as every other one).
+__device__ __forceinline__ bool wait_for(const int* counter, int target, int* status, volatile int* abort_flag) {
+  unsigned long long t_from = 0ull;
+  for (uint32_t i = 0;; ++i) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
+    if (v >= target) return true;
+    if (*abort_flag) return false;
+    if ((i & 255u) == 255u) {
+      const unsigned long long now = bspec::global_timer();
+      if (t_from == 0ull) t_from = now;
+      if (now - t_from > WAIT_NS || i >= WAIT_LIMIT || *reinterpret_cast<volatile int*>(status) != 0) {
+        atomicCAS(status, 0, 111);
+        *abort_flag = 1;
+        return false;
       }
     }
-    __syncwarp();                             // every lane has read the stage
-    fill();
-    if (last_stage || !more) {
-      done(a, acc);
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-      nt = tiles;
-      s = -1;
-      ++a;
-      if (FP8 && more) scales_of(a);
-    }
-    ++s;
   }
 }
+__device__ __forceinline__ float4 four_bf16(const __nv_bfloat16* from) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(from);
+  return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
+                     __uint_as_float(raw.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 scaled(const float4& v, float f) { return make_float4(f * v.x, f * v.y, f * v.z, f * v.w); }
 
-template <bool FP8, bool GLU, int T>
-__device__ __forceinline__ void run_layer(const LayerParams& p, const Lists& L, Block& B, Ring& R) {
-  using D = Depth<FP8>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int A = B.n_active, ffu = GLU ? 2 * p.ff : p.ff, warp_total = (p.n + 7) / 8 * 128;
-
-  // ---- up products: a piece is 16 rows of one expert (GLU: 8 gate rows and their 8 up rows), shared by the warps of a team
-  constexpr int OUT = GLU ? 8 : 16;
-  const int tiles = (p.ff + OUT - 1) / OUT, pieces = A * tiles, depth = (p.d + D::STAGE - 1) / D::STAGE;
-  // a team of 2 or 4 warps cuts a piece's k, as long as each has four stages: short pieces end at about the same time everywhere
-  const int team_size = depth >= 16 ? 4 : (depth >= 8 ? 2 : 1);
-  const int team = warp / team_size, member = warp % team_size;
-  const int per = (depth + team_size - 1) / team_size, from = min(depth, member * per), to = min(depth, from + per);
-  if (threadIdx.x == 0) B.base = atomicAdd(p.counters, WARPS / team_size);
-  __syncthreads();
-  int piece = B.base + team, mine = 0;
-  while (piece < pieces) {
-    int next = 0;
-    const int a = piece / tiles, i0 = (piece - a * tiles) * OUT, c0 = L.first[a], cnt = L.first[a + 1] - c0, nt = (cnt + 7) / 8;
-    float part[T][4];
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[t][i] = 0.f;
-    stream<FP8, T, false>(p, L, B, R, a * depth + from, to - from, depth, i0, GLU ? p.ff + i0 : i0 + 8, ffu, p.d, []() {},
-                          [&]() {             // not earlier: a CTA that starts first would take the others' first pieces
-                            if (member == 0 && lane == 0) next = atomicAdd(p.counters, 1);
-                          },
-                          [&](int, float (&acc)[T][4]) {
-#pragma unroll
-                            for (int t = 0; t < T; ++t)
-#pragma unroll
-                              for (int i = 0; i < 4; ++i) part[t][i] = acc[t][i];
-                          });
-    if (team_size > 1) {
-      if (member != 0) {
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-          if (t < nt) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) L.total[(t * 4 + i) * 32 + lane] = part[t][i];
-          }
-      }
-      if (member == 0 && lane == 0) B.drawn[team] = next;
-      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
-      if (member == 0) {
-        for (int m = 1; m < team_size; ++m)
-#pragma unroll
-          for (int t = 0; t < T; ++t)
-            if (t < nt) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) part[t][i] += L.total[m * warp_total + (t * 4 + i) * 32 + lane];
-            }
-      }
-      next = B.drawn[team];
-      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_size * 32) : "memory");
-    } else {
-      next = __shfl_sync(0xffffffffu, next, 0);
-    }
-    if (member == 0) {
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = 8 * t + 2 * q + i;
-          if (c >= cnt) continue;
-          __nv_bfloat16* u = p.u + (size_t)L.slot[c0 + c] * p.ff + i0 + g;
-          if (GLU) {
-            const float gv = part[t][i];
-            if (i0 + g < p.ff) *u = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * part[t][2 + i]);
-          } else {
-            if (i0 + g < p.ff) u[0] = __float2bfloat16_rn(gelu_erf(part[t][i]));
-            if (i0 + 8 + g < p.ff) u[8] = __float2bfloat16_rn(gelu_erf(part[t][2 + i]));
-          }
-        }
-      ++mine;
-    }
-    piece = next;
+// Shared memory behind the stages.  NB: columns, 16, 32 or 64.
+template <bool FP8, int NB>
+struct Layout {
+  static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
+  __host__ __device__ static int blocks(int k) { return (k + 63) / 64; }
+  // tile [NB][128], scales of a piece's u [ff / 64][NB], then the lists
+  __host__ __device__ static size_t fixed(int ff, int slots, int E) {
+    return (size_t)NB * TILE * 4 + (FP8 ? (size_t)blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
   }
-  if (member == 0 && lane == 0 && mine) atomicAdd(&B.done, mine);
-  __syncthreads();
+};
+
+template <bool FP8, bool GLU, int NB>
+__global__ void __launch_bounds__(LAYER_THREADS, 1)
+moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down,
+                         const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_u, LayerParams p) {
+  using Lay = Layout<FP8, NB>;
+  constexpr int STAGE_K = FP8 ? 128 : 64;                      // k of a stage
+  constexpr int WIDTH = FP8 ? 2 * NB : NB;                     // columns of an accumulator
+  constexpr uint32_t TMEM_COLS = SLOTS * WIDTH;                // 64 .. 512
+  constexpr int OUT = GLU ? 64 : 128;                          // numbers of u per up piece
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[SLOTS], acc_empty[SLOTS], q_full[QUEUE], q_empty[QUEUE], meet;
+  __shared__ Piece queue[QUEUE];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word, n_active;
+  volatile int* abort_flag = &abort_word;
+  const int slots = p.n * p.top, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* tile = reinterpret_cast<float*>(smem + (size_t)p.stages * Lay::STAGE);          // [NB][128]
+  float* ys = tile + NB * TILE;
+  int* pos = reinterpret_cast<int*>(ys + (FP8 ? Lay::blocks(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
+  int* tok = pos + slots;                                                                // [slots] tokens by expert
+  int* active = tok + slots;                                                             // [E] chosen experts, ascending
+  int* first = active + p.E;                                                             // [E + 1] where their entries begin
+  int* count = first + p.E + 1;                                                          // [E]
+
+  if (threadIdx.x >= 64 && threadIdx.x < 68) {
+    const CUtensorMap* map = threadIdx.x == 64 ? &map_up : (threadIdx.x == 65 ? &map_down : (threadIdx.x == 66 ? &map_h : &map_u));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   if (threadIdx.x == 0) {
-    if (B.done) {
-      __threadfence();
-      atomicAdd(p.counters + 1, B.done);
+    for (int i = 0; i < MAX_STAGES; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
     }
-    B.piece = atomicAdd(p.counters + 2, 1);
-  }
-  __syncthreads();
-  // ---- down products: a piece is 16 output columns over all chosen experts; the warps take equal shares of the (expert, k) stages
-  const int out_pieces = (p.d + 15) / 16, per_expert = (p.ff + D::STAGE - 1) / D::STAGE;
-  const int all = A * per_expert, w0 = (int)((long long)all * warp / WARPS), w1 = (int)((long long)all * (warp + 1) / WARPS);
-  bool waited = false;
-  auto up_done = [&]() {                      // every up piece of every CTA is done
-    if (waited) return;
-    waited = true;
-    if (threadIdx.x == 0) {
-      unsigned long long t_from = 0ull;
-      for (uint32_t i = 0; !B.stop; ++i) {
-        int v;
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.counters + 1) : "memory");
-        if (v >= pieces) break;
-        if ((i & 255u) == 255u) {
-          const unsigned long long now = bspec::global_timer();
-          if (t_from == 0ull) t_from = now;
-          if (now - t_from > WAIT_NS || i >= WAIT_LIMIT || *reinterpret_cast<volatile int*>(p.status) != 0) {
-            atomicCAS(p.status, 0, 111);
-            B.stop = 1;
-          }
-        }
-      }
-      __threadfence();
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 128);
     }
-    __syncthreads();
-  };
-  while (B.piece < out_pieces) {
-    const int n0 = B.piece * 16;
-    for (int i = lane; i < p.n * 16; i += 32) L.total[i] = 0.f;
-    __syncwarp();
-    stream<FP8, T, true>(p, L, B, R, w0, w1 - w0, per_expert, n0, n0 + 8, p.d, p.ff, up_done, []() {}, [&](int a, float (&acc)[T][4]) {
-      const int c0 = L.first[a], cnt = L.first[a + 1] - c0;
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = 8 * t + 2 * q + i;
-          if (c >= cnt) continue;
-          const int slot = L.slot[c0 + c];
-          const float w = p.wts[slot];
-          float* to = L.total + slot / p.top * 16 + g;
-          to[0] = fmaf(w, acc[t][i], to[0]);
-          to[8] = fmaf(w, acc[t][2 + i], to[8]);
-        }
-      __syncwarp();
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) B.base = atomicAdd(p.counters + 2, 1);
-    const float* totals = L.total - warp * warp_total;
-    if (!B.stop)
-      for (int i = threadIdx.x; i < p.n * 16; i += LAYER_THREADS) {
-        const int t = i >> 4, col = n0 + (i & 15);
-        if (col >= p.d) continue;
-        float v = 0.f;
-        if (p.add != nullptr) {
-          v = to_f32(p.add[(size_t)t * p.d + col]);
-          if (p.gate != nullptr) v *= 1.f / (1.f + expf(-p.gate[t]));
-        }
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) v += totals[w * warp_total + i];
-        for (int k = 0; k < p.top; ++k)
-          if (p.ids[(size_t)t * p.top + k] >= p.E) v = fmaf(p.wts[(size_t)t * p.top + k], to_f32(p.h[(size_t)t * p.d + col]), v);
-        p.out[(size_t)t * p.d + col] = __float2bfloat16_rn(v);
-      }
-    __syncthreads();
-    if (threadIdx.x == 0) B.piece = B.base;
-    __syncthreads();
+    for (int i = 0; i < QUEUE; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 129);
+    }
+    mbar_init(&meet, 128);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // after a wait that ran out: copies in flight land (they take microseconds) before the shared memory is given up
-  if (B.stop)
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-}
-
-// bytes of shared memory for the sums, the rings and the lists; a CTA's static shared memory comes on top
-__host__ __device__ inline size_t layer_smem(int n, int E, int top, int stages) {
-  return (size_t)WARPS * ((n + 7) / 8 * 128 * 4 + stages * STAGE_BYTES) + ((size_t)n * top + 2 * (size_t)most_active(n, E, top) + 1 + E) * 4;
-}
-constexpr int MAX_STAGES = 4;
-
-template <bool FP8, bool GLU>
-__global__ void __launch_bounds__(LAYER_THREADS, 1) moe_layer_experts_kernel(LayerParams p) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ Block B;
-  __shared__ uint64_t bars[WARPS * MAX_STAGES];
-  const int slots = p.n * p.top, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < WARPS * MAX_STAGES) mbar_init(bars + threadIdx.x, 1);
-  if (threadIdx.x == 0) B.done = B.stop = 0;
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  Lists L;
-  Ring R;
-  R.at = s32(smem) + (uint32_t)(warp * p.stages) * STAGE_BYTES;
-  R.bar = bars + warp * MAX_STAGES;
-  R.bars = s32(R.bar);
-  R.stages = p.stages;
-  R.fill = R.use = 0;
-  R.phase = 0u;
-  unsigned char* at = smem + (size_t)WARPS * p.stages * STAGE_BYTES;
-  L.total = reinterpret_cast<float*>(at) + (size_t)warp * ((p.n + 7) / 8 * 128);
-  at += (size_t)WARPS * ((p.n + 7) / 8 * 128) * 4;
-  L.slot = reinterpret_cast<int*>(at);
-  L.active = L.slot + slots;
-  L.first = L.active + most_active(p.n, p.E, p.top);
-  L.count = L.first + most_active(p.n, p.E, p.top) + 1;
-  for (int e = threadIdx.x; e < p.E; e += LAYER_THREADS) L.count[e] = 0;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  for (int e = threadIdx.x; e < p.E; e += LAYER_THREADS) count[e] = 0;
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
   bspec::pdl_prologue(85);
-  // the entries by expert: counted, then placed
+
+  // ---- the entries by expert: counted, then placed in the order of their numbers, so that every CTA has the same order
   for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
     const int e = p.ids[s];
-    if (e < p.E) atomicAdd(L.count + e, 1);
+    if (e < p.E) atomicAdd(count + e, 1);
   }
   __syncthreads();
   if (warp == 0) {
-    int n_active = 0, run = 0, most = 0;
+    int found = 0, run = 0;
+#pragma unroll 1
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane, c = e < p.E ? L.count[e] : 0, groups = (c + MOST_COLUMNS - 1) / MOST_COLUMNS;
-      int upto = c, upto_g = groups;
+      const int e = e0 + lane, c = e < p.E ? count[e] : 0;
+      int upto = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o), w = __shfl_up_sync(0xffffffffu, upto_g, o);
-        if (lane >= o) upto += v, upto_g += w;
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
       }
-      const int from = run + upto - c;
-      for (int i = 0; i < groups; ++i) {
-        L.active[n_active + upto_g - groups + i] = e;
-        L.first[n_active + upto_g - groups + i] = from + i * MOST_COLUMNS;
+      const unsigned mask = __ballot_sync(0xffffffffu, c > 0);
+      if (c > 0) {
+        const int at = found + __popc(mask & ((1u << lane) - 1u));
+        active[at] = e;
+        first[at] = count[e] = run + upto - c;
       }
-      if (c > 0) L.count[e] = from;                               // where the next entry of this expert goes
-      most = max(most, c);
-      n_active += __shfl_sync(0xffffffffu, upto_g, 31);
+      found += __popc(mask);
       run += __shfl_sync(0xffffffffu, upto, 31);
     }
-    most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
-      L.first[n_active] = run;
-      B.n_active = n_active;
-      B.most = most;
+      first[found] = run;
+      n_active = found;
     }
     __syncwarp();
-    // placed in the order of their numbers, so that every CTA has the same ones in an expert's first 16
+#pragma unroll 1
     for (int s0 = 0; s0 < slots; s0 += 32) {
       const int s = s0 + lane, e = s < slots ? p.ids[s] : p.E;
       const unsigned same = __match_any_sync(0xffffffffu, e);
       if (e < p.E) {
-        const int from = L.count[e];
-        L.slot[from + __popc(same & ((1u << lane) - 1u))] = s;
+        const int from = count[e], at = from + __popc(same & ((1u << lane) - 1u));
+        pos[s] = at;
+        tok[at] = s / p.top;
         __syncwarp(same);
-        if (lane == __ffs(same) - 1) L.count[e] = from + __popc(same);
+        if (lane == __ffs(same) - 1) count[e] = from + __popc(same);
+      } else if (s < slots) {
+        pos[s] = -1;
       }
       __syncwarp();
     }
   }
   __syncthreads();
-  if (B.most <= 8) run_layer<FP8, GLU, 1>(p, L, B, R);
-  else run_layer<FP8, GLU, 2>(p, L, B, R);
+
+  const int A = n_active, ffu = GLU ? 2 * p.ff : p.ff;
+  const int up_tiles = (p.ff + OUT - 1) / OUT, up_pieces = A * up_tiles, up_stages = (p.d + STAGE_K - 1) / STAGE_K;
+  const int down_tiles = (p.d + TILE - 1) / TILE, down_stages = (p.ff + STAGE_K - 1) / STAGE_K;
+  // slices of the down products' k, four stages each at least: more of them only where that fills the CTAs' rounds by a seventh better
+  int splits = 1;
+  {
+    const int whole = A * down_tiles, G = gridDim.x;
+    int best = (whole + G - 1) / G;                            // rounds, each of 1 / splits
+    for (int s = 2; s <= MAX_SPLITS && down_stages >= 4 * s; ++s) {
+      const int rounds = (whole * s + G - 1) / G;
+      if (rounds * splits * 7 <= best * s * 6) { best = rounds; splits = s; }
+    }
+  }
+  const int down_per = (down_stages + splits - 1) / splits, down_pieces = A * down_tiles * splits;
+  const int entries = first[A];
+
+  if (warp == 0) {
+    // Lane 0 and 1 copy the weights' two halves of a stage, the next lanes 16 rows of tokens each: a stage costs the warp one
+    // pass through this code, not one thread a pass per copy.
+    int st = 0, np = 0;                                        // stage of the ring, pieces so far
+    uint32_t phase = 0u;
+    bool ok = true;
+    auto push = [&](const Piece& piece) {
+      const int q = np % QUEUE;
+      if (ok) ok = mbar_wait(q_empty + q, ((uint32_t)(np / QUEUE) & 1u) ^ 1u, abort_flag, p.status, 113);
+      if (lane == 0 && ok) {
+        queue[q] = piece;
+        mbar_arrive(q_full + q);
+      }
+      ++np;
+      __syncwarp();
+    };
+    auto draw = [&](int counter) {
+      int t = 0;
+      if (lane == 0) t = atomicAdd(p.counters + counter, 1);
+      return __shfl_sync(0xffffffffu, t, 0);
+    };
+    // this lane's copy of a piece: map, row and place in a stage (`role` 0: none, 1: weights, 2: tokens)
+    const CUtensorMap* map = nullptr;
+    int y = 0, role = 0;
+    uint32_t dst = 0u, bytes = 0u;                             // bytes: of a whole stage
+    auto assign = [&](const CUtensorMap* weights, int y0, int y1, const CUtensorMap* tokens, int t0, int mid, int boxes) {
+      const int b = lane - 2;
+      role = lane < 2 ? 1 : (b < boxes * (FP8 ? 2 : 1) ? 2 : 0);
+      map = lane < 2 ? weights : tokens;
+      y = lane == 0 ? y0 : (lane == 1 ? y1 : (b < boxes ? t0 + 16 * b : mid + t0 + 16 * (b - boxes)));
+      dst = lane < 2 ? (uint32_t)lane * (A_BYTES / 2) : A_BYTES + (uint32_t)b * 2048u;
+      bytes = A_BYTES + (uint32_t)boxes * 2048u * (FP8 ? 2u : 1u);
+    };
+    auto step = [&]() {
+      if (++st == p.stages) { st = 0; phase ^= 1u; }
+    };
+    // stage s of the piece, the copies of the roles in `mask`; the first ones also say how many bytes will come
+    auto copy = [&](int s, int mask) {
+      if (mask & 1) {
+        if (ok) ok = mbar_wait(empty + st, phase ^ 1u, abort_flag, p.status, 114);
+        if (lane == 0 && ok) mbar_expect_tx(full + st, bytes);
+      }
+      if (ok && (role & mask)) tma_load_2d(smem + (size_t)st * Lay::STAGE + dst, map, full + st, s * STAGE_K, y);
+      __syncwarp();
+    };
+    // the up products
+    int t = draw(0);
+    while (ok && t < up_pieces) {
+      const int a = t / up_tiles, i0 = (t - a * up_tiles) * OUT, e = active[a];
+      push({0, a, t - a * up_tiles, 0, up_stages, 0});
+      assign(&map_up, e * ffu + i0, e * ffu + i0 + (GLU ? p.ff : 64), &map_h, 0, p.n, NB / 16);
+      for (int s = 0; s < up_stages && ok; ++s, step()) copy(s, 3);
+      t = draw(0);                                             // not earlier: a CTA that starts first would take the others' first pieces
+    }
+    // the down products
+    t = draw(2);
+    bool waited = false;
+    while (ok && t < down_pieces) {
+      const int split = t % splits, a = t / splits % A, dt = t / splits / A, e = active[a];
+      const int s0 = split * down_per, s1 = min(down_stages, s0 + down_per), c0 = first[a];
+      push({1, a, dt, s0, s1, split});
+      assign(&map_down, e * p.d + dt * TILE, e * p.d + dt * TILE + 64, &map_u, c0, slots, (first[a + 1] - c0 + 15) / 16);
+      int s = s0;
+      if (!waited) {
+        // the first weights are asked for before the wait for the up products
+        waited = true;
+        const int ahead = min(s1 - s0, p.stages), st_from = st;
+        const uint32_t phase_from = phase;
+        for (int i = 0; i < ahead && ok; ++i, step()) copy(s0 + i, 1);
+        if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        __threadfence();
+        fence_async_all();                                     // u was written through the generic proxy
+        st = st_from;
+        phase = phase_from;
+        for (int i = 0; i < ahead; ++i, step()) copy(s0 + i, 2);
+        s = s0 + ahead;
+      }
+      for (; s < s1 && ok; ++s, step()) copy(s, 3);
+      t = draw(2);
+    }
+    push({-1, 0, 0, 0, 0, 0});
+    if (*abort_flag)                                           // copies in flight land (they take microseconds) before the CTA ends
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int st = 0, slot = 0;
+      uint32_t phase = 0u, slot_phase = 0u;
+      bool ok = true;
+      const uint64_t desc0 = smem_desc(smem);
+      for (int np = 0; ok; ++np) {
+        const int q = np % QUEUE;
+        if (!(ok = mbar_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 115))) break;
+        const Piece piece = queue[q];
+        mbar_arrive(q_empty + q);
+        if (piece.down < 0) break;
+        const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
+        const int cols = boxes * 16 * (FP8 ? 2 : 1);
+        const uint32_t idesc = FP8 ? (1u << 4) | ((uint32_t)(cols >> 3) << 17) | (8u << 24) : instr_desc(cols);
+        auto next_slot = [&]() {
+          ok = ok && mbar_wait(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
+          tc_fence_after();
+        };
+        auto commit_slot = [&]() {
+          tc_commit(acc_full + slot);
+          if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+        };
+        if (!FP8) next_slot();
+        for (int s = piece.s0; s < piece.s1 && ok; ++s) {
+          if (!(ok = mbar_wait(full + st, phase, abort_flag, p.status, 117))) break;
+          tc_fence_after();
+          const uint64_t wd = desc0 + (uint64_t)(st * (Lay::STAGE / 16)), xd = wd + A_BYTES / 16;      // addresses count 16 bytes
+          if (FP8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool fresh = k == 0 || (k == 2 && piece.down);      // a stage has one accumulator, in the down products two
+              if (fresh) {
+                if (k > 0) commit_slot();
+                next_slot();
+                if (!ok) break;
+              }
+              mma_8bit(tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, fresh ? 0u : 1u);
+            }
+            if (!ok) break;
+            tc_commit(empty + st);
+            commit_slot();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma(tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, (s > piece.s0 || k > 0) ? 1u : 0u);
+            tc_commit(empty + st);
+          }
+          if (++st == p.stages) { st = 0; phase ^= 1u; }
+        }
+        if (!FP8 && ok) commit_slot();
+      }
+    }
+  } else {
+    const int et = threadIdx.x - 64, ew = warp - 2;
+    const uint32_t quad = warp & 3;
+    const int row = (int)quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + ((quad * 32u) << 16);
+    int slot = 0;
+    uint32_t slot_phase = 0u, meet_phase = 0u;
+    bool ok = true;
+    // the epilogue threads meet (a bounded wait, so that none is left behind when another one gives up)
+    auto meet_all = [&]() {
+      mbar_arrive(&meet);
+      ok = ok && mbar_wait(&meet, meet_phase, abort_flag, p.status, 118);
+      meet_phase ^= 1u;
+    };
+    for (int np = 0; ok; ++np) {
+      const int q = np % QUEUE;
+      if (!(ok = mbar_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
+      const Piece piece = queue[q];
+      mbar_arrive(q_empty + q);
+      if (piece.down < 0) break;
+      const int c0 = first[piece.a], cnt = first[piece.a + 1] - c0, e = active[piece.a];
+      const int cols = piece.down ? (cnt + 15) / 16 * 16 : NB;
+      float acc[FP8 ? NB : 1];
+      if (FP8) {
+#pragma unroll
+        for (int c = 0; c < NB; ++c) acc[c] = 0.f;
+        if (piece.down) {
+          // the scales of this expert's u, once its first product says that the up products are done; nobody reads the last piece's any more
+          ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+          meet_all();
+          const int blocks = Lay::blocks(p.ff);
+          for (int i = et; i < blocks * NB; i += 128) {
+            const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
+            ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
+          }
+          meet_all();
+        }
+        // the weights' scale of this thread's row
+        const int rows_all = piece.down ? p.d : ffu, K = piece.down ? p.ff : p.d, KB = (K + 127) / 128;
+        const int w_row = piece.down ? piece.tile * TILE + row : (GLU && row >= 64 ? p.ff + piece.tile * 64 + row - 64 : piece.tile * OUT + row);
+        const size_t ws_at = ((size_t)e * ((rows_all + 127) / 128) + min(w_row, rows_all - 1) / 128) * KB;
+        const float* ws = piece.down ? p.sd : p.su;
+        float w_next = block_scale(ws, p.e8m0, ws_at + piece.s0);
+        auto take = [&]() -> uint32_t {                        // the next accumulator
+          if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+          const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
+          if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+          return from;
+        };
+        for (int s = piece.s0; s < piece.s1 && ok; ++s) {
+          const float w = w_next;
+          if (s + 1 < piece.s1) w_next = block_scale(ws, p.e8m0, ws_at + s + 1);
+          const int slot_a = slot;
+          const uint32_t from = take();
+          if (!piece.down) {
+            tc_fence_after();
+#pragma unroll
+            for (int cc = 0; cc < NB; cc += 16) {
+              uint32_t hi[16], lo[16];
+              tc_ld16(from + cc, hi);
+              tc_ld16(from + NB + cc, lo);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                acc[cc + i] = fmaf(fmaf(__uint_as_float(lo[i]), 0.0625f, __uint_as_float(hi[i])), w, acc[cc + i]);
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty + slot_a);
+          } else {
+            const int slot_b = slot;
+            const uint32_t from_b = take();
+            tc_fence_after();
+            const bool two = s * 128 + 64 < K;                 // (a block behind the rows' ends has no scales)
+            const float4* fa = reinterpret_cast<const float4*>(ys + 2 * s * NB);
+            const float4* fb = reinterpret_cast<const float4*>(ys + (two ? 2 * s + 1 : 2 * s) * NB);
+            const float wb = two ? w : 0.f;
+#pragma unroll
+            for (int cc = 0; cc < NB; cc += 16)
+              if (cc < cols) {
+                uint32_t hi[16], lo[16], hb[16], lb[16];
+                tc_ld16(from + cc, hi);
+                tc_ld16(from + cols + cc, lo);
+                tc_ld16(from_b + cc, hb);
+                tc_ld16(from_b + cols + cc, lb);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float4 x = fa[cc / 4 + i], z = fb[cc / 4 + i];
+                  const float fx[4] = {x.x, x.y, x.z, x.w}, fz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const int c = 4 * i + j;
+                    const float va = fmaf(__uint_as_float(lo[c]), 0.0625f, __uint_as_float(hi[c]));
+                    const float vb = fmaf(__uint_as_float(lb[c]), 0.0625f, __uint_as_float(hb[c]));
+                    acc[cc + c] = fmaf(va * fx[j], w, fmaf(vb * fz[j], wb, acc[cc + c]));
+                  }
+                }
+              }
+            tc_fence_before();
+            mbar_arrive(acc_empty + slot_a);
+            mbar_arrive(acc_empty + slot_b);
+          }
+        }
+      } else {
+        ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+        tc_fence_after();
+      }
+      if (!piece.down) {
+        // all columns to shared memory, then the activation, entry by entry
+        meet_all();                                            // the last piece's tile has been read
+        if (FP8) {
+#pragma unroll
+          for (int c = 0; c < NB; ++c) tile[c * TILE + row] = acc[FP8 ? c : 0];
+        } else if (ok) {
+#pragma unroll
+          for (int cc = 0; cc < NB; cc += 16) {
+            uint32_t v[16];
+            tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) tile[(cc + c) * TILE + row] = __uint_as_float(v[c]);
+          }
+        }
+        meet_all();
+        const int blocks = Lay::blocks(p.ff);
+        for (int i = ew; i < cnt; i += 4) {
+          const float* from = tile + tok[c0 + i] * TILE;
+          const float hs = FP8 ? p.hs[tok[c0 + i]] : 1.f;
+#pragma unroll
+          for (int b = 0; b < OUT / 64; ++b) {
+            const int f0 = piece.tile * OUT + 64 * b;          // 64 numbers of u: two per lane
+            float v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float z = from[64 * b + 32 * j + lane] * hs;
+              v[j] = GLU ? z / (1.f + expf(-z)) * (from[64 + 32 * j + lane] * hs) : gelu_erf(z);
+            }
+            if (FP8) {
+              uint32_t m = 0u;
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (f0 + 32 * j + lane < p.ff) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+              m = __reduce_max_sync(0xffffffffu, m);
+              const int code = scale_code(m);
+              const float inv = inverse_scale(code);
+              uint32_t hi, lo;
+              two_e4m3x2(v[0], v[1], inv, hi, lo);
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (f0 + 32 * j + lane < p.ff) {
+                  unsigned char* to = p.u + (size_t)(c0 + i) * p.ff + f0 + 32 * j + lane;
+                  to[0] = (unsigned char)(hi >> (8 * j));
+                  to[(size_t)slots * p.ff] = (unsigned char)(lo >> (8 * j));
+                }
+              if (lane == 0 && f0 < p.ff) p.us[(size_t)(c0 + i) * blocks + f0 / 64] = scale_value(code);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (f0 + 32 * j + lane < p.ff)
+                  reinterpret_cast<__nv_bfloat16*>(p.u)[(size_t)(c0 + i) * p.ff + f0 + 32 * j + lane] = __float2bfloat16_rn(v[j]);
+            }
+          }
+        }
+        fence_async_all();                                     // u is read through the async proxy
+        __threadfence();
+        meet_all();
+        if (et == 0 && ok) atomicAdd(p.counters + 1, 1);
+      } else {
+        const int col = piece.tile * TILE + row;
+        float* y = p.y + ((size_t)piece.split * entries + c0) * p.d + col;
+        if (FP8) {
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+            if (c < cnt && col < p.d) y[(size_t)c * p.d] = acc[FP8 ? c : 0];
+        } else if (ok) {
+#pragma unroll
+          for (int cc = 0; cc < NB; cc += 16)
+            if (cc < cols) {
+              uint32_t v[16];
+              tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c)
+                if (cc + c < cnt && col < p.d) y[(size_t)(cc + c) * p.d] = __uint_as_float(v[c]);
+            }
+        }
+        __threadfence();
+        meet_all();
+        if (et == 0 && ok) atomicAdd(p.counters + 3, 1);
+      }
+      if (!FP8) {
+        tc_fence_before();
+        mbar_arrive(acc_empty + slot);
+        if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+      }
+    }
+    // ---- when every down piece of every CTA is done: the sums over the choices, four columns of a token per thread
+    if (et == 0 && ok && !wait_for(p.counters + 3, down_pieces, p.status, abort_flag)) ok = false;
+    __threadfence();
+    meet_all();
+    const int quads = p.d / 4, parts = p.top * splits;
+    for (long long i = (long long)blockIdx.x * 128 + et; ok && i < (long long)p.n * quads; i += (long long)gridDim.x * 128) {
+      const int t = (int)(i / quads), c4 = 4 * (int)(i - (long long)t * quads);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p.add != nullptr) sum = scaled(four_bf16(p.add + (size_t)t * p.d + c4), p.gate != nullptr ? 1.f / (1.f + expf(-p.gate[t])) : 1.f);
+      int k = 0, split = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < parts; i0 += 8) {                  // eight (choice, slice) results in flight
+        float4 x[8];
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          w[j] = 0.f;
+          x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + j < parts) {
+            const int at = pos[t * p.top + k];
+            w[j] = p.wts[t * p.top + k];
+            if (at >= 0) x[j] = __ldcg(reinterpret_cast<const float4*>(p.y + ((size_t)split * entries + at) * p.d + c4));
+            else if (split == 0) x[j] = four_bf16(p.h + (size_t)t * p.d + c4);
+          }
+          if (++split == splits) { split = 0; ++k; }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          sum = make_float4(fmaf(w[j], x[j].x, sum.x), fmaf(w[j], x[j].y, sum.y), fmaf(w[j], x[j].z, sum.z), fmaf(w[j], x[j].w, sum.w));
+      }
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+      *reinterpret_cast<uint2*>(p.out + (size_t)t * p.d + c4) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// rows x K numbers of one or two bytes; box = box_rows x 128 bytes, 128-byte swizzle; what lies outside reads as 0
+bool make_map(CUtensorMap* map, const void* base, long long rows, int K, int bytes, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)K * bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  return fn(map, bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
+            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, bool GLU, int NB>
+int launch_experts(const CUtensorMap* maps, LayerParams p, cudaStream_t stream) {
+  using Lay = Layout<FP8, NB>;
+  const size_t fixed = 1024 + Lay::fixed(p.ff, p.n * p.top, p.E);
+  if (fixed + 3 * (size_t)Lay::STAGE > SMEM_BUDGET) return (int)cudaErrorInvalidValue;
+  const size_t room = (SMEM_BUDGET - fixed) / Lay::STAGE;
+  p.stages = room > MAX_STAGES ? MAX_STAGES : (int)room;
+  static bool set_dev[bspec::kMaxDevices] = {};
+  bool& set = set_dev[bspec::current_device()];
+  if (!set) {
+    const cudaError_t e = cudaFuncSetAttribute(moe_layer_experts_kernel<FP8, GLU, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  BSPEC_LAUNCH((moe_layer_experts_kernel<FP8, GLU, NB>), bspec::sm_count(), LAYER_THREADS, fixed + (size_t)p.stages * Lay::STAGE, stream,
+               maps[0], maps[1], maps[2], maps[3], p);
+  return BSPEC_LAUNCH_CHECK();
 }
 
 }  // namespace
 
-// counters: 4 ints, ids [n top], wts [n top] and gate [n] floats: the results of the router and of its choice, and zeroed counters.
-// rows: of the router, C = experts and identity experts, then perhaps one for the gate.
-BSPEC_API int bspec_moe_layer_route(const void* h, int n, int d, const void* router, int rows, const void* corr, int corr_dtype, int C,
-                                    int G, int keep, int top, float scale, int rule, int* ids, float* wts, float* gate, int* counters,
-                                    cudaStream_t stream) {
+namespace {
+// Places of a call's intermediate results in its scratch (counters at 0): expert numbers, weights, gate logits, the tokens' 8-bit numbers and their
+// scales, u and its scales, the experts' results.  Returns the size.
+enum { AT_IDS, AT_WTS, AT_GATE, AT_HQ, AT_HS, AT_U, AT_US, AT_Y, AT_PARTS };
+long long places(int n, int d, int ff, int top, bool fp8, long long (&at)[AT_PARTS]) {
+  const long long slots = (long long)n * top, blocks_ff = (ff + 63) / 64;
+  const long long bytes[AT_PARTS] = {4 * slots, 4 * slots, 4ll * n, fp8 ? 2ll * n * d : 0, fp8 ? 4ll * n : 0,
+                                     2 * slots * ff, fp8 ? 4 * slots * blocks_ff : 0, 4 * MAX_SPLITS * slots * d};
+  long long size = 16;
+  for (int i = 0; i < AT_PARTS; ++i) {
+    at[i] = (size + 127) / 128 * 128;
+    size = at[i] + bytes[i];
+  }
+  return size;
+}
+}  // namespace
+
+// Bytes of scratch of a call.
+BSPEC_API long long bspec_moe_layer_scratch(int n, int d, int ff, int top, int fp8) {
+  long long at[AT_PARTS];
+  return places(n, d, ff, top, fp8 != 0, at);
+}
+
+// h, add (may be null), out: bfloat16 [n, d].  router: `rows` rows, C = experts and identity experts, then perhaps one (rows = C + 1) whose
+// logit's sigmoid multiplies add.  corr (may be null): C numbers.  wu [E, ff, d] (glu: [E, 2 ff, d]), wd [E, d, ff]: bfloat16, or e4m3 with
+// su, sd, the scales of their 128 x 128 blocks (float32, or 8-bit exponents with e8m0).  status: one int on the device, 0 unless a
+// bounded wait ran out.
+BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, int rows, const void* corr, int corr_dtype, int C, int G,
+                              int keep, int top, float scale, int rule, const void* wu, const void* wd, const void* su, const void* sd,
+                              int e8m0, int E, int ff, int glu, const void* add, void* out, void* scratch, int* status, cudaStream_t stream) {
   if (n <= 0) return 0;
-  if (n > LAYER_TOKENS || d <= 0 || d % 8 != 0 || C <= 0 || C > MAX_EXPERTS || rows < C || rows > C + 1 || top <= 0 || top > C || G <= 0 || C % G ||
-      keep <= 0 || keep > G || (long long)keep * (C / G) < top || (reinterpret_cast<uintptr_t>(h) & 15) ||
-      (reinterpret_cast<uintptr_t>(router) & 15))
+  const bool fp8 = su != nullptr;
+  const int unit = fp8 ? 16 : 8, bytes = fp8 ? 1 : 2, ffu = glu ? 2 * ff : ff;
+  if (n > LAYER_TOKENS || d <= 0 || ff <= 0 || d % unit || ff % unit || E <= 0 || C < E || C > MAX_EXPERTS || rows < C || rows > C + 1 || top <= 0 ||
+      top > C || G <= 0 || C % G || keep <= 0 || keep > G || (long long)keep * (C / G) < top || (fp8 && sd == nullptr) || (rows > C && add == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(wu) | reinterpret_cast<uintptr_t>(wd) |
+        reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(add)) & 15) ||
+      (long long)E * ffu > 0x7fffffff - 256 || (long long)E * d > 0x7fffffff - 256)
     return (int)cudaErrorInvalidValue;
+  long long at[AT_PARTS];
+  places(n, d, ff, top, fp8, at);
+  char* base = (char*)scratch;
+  int* counters = (int*)base;
+  LayerParams p = {};
+  p.su = (const float*)su; p.sd = (const float*)sd; p.e8m0 = e8m0;
+  p.ids = (const int*)(base + at[AT_IDS]); p.wts = (const float*)(base + at[AT_WTS]);
+  p.gate = rows > C ? (const float*)(base + at[AT_GATE]) : nullptr;
+  p.h = (const __nv_bfloat16*)h; p.add = (const __nv_bfloat16*)add;
+  p.hs = (const float*)(base + at[AT_HS]); p.u = (unsigned char*)(base + at[AT_U]); p.us = (float*)(base + at[AT_US]);
+  p.y = (float*)(base + at[AT_Y]);
+  p.out = (__nv_bfloat16*)out; p.counters = counters; p.status = status;
+  p.n = n; p.d = d; p.ff = ff; p.E = E; p.top = top;
+  CUtensorMap maps[4];
+  if (!make_map(maps, wu, (long long)E * ffu, d, bytes, 64) || !make_map(maps + 1, wd, (long long)E * d, ff, bytes, 64) ||
+      !make_map(maps + 2, fp8 ? (const void*)(base + at[AT_HQ]) : h, fp8 ? 2 * n : n, d, bytes, 16) ||
+      !make_map(maps + 3, p.u, (fp8 ? 2ll : 1ll) * n * top, ff, bytes, 16))
+    return (int)cudaErrorInvalidValue;
+
   const int tiles = (rows + 15) / 16, steps = (d + 31) / 32;
-  int slices = ROUTE_CLUSTER * ROUTE_WARPS / tiles;              // of k: as many as there are warps left
+  int slices = ROUTE_CLUSTER * ROUTE_WARPS / tiles;              // of the router's k: as many as there are warps left
   if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;        // at least one batch of loads each
   if (slices < 1) slices = 1;
   const size_t smem = ((size_t)tiles * slices * 16 * ROUTE_TOKENS + (size_t)(ROUTE_WARPS * 3 + 1) * C) * 4;
@@ -625,45 +822,15 @@ BSPEC_API int bspec_moe_layer_route(const void* h, int n, int d, const void* rou
   }
   BSPEC_LAUNCH((moe_layer_route_kernel), ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS), 32 * ROUTE_WARPS, smem, stream,
                (const __nv_bfloat16*)h, n, d, (const __nv_bfloat16*)router, rows, slices, corr, corr_dtype, C, G, keep, top, scale, rule,
-               ids, wts, gate, counters);
-  return BSPEC_LAUNCH_CHECK();
-}
-
-// The experts' products and the weighted sum, after bspec_moe_layer_route on the same stream.  su, sd: scales of the 128 x 128 blocks of
-// e4m3 weights (float32, or 8-bit exponents with e8m0), null for bfloat16 weights.  u: [n top, ff] bfloat16 scratch.
-BSPEC_API int bspec_moe_layer_experts(const void* h, int n, int d, const void* wu, const void* wd, const void* su, const void* sd, int e8m0,
-                                      int E, int ff, int glu, const int* ids, const float* wts, int top, const float* gate, const void* add,
-                                      void* u, void* out, int* counters, int* status, cudaStream_t stream) {
-  if (n <= 0) return 0;
-  const bool fp8 = su != nullptr;
-  const int unit = fp8 ? 16 : 8;
-  if (n > LAYER_TOKENS || d <= 0 || ff <= 0 || d % unit || ff % unit || E <= 0 || E > MAX_EXPERTS || top <= 0 || (fp8 && sd == nullptr) ||
-      ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(wu) | reinterpret_cast<uintptr_t>(wd) | reinterpret_cast<uintptr_t>(u)) & 15))
-    return (int)cudaErrorInvalidValue;
-  LayerParams p = {};
-  p.h = (const __nv_bfloat16*)h; p.wu = (const unsigned char*)wu; p.wd = (const unsigned char*)wd;
-  p.su = su; p.sd = sd; p.e8m0 = e8m0; p.ids = ids; p.wts = wts; p.gate = gate; p.add = (const __nv_bfloat16*)add;
-  p.u = (__nv_bfloat16*)u; p.out = (__nv_bfloat16*)out; p.counters = counters; p.status = status;
-  p.n = n; p.d = d; p.ff = ff; p.E = E; p.top = top;
-  p.stages = 2;
-  while (p.stages < MAX_STAGES && layer_smem(n, E, top, p.stages + 1) <= SMEM_BUDGET) ++p.stages;
-  const size_t smem = layer_smem(n, E, top, p.stages);
-  if (smem > SMEM_BUDGET) return (int)cudaErrorInvalidValue;
-#define LE(F, G)                                                                                                          \
-  do {                                                                                                                    \
-    static bool set_dev[bspec::kMaxDevices] = {};                                                                         \
-    bool& set = set_dev[bspec::current_device()];                                                                         \
-    if (!set) {                                                                                                           \
-      const cudaError_t e = cudaFuncSetAttribute(moe_layer_experts_kernel<F, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET); \
-      if (e != cudaSuccess) return (int)e;                                                                                \
-      set = true;                                                                                                         \
-    }                                                                                                                     \
-    BSPEC_LAUNCH((moe_layer_experts_kernel<F, G>), bspec::sm_count(), LAYER_THREADS, smem, stream, p);                    \
-  } while (0)
-  if (fp8) { if (glu) LE(true, true); else LE(true, false); }
-  else { if (glu) LE(false, true); else LE(false, false); }
-#undef LE
-  return BSPEC_LAUNCH_CHECK();
+               (int*)(base + at[AT_IDS]), (float*)(base + at[AT_WTS]), (float*)(base + at[AT_GATE]), counters,
+               fp8 ? (uint8_t*)(base + at[AT_HQ]) : (uint8_t*)nullptr, (float*)(base + at[AT_HS]));
+  const int e = BSPEC_LAUNCH_CHECK();
+  if (e != 0) return e;
+#define LN(F, G) (n <= 16 ? launch_experts<F, G, 16>(maps, p, stream) : n <= 32 ? launch_experts<F, G, 32>(maps, p, stream) \
+                                                                              : launch_experts<F, G, 64>(maps, p, stream))
+  if (fp8) return glu ? LN(true, true) : LN(true, false);
+  return glu ? LN(false, true) : LN(false, false);
+#undef LN
 }
 
 BSPEC_DEFINE_TRACE_SETTER(bspec_trace_set_moe_layer)

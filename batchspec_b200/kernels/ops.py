@@ -132,10 +132,9 @@ _SIGNATURES = {
                            c_int, c_void_p],
     "bspec_gemm_fp8": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
-    "bspec_moe_layer_route": [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
-    "bspec_moe_layer_experts": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
-                                c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "bspec_moe_layer_scratch": [c_int] * 5,
+    "bspec_moe_layer": [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
+                        c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "bspec_moe_route": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                         c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_void_p],
     "bspec_moe_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
@@ -1255,7 +1254,8 @@ WAIT_CODES = ((1, 1, "GEMM: stage never freed"), (2, 2, "GEMM: operands never ar
               (91, 91, "float32 product of few rows: stage never freed"),
               (92, 92, "float32 product of few rows: operands never arrived"),
               (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"),
-              (111, 112, "routed layer of a few tokens: the up products never completed, or weights never arrived"))
+              (111, 111, "routed layer of a few tokens: the up products never completed"),
+              (113, 120, "routed layer of a few tokens: a stage, an accumulator or a piece of work never came or was never freed"))
 
 
 def wait_meaning(code: int) -> str:
@@ -1911,8 +1911,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     ``router`` [E + identity (+ 1)] rows: the experts, then ``identity`` experts whose result is h itself, then, with ``add_gated``, the row
     whose logit's sigmoid multiplies ``add``.  ``w_up`` [E, ff, d] (``glu``: [E, 2 ff, d], gates first), ``w_down`` [E, d, ff]: bfloat16,
     or float8_e4m3fn with ``up_scale`` / ``down_scale``, a float32 or float8_e8m0fnu scale per 128 x 128 block of every expert (both of one
-    type; what ``quantize_fp8`` makes of the stacked matrices).  8-bit weights have to be finite numbers (a NaN shows through its block's
-    scale, as ``quantize_fp8`` leaves it).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps: ``moe_route`` and
+    type; what ``quantize_fp8`` makes of the stacked matrices).  With 8-bit weights the activations keep
+    8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps: ``moe_route`` and
     ``moe_experts``."""
     stream = _stream_of(h, router, correction, w_up, w_down, up_scale, down_scale, add)
     if h.dim() != 2 or w_up.dim() != 3 or w_down.dim() != 3 or router.dim() != 2:
@@ -1941,8 +1941,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
             raise KernelError(f"moe_layer: {name} has to be contiguous and to start on a 16-byte boundary")
     if correction is not None and (tuple(correction.shape) != (many,) or not correction.is_contiguous()):
         raise KernelError(f"moe_layer: correction has to be a dense vector of {many} numbers")
-    if add is not None and (add.shape != h.shape or add.dtype != h.dtype or not add.is_contiguous()):
-        raise KernelError("moe_layer: add has to be a dense bfloat16 matrix like h")
+    if add is not None and (add.shape != h.shape or add.dtype != h.dtype or not add.is_contiguous() or add.data_ptr() % 16):
+        raise KernelError("moe_layer: add has to be a dense bfloat16 matrix like h, on a 16-byte boundary")
     e8m0 = 0
     if fp8:
         if up_scale is None or down_scale is None:
@@ -1960,20 +1960,15 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     if n == 0:
         return out
     lib = load_library(features=("moe",))
-    # counters, expert numbers, weights and gate logits of this call, then u: a buffer of its own, so that calls on other streams or in
-    # other graphs share nothing
-    slots = n * top
-    head = (4 + 2 * slots + n + 3) // 4 * 16
-    scratch = torch.empty((head + 2 * slots * ff,), dtype=torch.uint8, device=h.device)
-    at = scratch.data_ptr()
-    ids, wts, gate, u = at + 16, at + 16 + 4 * slots, at + 16 + 8 * slots, at + head
+    # everything between the two kernels, counters too: a buffer of its own, so that calls on other streams or in other graphs share nothing
+    scratch = torch.empty((lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8)),), dtype=torch.uint8, device=h.device)
     rule = (1 if softmax_top else 2 if softmax else 0) + (4 if group_max else 0) + (8 if renormalise else 0)
-    _check(lib.bspec_moe_layer_route(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),
-                                     _dtype_code(correction.dtype) if correction is not None else F32, many, int(n_groups), int(keep),
-                                     int(top), float(scale), rule, ids, wts, gate, at, stream), "moe_layer_route")
-    _check(lib.bspec_moe_layer_experts(h.data_ptr(), n, d, w_up.data_ptr(), w_down.data_ptr(), _ptr(up_scale), _ptr(down_scale), e8m0, E, ff,
-                                       int(bool(glu)), ids, wts, int(top), gate if add_gated else None, _ptr(add), u, out.data_ptr(), at,
-                                       _status_word(h.device).data_ptr(), stream), "moe_layer_experts")
+    _check(lib.bspec_moe_layer(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),
+                               _dtype_code(correction.dtype) if correction is not None else F32, many, int(n_groups), int(keep), int(top),
+                               float(scale), rule, w_up.data_ptr(), w_down.data_ptr(), _ptr(up_scale), _ptr(down_scale), e8m0, E, ff,
+                               int(bool(glu)), _ptr(add), out.data_ptr(), scratch.data_ptr(), _status_word(h.device).data_ptr(), stream),
+           "moe_layer")
+    count_launches(1)
     return out
 
 
