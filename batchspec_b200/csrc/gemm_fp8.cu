@@ -17,6 +17,9 @@
 #include "umma.cuh"
 
 using namespace bspec;
+#ifndef FORCE_WIDE
+#define FORCE_WIDE 1
+#endif
 
 namespace {
 
@@ -24,8 +27,8 @@ constexpr int KBYTES = 128;            // k per stage: one scale block, one 128-
 constexpr int TILE_ROWS = 128;
 constexpr int FEW_THREADS = 192;       // TMA warp, MMA warp, 4 epilogue warps
 constexpr int FEW_WINDOW = 32;         // k blocks whose scales wait in shared memory at a time
-constexpr int MANY_THREADS = 320;      // TMA warp, MMA warp, 8 epilogue warps
-constexpr int MANY_BN = 256, MANY_STAGES = 4;
+constexpr int many_threads(int bn) { return 128 + 2 * bn; }  // TMA warp, MMA warp, two idle ones, four epilogue warps for every 64 columns
+constexpr int many_stages(int bn) { return bn == 192 ? 5 : 6; }
 
 struct Scales {
   const void* p;
@@ -62,6 +65,17 @@ __device__ __forceinline__ uint32_t e4m3_desc(int bn) {
 __device__ __forceinline__ void put(void* C, int out_f32, size_t at, float v) {
   if (out_f32) reinterpret_cast<float*>(C)[at] = v;
   else reinterpret_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
+}
+// sixteen numbers as bfloat16, 32 bytes in one store: a whole sector, where two of 16 bytes would be two partial ones
+__device__ __forceinline__ void put16(__nv_bfloat16* to, const float* v) {
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    w[j] = *reinterpret_cast<uint32_t*>(&h);
+  }
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 // Let copies in flight land before the CTA gives up its shared memory (after a wait ran out).
 __device__ __forceinline__ void drain(uint64_t* full, int armed, int stages) {
@@ -106,7 +120,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(acc_full + b, 1);
-      mbar_init(acc_empty + b, 128);
+      mbar_init(acc_empty + b, 4);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -200,7 +214,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
       }
       tc_fence_before();
-      mbar_arrive(acc_empty + b);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + b);               // one arrival per warp: those of its lanes would come one after the other
     }
     const int row = (int)quad * 32 + lane, n = tile_n * TILE_ROWS + row;
     if (p.splits == 1) {
@@ -264,10 +279,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens
-__global__ void __launch_bounds__(MANY_THREADS, 1)
+template <int MANY_BN>
+__global__ void __launch_bounds__(many_threads(MANY_BN), 1)
 gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
   constexpr int X_BYTES = TILE_ROWS * KBYTES, W_BYTES = MANY_BN * KBYTES, STAGE = X_BYTES + W_BYTES;
-  constexpr int NB = 2;
+  constexpr int MANY_STAGES = many_stages(MANY_BN), NB = 2, COLS = 64;   // accumulators; columns of an epilogue thread
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + MANY_STAGES * STAGE);
@@ -285,7 +301,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(acc_full + b, 1);
-      mbar_init(acc_empty + b, 256);
+      mbar_init(acc_empty + b, MANY_BN / 16);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -302,6 +318,9 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   const int nkb = (p.K + KBYTES - 1) / KBYTES;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
 
+  if (warp < 4) {
+  // registers: the first four warps leave theirs to the others (512 threads x 128 = 128 x 40 + 384 x 152 + 2,048 to spare)
+  if (MANY_BN == 192) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     if (lane == 0) {
       int armed = 0;
@@ -338,63 +357,61 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         }
       }
     }
+  }
   } else {
+    if (MANY_BN == 192) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     const uint32_t quad = warp & 3;
-    const int half = (warp - 2) >> 2;                                   // columns 128 half .. of the tile: one row of W's scales
-    const uint32_t lane_base = tmem_base + ((quad * 32u) << 16) + (uint32_t)(half * 128);
+    const int group = (warp - 4) >> 2;                                  // columns 64 group .. of the tile: in one row of W's scales
+    const uint32_t lane_base = tmem_base + ((quad * 32u) << 16) + (uint32_t)(group * COLS);
     const int row = (int)quad * 32 + lane;
-    int i = 0;
+    int b = 0;
+    uint32_t phase = 0u;
     bool ok = true;
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int m = (int)(t % p.tiles_m) * TILE_ROWS + row, n0 = (int)(t / p.tiles_m) * MANY_BN + half * 128;
+      const int m = (int)(t % p.tiles_m) * TILE_ROWS + row, n0 = (int)(t / p.tiles_m) * MANY_BN + group * COLS;
       const long long srow = min(m, p.M - 1), wrow = min(n0, p.N - 1) / 128;
-      uint64_t acc[64];
+      float acc[COLS];
 #pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0ull;
-      float f_next = scale_at(p.xs, srow, 0) * scale_at(p.ws, wrow, 0);
-      for (int kb = 0; kb < nkb; ++kb, ++i) {
-        const float f = f_next;
-        if (kb + 1 < nkb) f_next = scale_at(p.xs, srow, kb + 1) * scale_at(p.ws, wrow, kb + 1);
-        const uint64_t ff = pack2(f, f);
-        const int b = i % NB;
-        if (!(ok = mbar_wait(acc_full + b, (uint32_t)(i / NB) & 1u, abort_flag, p.status, 108))) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t v[32];
-          tc_ld32(lane_base + (uint32_t)(b * MANY_BN + c0), v);
-          tc_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c0 / 2 + j] = fma2(pack2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), ff, acc[c0 / 2 + j]);
+      for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+      float x_next = scale_at(p.xs, srow, 0), w_next = scale_at(p.ws, wrow, 0);
+      uint32_t v0[32], v1[32];
+      ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108);
+      tc_fence_after();
+      tc_ld32(lane_base + (uint32_t)(b * MANY_BN), v0);
+      for (int kb = 0; kb < nkb && ok; ++kb) {
+        const float f = x_next * w_next;
+        if (kb + 1 < nkb) {
+          x_next = scale_at(p.xs, srow, kb + 1);
+          w_next = scale_at(p.ws, wrow, kb + 1);
         }
+        // 32 columns are on their way while the 32 before them are added, from block to block too
+        tc_wait_ld();
+        tc_ld32(lane_base + (uint32_t)(b * MANY_BN + 32), v1);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v0[j]), f, acc[j]);
+        tc_wait_ld();
         tc_fence_before();
-        mbar_arrive(acc_empty + b);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + b);
+        if (++b == NB) { b = 0; phase ^= 1u; }
+        if (kb + 1 < nkb) {
+          ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108);
+          tc_fence_after();
+          tc_ld32(lane_base + (uint32_t)(b * MANY_BN), v0);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v1[j]), f, acc[32 + j]);
       }
+      tc_wait_ld();
       if (ok && m < p.M) {
         const size_t base = (size_t)m * p.N + n0;
-        if (!p.out_f32 && p.N % 8 == 0 && n0 + 128 <= p.N) {
-          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.C) + base);
+        if (!p.out_f32 && p.N % 16 == 0 && n0 + COLS <= p.N) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float lo, hi;
-              unpack2(acc[4 * c + j], lo, hi);
-              __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-              w[j] = *reinterpret_cast<uint32_t*>(&h);
-            }
-            dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int c = 0; c < COLS; c += 16) put16(reinterpret_cast<__nv_bfloat16*>(p.C) + base + c, acc + c);
         } else {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            float lo, hi;
-            unpack2(acc[c], lo, hi);
-            if (n0 + 2 * c < p.N) put(p.C, p.out_f32, base + 2 * c, lo);
-            if (n0 + 2 * c + 1 < p.N) put(p.C, p.out_f32, base + 2 * c + 1, hi);
-          }
+          for (int c = 0; c < COLS; ++c)
+            if (n0 + c < p.N) put(p.C, p.out_f32, base + c, acc[c]);
         }
       }
     }
@@ -404,6 +421,258 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ many tokens, powers of two as scales
+// Both matrices' scales in 8 bits (e8m0): the tensor cores take them (kind::mxf8f6f4, a scale per 32 k, here the same one four times), nothing is
+// added outside of them, and the sums of a whole row stay in tensor memory.  What then bounds a product is the way from the L2 into an SM (64 bytes
+// a clock): a 128 x 256 tile of one CTA asks for 48 KB per 128 k, 750 clocks where its products take 512.  So two CTAs work on one tile of
+// 256 x PAIR_BN (cta_group::2): each keeps its own 128 rows of X and half the rows of W, 30 KB per 128 k for 448 clocks of products.
+//   TMA warp      its CTA's halves of a stage; the bytes are counted on the first CTA's barrier
+//   MMA warp      (first CTA) copies the scales of both CTAs into their tensor memory and issues the products for both
+//   scale warps   bring the scales of four stages into the form that is copied: 32 lanes x 16 bytes, rows l, l + 32, l + 64, l + 96, a byte per
+//                 stage (the products of a stage name its byte)
+//   epilogue      eight warps: 128 rows x half the columns, read at once, freed, converted and stored while the next tile's products run
+constexpr int PAIR_BN = 224, PAIR_STAGES = 7, PAIR_SF_SLOTS = 4, PAIR_SF_BUFS = 5, PAIR_THREADS = 448;
+constexpr int PAIR_X = TILE_ROWS * KBYTES, PAIR_W = PAIR_BN / 2 * KBYTES, PAIR_STAGE = PAIR_X + PAIR_W;
+constexpr int PAIR_SF = 512 + 1024;          // the scales of four stages: 128 rows of X, 256 of W
+constexpr int PAIR_SF_COL = 2 * PAIR_BN;     // tensor memory columns: two accumulators, then five places for scales, 4 + 8 columns
+                                             // each: the stages in flight reach over three of them at most
+
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {     // the same place in another CTA's shared memory
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(s32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_in(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(s32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+// The warp that issues products stays together, and one lane of it issues (`one`): what the instructions take from registers common to the
+// warp is then at hand.  Issued from a branch of a single lane they take some 200 clocks each.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
+}
+__device__ __forceinline__ void commit_pair(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+      ::"r"(s32(bar)), "h"((uint16_t)3), "r"(one) : "memory");
+}
+__device__ __forceinline__ void copy_scales(uint32_t one, uint32_t tmem, const void* smem) {
+  const uint64_t desc = (uint64_t)((s32(smem) & 0x3FFFFu) >> 4) | (8ull << 32) | (1ull << 46);     // 8-row groups 128 bytes apart, no swizzle
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem), "l"(desc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void mma_scaled(uint32_t one, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                           uint32_t sfb, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accum), "r"(one) : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  unsigned char* sf = smem + PAIR_STAGES * PAIR_STAGE;
+  __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], sf_full[PAIR_SF_SLOTS], sf_empty[PAIR_SF_SLOTS], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = blockIdx.x & 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PAIR_STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int s = 0; s < PAIR_SF_SLOTS; ++s) {
+      mbar_init(sf_full + s, 2);             // a scale warp of each CTA
+      mbar_init(sf_empty + s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + b, 1);
+      mbar_init(acc_empty + b, 16);          // the epilogue warps of both CTAs
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  // both CTAs run and have their barriers before one writes to the other
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  bspec::pdl_prologue(86);
+  const int nkb = (p.K + KBYTES - 1) / KBYTES;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      uint32_t phase = 0u;
+      bool ok = true;
+      for (long long t = pair; t < tiles && ok; t += pairs) {
+        const int m0 = (int)(t % p.tiles_m) * 256 + (int)rank * TILE_ROWS, n0 = (int)(t / p.tiles_m) * PAIR_BN + (int)rank * (PAIR_BN / 2);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!(ok = mbar_wait(empty + st, phase ^ 1u, abort_flag, p.status, 121))) break;
+          if (rank == 0) mbar_expect_tx(full + st, 2 * PAIR_STAGE);
+          const uint32_t bar = in_cta(full + st, 0);
+          unsigned char* at = smem + st * PAIR_STAGE;
+          tma_load_pair(at, &map_x, bar, kb * KBYTES, m0);
+          tma_load_pair(at + PAIR_X, &map_w, bar, kb * KBYTES, n0);
+          if (++st == PAIR_STAGES) { st = 0; phase ^= 1u; }
+        }
+      }
+      if (*abort_flag)                       // copies in flight land (they take microseconds) before the CTA ends
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t one = elect_one();
+      // float32 sums, e4m3 X and W, e8m0 scales, M = 256, N = PAIR_BN
+      const uint32_t idesc = ((uint32_t)(PAIR_BN >> 3) << 17) | (1u << 23) | (16u << 24);
+      int st = 0, b = 0, slot = 0, buf = 0;
+      uint32_t phase = 0u, acc_phase = 0u, sf_phase = 0u;
+      bool ok = true;
+      for (long long t = pair; t < tiles && ok; t += pairs) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(acc_empty + b, acc_phase ^ 1u, abort_flag, p.status, 122)))) break;
+        tc_fence_after();
+        uint32_t sfa = 0u, sfb = 0u;
+        for (int kb = 0; kb < nkb; ++kb) {
+          if ((kb & 3) == 0) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(sf_full + slot, sf_phase, abort_flag, p.status, 126)))) break;
+            tc_fence_after();
+            sfa = tmem_base + PAIR_SF_COL + buf * 12;
+            sfb = sfa + 4;
+            copy_scales(one, sfa, sf + slot * PAIR_SF);
+            copy_scales(one, sfb, sf + slot * PAIR_SF + 512);
+            copy_scales(one, sfb + 4, sf + slot * PAIR_SF + 1024);
+            commit_pair(one, sf_empty + slot);
+            if (++buf == PAIR_SF_BUFS) buf = 0;
+            if (++slot == PAIR_SF_SLOTS) { slot = 0; sf_phase ^= 1u; }
+          }
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(full + st, phase, abort_flag, p.status, 123)))) break;
+          tc_fence_after();
+          const uint32_t desc = idesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+          const uint64_t xd = smem_desc(smem + st * PAIR_STAGE), wd = smem_desc(smem + st * PAIR_STAGE + PAIR_X);
+#pragma unroll
+          for (int k = 0; k < KBYTES / 32; ++k)
+            mma_scaled(one, tmem_base + b * PAIR_BN, xd + 2 * k, wd + 2 * k, desc, sfa, sfb, (kb > 0 || k > 0) ? 1u : 0u);
+          commit_pair(one, empty + st);
+          if (++st == PAIR_STAGES) { st = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        commit_pair(one, acc_full + b);
+        if (++b == 2) { b = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else if (warp < 6) {
+    // groups of four stages go round the four warps, each with a place of its own; the next group's loads are on their way while this one waits
+    const uint8_t* xs = reinterpret_cast<const uint8_t*>(p.xs.p);
+    const uint8_t* ws = reinterpret_cast<const uint8_t*>(p.ws.p);
+    const int groups = (nkb + 3) / 4;
+    long long t = pair;
+    static_assert(PAIR_SF_SLOTS == 4, "a place per warp: one that fills another's would not know its turn by the barrier's parity");
+    const int slot = warp - 2;
+    int g = slot;
+    uint32_t phase = 0u;
+    bool ok = true;
+    uint32_t v[3][4];                        // X, W up to 128 rows of the tile and behind; rows lane, lane + 32, ...
+    auto fetch = [&]() {
+      while (g >= groups) {
+        g -= groups;
+        t += pairs;
+      }
+      if (t >= tiles) return;
+      const int tn = (int)(t / p.tiles_m), tm = (int)(t - (long long)tn * p.tiles_m);
+      const int m = tm * 256 + (int)rank * TILE_ROWS + lane, n = tn * PAIR_BN + lane, kb = 4 * g;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* from[3] = {xs + (long long)min(m + 32 * j, p.M - 1) * p.xs.ld, ws + (long long)(min(n + 32 * j, p.N - 1) / 128) * p.ws.ld,
+                                  ws + (long long)(min(n + 128 + 32 * j, p.N - 1) / 128) * p.ws.ld};
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          v[i][j] = 0u;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[i][j] |= (uint32_t)__ldg(from[i] + min(kb + k, nkb - 1)) << (8 * k);
+        }
+      }
+    };
+    fetch();
+    while (t < tiles && ok) {
+      uint4 w[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) w[i] = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+      g += 4;
+      fetch();
+      if (!(ok = mbar_wait(sf_empty + slot, phase ^ 1u, abort_flag, p.status, 124))) break;
+      unsigned char* to = sf + slot * PAIR_SF + lane * 16;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(to + 512 * i) = w[i];
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_in(in_cta(sf_full + slot, 0));
+      phase ^= 1u;
+    }
+  } else {
+    const uint32_t quad = warp & 3;
+    const int half = (warp - 6) >> 2;        // columns PAIR_BN / 2 half ..
+    constexpr int COLS = PAIR_BN / 2;
+    const int row = (int)quad * 32 + lane;
+    int b = 0;
+    uint32_t phase = 0u;
+    bool ok = true;
+    for (long long t = pair; t < tiles && ok; t += pairs) {
+      const int m = (int)(t % p.tiles_m) * 256 + (int)rank * TILE_ROWS + row, n0 = (int)(t / p.tiles_m) * PAIR_BN + half * COLS;
+      if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 125))) break;
+      tc_fence_after();
+      float acc[COLS];
+#pragma unroll
+      for (int c = 0; c < COLS; c += 16)
+        tc_ld16(tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * PAIR_BN + half * COLS + c), *reinterpret_cast<uint32_t(*)[16]>(acc + c));
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_in(in_cta(acc_empty + b, 0));
+      if (++b == 2) { b = 0; phase ^= 1u; }
+      if (m < p.M) {
+        const size_t base = (size_t)m * p.N + n0;
+        if (!p.out_f32 && p.N % 16 == 0 && n0 + COLS <= p.N) {
+#pragma unroll
+          for (int c = 0; c < COLS; c += 16) put16(reinterpret_cast<__nv_bfloat16*>(p.C) + base + c, acc + c);
+        } else {
+#pragma unroll
+          for (int c = 0; c < COLS; ++c)
+            if (n0 + c < p.N) put(p.C, p.out_f32, base + c, acc[c]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  // nobody leaves while the other may still use its memory
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
   }
 }
 
@@ -468,6 +737,21 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, Fp8Params p, 
   return BSPEC_LAUNCH_CHECK();
 }
 
+template <int BN>
+int launch_many(const CUtensorMap& map_x, const CUtensorMap& map_w, const Fp8Params& p, int sms, cudaStream_t stream) {
+  const size_t smem = 1024 + (size_t)many_stages(BN) * (TILE_ROWS + BN) * KBYTES + 256;
+  static bool set_dev[bspec::kMaxDevices] = {};
+  bool& set = set_dev[bspec::current_device()];
+  if (!set) {
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_many_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  BSPEC_LAUNCH((gemm_fp8_many_kernel<BN>), (unsigned)(tiles < sms ? tiles : sms), many_threads(BN), smem, stream, map_x, map_w, p);
+  return BSPEC_LAUNCH_CHECK();
+}
+
 }  // namespace
 
 // C [M, N] = X W^T with block scales.  X, W: e4m3, rows ldx / ldw bytes apart (multiples of 16, bases on 16 bytes); xs [M, ceil(K / 128)]
@@ -485,11 +769,31 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
   p.ws = {ws, ldws, ws_e8m0};
   p.M = M; p.N = N; p.K = K; p.out_f32 = out_f32; p.w_ahead = w_ahead;
   const int sms = bspec::sm_count();
-  const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + MANY_BN - 1) / MANY_BN;
+  if (xs_e8m0 && ws_e8m0 && M > 128) {
+    CUtensorMap map_x, map_w;
+    if (!make_map_bytes(&map_x, X, M, K, ldx, TILE_ROWS) || !make_map_bytes(&map_w, W, N, K, ldw, PAIR_BN / 2)) return (int)cudaErrorInvalidValue;
+    p.tiles_m = (M + 255) / 256;
+    p.tiles_n = (N + PAIR_BN - 1) / PAIR_BN;
+    const size_t smem = 1024 + (size_t)PAIR_STAGES * PAIR_STAGE + PAIR_SF_SLOTS * PAIR_SF;
+    static bool set_dev[bspec::kMaxDevices] = {};
+    bool& set = set_dev[bspec::current_device()];
+    if (!set) {
+      const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return (int)e;
+      set = true;
+    }
+    const long long tiles = (long long)p.tiles_m * p.tiles_n, pairs = sms / 2;
+    BSPEC_LAUNCH((gemm_fp8_pair_kernel), (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, smem, stream, map_x, map_w, p);
+    return BSPEC_LAUNCH_CHECK();
+  }
+  const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS;
+  const int wide = FORCE_WIDE;
+  const int many_bn = wide ? 192 : 128;
+  const long long tiles_n = (N + many_bn - 1) / many_bn;
   const bool many = M > 64 && tiles_m * tiles_n * 4 >= 3ll * sms;
   CUtensorMap map_x, map_w;
   const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-  if (!make_map_bytes(&map_x, X, M, K, ldx, many ? TILE_ROWS : bn) || !make_map_bytes(&map_w, W, N, K, ldw, many ? MANY_BN : TILE_ROWS))
+  if (!make_map_bytes(&map_x, X, M, K, ldx, many ? TILE_ROWS : bn) || !make_map_bytes(&map_w, W, N, K, ldw, many ? many_bn : TILE_ROWS))
     return (int)cudaErrorInvalidValue;
   if (!many) {
     if (bn == 16) return launch_few<16>(map_w, map_x, p, sms, stream);
@@ -498,17 +802,7 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
     return launch_few<128>(map_w, map_x, p, sms, stream);
   }
   p.tiles_m = (int)tiles_m; p.tiles_n = (int)tiles_n;
-  const size_t smem = 1024 + (size_t)MANY_STAGES * (TILE_ROWS + MANY_BN) * KBYTES + 256;
-  static bool set_dev[bspec::kMaxDevices] = {};
-  bool& set = set_dev[bspec::current_device()];
-  if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
-  const long long tiles = tiles_m * tiles_n;
-  BSPEC_LAUNCH((gemm_fp8_many_kernel), (unsigned)(tiles < sms ? tiles : sms), MANY_THREADS, smem, stream, map_x, map_w, p);
-  return BSPEC_LAUNCH_CHECK();
+  return wide ? launch_many<192>(map_x, map_w, p, sms, stream) : launch_many<128>(map_x, map_w, p, sms, stream);
 }
 
 BSPEC_DEFINE_TRACE_SETTER(bspec_trace_set_gemm_fp8)

@@ -215,9 +215,9 @@ template <bool FP8, int NB>
 struct Layout {
   static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
   __host__ __device__ static int blocks(int k) { return (k + 63) / 64; }
-  // tile [NB][128], scales of a piece's u [ff / 64][NB], then the lists
+  // tile [NB][128], scales of two pieces' u [ff / 64][NB], then the lists
   __host__ __device__ static size_t fixed(int ff, int slots, int E) {
-    return (size_t)NB * TILE * 4 + (FP8 ? (size_t)blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
+    return (size_t)NB * TILE * 4 + (FP8 ? (size_t)2 * blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
   }
 };
 
@@ -240,7 +240,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   const int slots = p.n * p.top, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* tile = reinterpret_cast<float*>(smem + (size_t)p.stages * Lay::STAGE);          // [NB][128]
   float* ys = tile + NB * TILE;
-  int* pos = reinterpret_cast<int*>(ys + (FP8 ? Lay::blocks(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
+  int* pos = reinterpret_cast<int*>(ys + (FP8 ? 2 * Lay::blocks(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
   int* tok = pos + slots;                                                                // [slots] tokens by expert
   int* active = tok + slots;                                                             // [E] chosen experts, ascending
   int* first = active + p.E;                                                             // [E + 1] where their entries begin
@@ -257,13 +257,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     }
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 128);
+      mbar_init(acc_empty + i, 4);
     }
     for (int i = 0; i < QUEUE; ++i) {
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, 129);
+      mbar_init(q_empty + i, 5);
     }
-    mbar_init(&meet, 128);
+    mbar_init(&meet, 4);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -487,10 +487,15 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     const uint32_t lane_base = tmem_base + ((quad * 32u) << 16);
     int slot = 0;
     uint32_t slot_phase = 0u, meet_phase = 0u;
-    bool ok = true;
+    bool ok = true, up_known = false;
+    // one arrival per warp: those of 32 lanes on one barrier would come one after the other
+    auto arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
     // the epilogue threads meet (a bounded wait, so that none is left behind when another one gives up)
     auto meet_all = [&]() {
-      mbar_arrive(&meet);
+      arrive(&meet);
       ok = ok && mbar_wait(&meet, meet_phase, abort_flag, p.status, 118);
       meet_phase ^= 1u;
     };
@@ -498,7 +503,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int q = np % QUEUE;
       if (!(ok = mbar_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
       const Piece piece = queue[q];
-      mbar_arrive(q_empty + q);
+      arrive(q_empty + q);
       if (piece.down < 0) break;
       const int c0 = first[piece.a], cnt = first[piece.a + 1] - c0, e = active[piece.a];
       const int cols = piece.down ? (cnt + 15) / 16 * 16 : NB;
@@ -507,31 +512,41 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
 #pragma unroll
         for (int c = 0; c < NB; ++c) acc[c] = 0.f;
         if (piece.down) {
-          // the scales of this expert's u, once its first product says that the up products are done; nobody reads the last piece's any more
-          ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
-          meet_all();
+          // the scales of this expert's u, for the first such piece once its first product says that the up products are done; into the other
+          // one of two buffers: the last piece's may still be read
+          if (!up_known) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+          up_known = true;
+          ys = tile + NB * TILE + (np & 1) * Lay::blocks(p.ff) * NB;
           const int blocks = Lay::blocks(p.ff);
           for (int i = et; i < blocks * NB; i += 128) {
             const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
-            ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
+            if (c < cols) ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
           }
           meet_all();
         }
         // the weights' scale of this thread's row
         const int rows_all = piece.down ? p.d : ffu, K = piece.down ? p.ff : p.d, KB = (K + 127) / 128;
         const int w_row = piece.down ? piece.tile * TILE + row : (GLU && row >= 64 ? p.ff + piece.tile * 64 + row - 64 : piece.tile * OUT + row);
-        const size_t ws_at = ((size_t)e * ((rows_all + 127) / 128) + min(w_row, rows_all - 1) / 128) * KB;
+        // lane l holds those of stage l of the next 32, for the two row blocks that the warp's rows can lie in
+        const int w_block = min(w_row, rows_all - 1) / 128, block_a = __shfl_sync(0xffffffffu, w_block, 0), block_b = __shfl_sync(0xffffffffu, w_block, 31);
+        const size_t ws_at = (size_t)e * ((rows_all + 127) / 128);
         const float* ws = piece.down ? p.sd : p.su;
-        float w_next = block_scale(ws, p.e8m0, ws_at + piece.s0);
+        float wa = 0.f, wb = 0.f;
         auto take = [&]() -> uint32_t {                        // the next accumulator
           if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
           if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
           return from;
         };
-        for (int s = piece.s0; s < piece.s1 && ok; ++s) {
-          const float w = w_next;
-          if (s + 1 < piece.s1) w_next = block_scale(ws, p.e8m0, ws_at + s + 1);
+        for (int s = piece.s0; s < piece.s1; ++s) {
+          const int ahead = (s - piece.s0) & 31;
+          if (ahead == 0 && s + lane < piece.s1) {
+            wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + s + lane);
+            wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + s + lane);
+          }
+          __syncwarp();
+          const float w_a = __shfl_sync(0xffffffffu, wa, ahead), w_b = __shfl_sync(0xffffffffu, wb, ahead);
+          const float w = w_block == block_a ? w_a : w_b;
           const int slot_a = slot;
           const uint32_t from = take();
           if (!piece.down) {
@@ -547,7 +562,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
                 acc[cc + i] = fmaf(fmaf(__uint_as_float(lo[i]), 0.0625f, __uint_as_float(hi[i])), w, acc[cc + i]);
             }
             tc_fence_before();
-            mbar_arrive(acc_empty + slot_a);
+            arrive(acc_empty + slot_a);
           } else {
             const int slot_b = slot;
             const uint32_t from_b = take();
@@ -555,7 +570,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
             const bool two = s * 128 + 64 < K;                 // (a block behind the rows' ends has no scales)
             const float4* fa = reinterpret_cast<const float4*>(ys + 2 * s * NB);
             const float4* fb = reinterpret_cast<const float4*>(ys + (two ? 2 * s + 1 : 2 * s) * NB);
-            const float wb = two ? w : 0.f;
+            const float w2 = two ? w : 0.f;
 #pragma unroll
             for (int cc = 0; cc < NB; cc += 16)
               if (cc < cols) {
@@ -574,13 +589,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
                     const int c = 4 * i + j;
                     const float va = fmaf(__uint_as_float(lo[c]), 0.0625f, __uint_as_float(hi[c]));
                     const float vb = fmaf(__uint_as_float(lb[c]), 0.0625f, __uint_as_float(hb[c]));
-                    acc[cc + c] = fmaf(va * fx[j], w, fmaf(vb * fz[j], wb, acc[cc + c]));
+                    acc[cc + c] = fmaf(va * fx[j], w, fmaf(vb * fz[j], w2, acc[cc + c]));
                   }
                 }
               }
             tc_fence_before();
-            mbar_arrive(acc_empty + slot_a);
-            mbar_arrive(acc_empty + slot_b);
+            arrive(acc_empty + slot_a);
+            arrive(acc_empty + slot_b);
           }
         }
       } else {
@@ -672,7 +687,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       }
       if (!FP8) {
         tc_fence_before();
-        mbar_arrive(acc_empty + slot);
+        arrive(acc_empty + slot);
         if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
       }
     }

@@ -28,6 +28,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
+// ... and everything that other CTAs of the cluster did before their arrivals is seen
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ uint64_t wall_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -37,12 +47,14 @@ __device__ __forceinline__ uint64_t wall_ns() {
 // limit (polls or time) is hit, or when any CTA of this or an earlier launch has given up (the status word in
 // global memory is set: the step's result is lost anyway, so the rest of the grid leaves at once instead of
 // waiting out its own limits one CTA after the other).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
                                           int code) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto done = [&]() { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (done()) return true;
   uint64_t t0 = 0;
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (done()) return true;
     if (*abort_flag) return false;
     if ((i & 255u) == 255u) {
       if (*reinterpret_cast<volatile int*>(status) != 0) {

@@ -256,7 +256,7 @@ TRACE_KERNEL_NAMES = {1: "embed", 2: "add_rmsnorm", 3: "gather_rows_add", 4: "si
                       66: "scan_conv", 67: "selective_scan", 70: "stream_expand", 71: "stream_norm", 72: "stream_gather", 73: "branch_join", 74: "state_space", 75: "matrix_memory", 21: "pool_append", 20: "gemm_tcgen05", 30: "attn_prefill_tc", 40: "latent_prepare",
                       41: "latent_attn_generic", 42: "gate_heads", 43: "latent_attn_mma", 44: "latent_attn_join",
                       50: "moe_route", 51: "moe_plan", 52: "moe_grouped", 53: "moe_gather", 54: "moe_combine", 55: "moe_skinny", 56: "moe_skinny_mma", 57: "moe_rank", 58: "moe_offsets", 59: "moe_place",
-                      80: "quantize_rows", 81: "quantize_blocks", 82: "gemm_fp8_few", 83: "gemm_fp8_many",
+                      80: "quantize_rows", 81: "quantize_blocks", 82: "gemm_fp8_few", 83: "gemm_fp8_many", 86: "gemm_fp8_pair",
                       84: "moe_layer_route", 85: "moe_layer_experts"}
 
 
@@ -1255,7 +1255,8 @@ WAIT_CODES = ((1, 1, "GEMM: stage never freed"), (2, 2, "GEMM: operands never ar
               (92, 92, "float32 product of few rows: operands never arrived"),
               (101, 108, "8-bit product: a stage or an accumulator never freed, operands or an accumulator never complete"),
               (111, 111, "routed layer of a few tokens: the up products never completed"),
-              (113, 120, "routed layer of a few tokens: a stage, an accumulator or a piece of work never came or was never freed"))
+              (113, 120, "routed layer of a few tokens: a stage, an accumulator or a piece of work never came or was never freed"),
+              (121, 126, "8-bit product of pairs of CTAs: a stage or an accumulator never freed, operands or sums never complete"))
 
 
 def wait_meaning(code: int) -> str:
