@@ -7,19 +7,21 @@
 // the epilogue warps read it back, multiply by its scales and add it to float32 sums in registers while the next blocks' products
 // run.  The sum over blocks is in ascending k.
 //
-// Two arrangements:
-//   rows of W on the accumulator's 128 rows, tokens on its columns (few tokens): every weight is streamed once at full tile
-//     efficiency.  K may be cut into `splits` slices run by the CTAs of one cluster, whose partial tiles are joined in slice
-//     order through distributed shared memory.
-//   tokens on the rows, 256 rows of W on the columns (many tokens): one persistent CTA per SM; eight epilogue warps hold the
-//     128 x 256 sums.
+// Three arrangements, chosen by an estimate of their times (`choose`):
+//   few tokens    rows of W on the accumulator's 128 rows, tokens on its columns: every weight is streamed once at full tile efficiency.  K
+//                 may be cut into `splits` slices run by the CTAs of one cluster, whose partial tiles are joined in slice order through
+//                 distributed shared memory.
+//   many tokens   tokens on the rows, 128 rows of W on the columns: one persistent CTA per SM; eight epilogue warps hold the 128 x 128 sums.
+//                 The way back from tensor memory bounds it: 512 bytes a clock are asked for by 128 x 128 numbers per 128 k.
+//   pairs         many tokens where both scales are powers of two: the tensor cores multiply by the scales and keep the sums of a whole
+//                 row, two CTAs share a tile (below).
+//
+// Measured on B200: 8 x 28,672 x 4,096 in 20 us (5.8 TB/s), 1,537 x 4,096 x 14,336 with float32 scales in 120 us (1.5 PFLOP/s), 2,048 x 28,672 x
+// 4,096 with e8m0 scales in 182 us (2.65 PFLOP/s; all zeros, which the power limit does not slow down, run at 4.1).
 #include "e4m3.cuh"
 #include "umma.cuh"
 
 using namespace bspec;
-#ifndef FORCE_WIDE
-#define FORCE_WIDE 1
-#endif
 
 namespace {
 
@@ -27,8 +29,8 @@ constexpr int KBYTES = 128;            // k per stage: one scale block, one 128-
 constexpr int TILE_ROWS = 128;
 constexpr int FEW_THREADS = 192;       // TMA warp, MMA warp, 4 epilogue warps
 constexpr int FEW_WINDOW = 32;         // k blocks whose scales wait in shared memory at a time
-constexpr int many_threads(int bn) { return 128 + 2 * bn; }  // TMA warp, MMA warp, two idle ones, four epilogue warps for every 64 columns
-constexpr int many_stages(int bn) { return bn == 192 ? 5 : 6; }
+constexpr int MANY_THREADS = 320;      // TMA warp, MMA warp, 8 epilogue warps
+constexpr int MANY_BN = 128, MANY_STAGES = 6;
 
 struct Scales {
   const void* p;
@@ -51,31 +53,28 @@ struct Fp8Params {
   int tiles_m, tiles_n;  // many tokens
 };
 
-__device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
-}
-// float32 accumulator, e4m3 A and B (format code 0), both K-major, M = 128, N = bn
-__device__ __forceinline__ uint32_t e4m3_desc(int bn) {
-  return (1u << 4) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
-}
 __device__ __forceinline__ void put(void* C, int out_f32, size_t at, float v) {
   if (out_f32) reinterpret_cast<float*>(C)[at] = v;
   else reinterpret_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
 }
-// sixteen numbers as bfloat16, 32 bytes in one store: a whole sector, where two of 16 bytes would be two partial ones
-__device__ __forceinline__ void put16(__nv_bfloat16* to, const float* v) {
+// 16 neighbours in stores of 32 bytes: whole sectors, where stores of 16 bytes would be partial ones.  `to` on a 32-byte boundary.
+__device__ __forceinline__ void put32b(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ void put16(void* C, int out_f32, size_t at, const float* v) {
+  if (out_f32) {
+    put32b(reinterpret_cast<float*>(C) + at, reinterpret_cast<const uint32_t*>(v));
+    put32b(reinterpret_cast<float*>(C) + at + 8, reinterpret_cast<const uint32_t*>(v + 8));
+    return;
+  }
   uint32_t w[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
     w[j] = *reinterpret_cast<uint32_t*>(&h);
   }
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  put32b(reinterpret_cast<__nv_bfloat16*>(C) + at, w);
 }
 // Let copies in flight land before the CTA gives up its shared memory (after a wait ran out).
 __device__ __forceinline__ void drain(uint64_t* full, int armed, int stages) {
@@ -86,12 +85,12 @@ __device__ __forceinline__ void drain(uint64_t* full, int armed, int stages) {
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
-constexpr int few_buffers(int bn) { return bn >= 128 ? 2 : 4; }      // accumulators: two CTAs of an SM share 512 columns
+constexpr int FEW_BUFFERS = 4;         // accumulators: two CTAs of an SM share 512 columns
 
 template <int BN>
 __global__ void __launch_bounds__(FEW_THREADS)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, Fp8Params p) {
-  constexpr int NB = few_buffers(BN);
+  constexpr int NB = FEW_BUFFERS;
   constexpr uint32_t COLS = NB * BN;                                   // 64, 128 or 256: powers of two
   constexpr int W_BYTES = TILE_ROWS * KBYTES, X_BYTES = BN * KBYTES, STAGE = W_BYTES + X_BYTES;
   extern __shared__ unsigned char smem_dyn[];
@@ -139,44 +138,47 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   for (int c = 0; c < BN; ++c) acc[c] = 0.f;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int armed = 0;
-      if (!p.w_ahead) bspec::pdl_wait();
-      const int pre = min(nkb, p.stages);
-      for (int i = 0; i < pre; ++i) {
-        mbar_expect_tx(full + i, (uint32_t)STAGE);
-        tma_load_2d(smem + (size_t)i * STAGE, &map_w, full + i, (kb0 + i) * KBYTES, tile_n * TILE_ROWS);
-      }
-      bspec::pdl_wait();
-      bspec::trace_record(82, t_trace);
-      for (int i = 0; i < pre; ++i)
-        tma_load_2d(smem + (size_t)i * STAGE + W_BYTES, &map_x, full + i, (kb0 + i) * KBYTES, tok0);
-      armed = pre;
-      for (int i = pre; i < nkb; ++i) {
-        const int s = i % p.stages;
-        if (!mbar_wait(empty + s, ((uint32_t)(i / p.stages) & 1u) ^ 1u, abort_flag, p.status, 101)) break;
-        mbar_expect_tx(full + s, (uint32_t)STAGE);
-        tma_load_2d(smem + (size_t)s * STAGE, &map_w, full + s, (kb0 + i) * KBYTES, tile_n * TILE_ROWS);
-        tma_load_2d(smem + (size_t)s * STAGE + W_BYTES, &map_x, full + s, (kb0 + i) * KBYTES, tok0);
-        armed = i + 1;
-      }
-      if (*abort_flag) drain(full, armed, p.stages);
+    const uint32_t one = elect_one();
+    int armed = 0;
+    if (!p.w_ahead) bspec::pdl_wait();
+    const int pre = min(nkb, p.stages);
+    for (int i = 0; i < pre; ++i) {
+      mbar_expect_tx_by(one, full + i, (uint32_t)STAGE);
+      tma_load_2d_by(one, smem + (size_t)i * STAGE, &map_w, full + i, (kb0 + i) * KBYTES, tile_n * TILE_ROWS);
     }
+    bspec::pdl_wait();
+    bspec::trace_record(82, t_trace);
+    for (int i = 0; i < pre; ++i)
+      tma_load_2d_by(one, smem + (size_t)i * STAGE + W_BYTES, &map_x, full + i, (kb0 + i) * KBYTES, tok0);
+    armed = pre;
+    int s = 0;
+    uint32_t phase = 0u;
+    for (int i = pre; i < nkb; ++i) {
+      if (!warp_wait(empty + s, phase, abort_flag, p.status, 101)) break;
+      mbar_expect_tx_by(one, full + s, (uint32_t)STAGE);
+      tma_load_2d_by(one, smem + (size_t)s * STAGE, &map_w, full + s, (kb0 + i) * KBYTES, tile_n * TILE_ROWS);
+      tma_load_2d_by(one, smem + (size_t)s * STAGE + W_BYTES, &map_x, full + s, (kb0 + i) * KBYTES, tok0);
+      armed = i + 1;
+      if (++s == p.stages) { s = 0; phase ^= 1u; }
+    }
+    if (*abort_flag) drain(full, armed, p.stages);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = e4m3_desc(BN);
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % p.stages, b = i % NB;
-        if (!mbar_wait(full + s, (uint32_t)(i / p.stages) & 1u, abort_flag, p.status, 102)) break;
-        if (!mbar_wait(acc_empty + b, ((uint32_t)(i / NB) & 1u) ^ 1u, abort_flag, p.status, 103)) break;
-        tc_fence_after();
-        unsigned char* w_src = smem + (size_t)s * STAGE;
-        const uint64_t wd = smem_desc(w_src), xd = smem_desc(w_src + W_BYTES);
+    const uint32_t one = elect_one();
+    const uint32_t idesc = instr_desc_e4m3(BN);
+    const uint64_t desc0 = smem_desc(smem);
+    int s = 0, b = 0;
+    uint32_t phase = 0u, acc_phase = 0u;
+    for (int i = 0; i < nkb; ++i) {
+      if (!warp_wait(full + s, phase, abort_flag, p.status, 102)) break;
+      if (!warp_wait(acc_empty + b, acc_phase ^ 1u, abort_flag, p.status, 103)) break;
+      tc_fence_after();
+      const uint64_t wd = desc0 + (uint64_t)(s * (STAGE / 16)), xd = wd + W_BYTES / 16;      // addresses count 16 bytes
 #pragma unroll
-        for (int k = 0; k < KBYTES / 32; ++k) mma_e4m3(tmem_base + b * BN, wd + 2 * k, xd + 2 * k, idesc, k > 0 ? 1u : 0u);
-        tc_commit(empty + s);
-        tc_commit(acc_full + b);
-      }
+      for (int k = 0; k < KBYTES / 32; ++k) tc_mma_8bit_by(one, tmem_base + b * BN, wd + 2 * k, xd + 2 * k, idesc, k > 0 ? 1u : 0u);
+      tc_commit_by(one, empty + s);
+      tc_commit_by(one, acc_full + b);
+      if (++s == p.stages) { s = 0; phase ^= 1u; }
+      if (++b == NB) { b = 0; acc_phase ^= 1u; }
     }
   } else {
     const uint32_t quad = warp & 3;
@@ -199,23 +201,27 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       if (!ok) continue;
       tc_fence_after();
       const float4* f = reinterpret_cast<const float4*>(scales + (i % FEW_WINDOW) * BN);
+      const uint32_t from = tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * BN);
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + b);             // one arrival per warp: those of its lanes would come one after the other
+      };
+      // an accumulator is read in one trip, and is free for the next products before its numbers are added
+      uint32_t v[BN];
+      if constexpr (BN == 16) tc_ld16(from, v);
+      else if constexpr (BN == 32) tc_ld32(from, v);
+      else tc_ld64(from, v);
+      tc_wait_ld();
+      release();
 #pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 16) {
-        uint32_t v[16];
-        tc_ld16(tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * BN + c0), v);
-        tc_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 g = f[c0 / 4 + j];
-          acc[c0 + 4 * j] = fmaf(__uint_as_float(v[4 * j]), g.x, acc[c0 + 4 * j]);
-          acc[c0 + 4 * j + 1] = fmaf(__uint_as_float(v[4 * j + 1]), g.y, acc[c0 + 4 * j + 1]);
-          acc[c0 + 4 * j + 2] = fmaf(__uint_as_float(v[4 * j + 2]), g.z, acc[c0 + 4 * j + 2]);
-          acc[c0 + 4 * j + 3] = fmaf(__uint_as_float(v[4 * j + 3]), g.w, acc[c0 + 4 * j + 3]);
-        }
+      for (int c = 0; c < BN; c += 4) {
+        const float4 g = f[c / 4];
+        acc[c] = fmaf(__uint_as_float(v[c]), g.x, acc[c]);
+        acc[c + 1] = fmaf(__uint_as_float(v[c + 1]), g.y, acc[c + 1]);
+        acc[c + 2] = fmaf(__uint_as_float(v[c + 2]), g.z, acc[c + 2]);
+        acc[c + 3] = fmaf(__uint_as_float(v[c + 3]), g.w, acc[c + 3]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + b);               // one arrival per warp: those of its lanes would come one after the other
     }
     const int row = (int)quad * 32 + lane, n = tile_n * TILE_ROWS + row;
     if (p.splits == 1) {
@@ -279,11 +285,10 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens
-template <int MANY_BN>
-__global__ void __launch_bounds__(many_threads(MANY_BN), 1)
+__global__ void __launch_bounds__(MANY_THREADS, 1)
 gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
   constexpr int X_BYTES = TILE_ROWS * KBYTES, W_BYTES = MANY_BN * KBYTES, STAGE = X_BYTES + W_BYTES;
-  constexpr int MANY_STAGES = many_stages(MANY_BN), NB = 2, COLS = 64;   // accumulators; columns of an epilogue thread
+  constexpr int NB = 2, COLS = 64;   // accumulators; columns of an epilogue thread
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + MANY_STAGES * STAGE);
@@ -318,50 +323,48 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   const int nkb = (p.K + KBYTES - 1) / KBYTES;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
 
-  if (warp < 4) {
-  // registers: the first four warps leave theirs to the others (512 threads x 128 = 128 x 40 + 384 x 152 + 2,048 to spare)
-  if (MANY_BN == 192) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 0) {
-    if (lane == 0) {
-      int armed = 0;
+  if (warp < 2) {
+    const uint32_t one = elect_one();
+    if (warp == 0) {
+      int s = 0;
+      uint32_t phase = 0u;
       bool ok = true;
       for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const int m0 = (int)(t % p.tiles_m) * TILE_ROWS, n0 = (int)(t / p.tiles_m) * MANY_BN;
         for (int kb = 0; kb < nkb; ++kb) {
-          const int s = armed % MANY_STAGES;
-          if (!(ok = mbar_wait(empty + s, ((uint32_t)(armed / MANY_STAGES) & 1u) ^ 1u, abort_flag, p.status, 105))) break;
-          mbar_expect_tx(full + s, (uint32_t)STAGE);
-          tma_load_2d(smem + s * STAGE, &map_x, full + s, kb * KBYTES, m0);
-          tma_load_2d(smem + s * STAGE + X_BYTES, &map_w, full + s, kb * KBYTES, n0);
-          ++armed;
+          if (!(ok = warp_wait(empty + s, phase ^ 1u, abort_flag, p.status, 105))) break;
+          mbar_expect_tx_by(one, full + s, (uint32_t)STAGE);
+          tma_load_2d_by(one, smem + s * STAGE, &map_x, full + s, kb * KBYTES, m0);
+          tma_load_2d_by(one, smem + s * STAGE + X_BYTES, &map_w, full + s, kb * KBYTES, n0);
+          if (++s == MANY_STAGES) { s = 0; phase ^= 1u; }
         }
       }
-      if (*abort_flag) drain(full, armed, MANY_STAGES);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = e4m3_desc(MANY_BN);
-      int i = 0;
+      if (*abort_flag)                       // copies in flight land (they take microseconds) before the CTA ends
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else {
+      const uint32_t idesc = instr_desc_e4m3(MANY_BN);
+      const uint64_t desc0 = smem_desc(smem);
+      int s = 0, b = 0;
+      uint32_t phase = 0u, acc_phase = 0u;
       bool ok = true;
       for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        for (int kb = 0; kb < nkb; ++kb, ++i) {
-          const int s = i % MANY_STAGES, b = i % NB;
-          if (!(ok = mbar_wait(full + s, (uint32_t)(i / MANY_STAGES) & 1u, abort_flag, p.status, 106))) break;
-          if (!(ok = mbar_wait(acc_empty + b, ((uint32_t)(i / NB) & 1u) ^ 1u, abort_flag, p.status, 107))) break;
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!(ok = warp_wait(full + s, phase, abort_flag, p.status, 106))) break;
+          if (!(ok = warp_wait(acc_empty + b, acc_phase ^ 1u, abort_flag, p.status, 107))) break;
           tc_fence_after();
-          const uint64_t xd = smem_desc(smem + s * STAGE), wd = smem_desc(smem + s * STAGE + X_BYTES);
+          const uint64_t xd = desc0 + (uint64_t)(s * (STAGE / 16)), wd = xd + X_BYTES / 16;
 #pragma unroll
-          for (int k = 0; k < KBYTES / 32; ++k) mma_e4m3(tmem_base + b * MANY_BN, xd + 2 * k, wd + 2 * k, idesc, k > 0 ? 1u : 0u);
-          tc_commit(empty + s);
-          tc_commit(acc_full + b);
+          for (int k = 0; k < KBYTES / 32; ++k) tc_mma_8bit_by(one, tmem_base + b * MANY_BN, xd + 2 * k, wd + 2 * k, idesc, k > 0 ? 1u : 0u);
+          tc_commit_by(one, empty + s);
+          tc_commit_by(one, acc_full + b);
+          if (++s == MANY_STAGES) { s = 0; phase ^= 1u; }
+          if (++b == NB) { b = 0; acc_phase ^= 1u; }
         }
       }
     }
-  }
   } else {
-    if (MANY_BN == 192) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     const uint32_t quad = warp & 3;
-    const int group = (warp - 4) >> 2;                                  // columns 64 group .. of the tile: in one row of W's scales
+    const int group = (warp - 2) >> 2;                                  // columns 64 group .. of the tile: in one row of W's scales
     const uint32_t lane_base = tmem_base + ((quad * 32u) << 16) + (uint32_t)(group * COLS);
     const int row = (int)quad * 32 + lane;
     int b = 0;
@@ -374,40 +377,34 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
       for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
       float x_next = scale_at(p.xs, srow, 0), w_next = scale_at(p.ws, wrow, 0);
-      uint32_t v0[32], v1[32];
-      ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108);
-      tc_fence_after();
-      tc_ld32(lane_base + (uint32_t)(b * MANY_BN), v0);
-      for (int kb = 0; kb < nkb && ok; ++kb) {
+      for (int kb = 0; kb < nkb; ++kb) {
         const float f = x_next * w_next;
         if (kb + 1 < nkb) {
           x_next = scale_at(p.xs, srow, kb + 1);
           w_next = scale_at(p.ws, wrow, kb + 1);
         }
-        // 32 columns are on their way while the 32 before them are added, from block to block too
-        tc_wait_ld();
-        tc_ld32(lane_base + (uint32_t)(b * MANY_BN + 32), v1);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v0[j]), f, acc[j]);
+        if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108))) break;
+        tc_fence_after();
+        // all columns in one load: what bounds this loop is the number of trips to the tensor memory, not their width
+        uint32_t v[COLS];
+        tc_ld64(lane_base + (uint32_t)(b * MANY_BN), v);
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + b);
         if (++b == NB) { b = 0; phase ^= 1u; }
-        if (kb + 1 < nkb) {
-          ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108);
-          tc_fence_after();
-          tc_ld32(lane_base + (uint32_t)(b * MANY_BN), v0);
-        }
+        const uint64_t ff = pack2(f, f);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v1[j]), f, acc[32 + j]);
+        for (int c = 0; c < COLS; c += 2) {                             // two to an instruction: the loop's time is what it issues
+          const uint64_t sum = fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), ff, pack2(acc[c], acc[c + 1]));
+          unpack2(sum, acc[c], acc[c + 1]);
+        }
       }
-      tc_wait_ld();
       if (ok && m < p.M) {
         const size_t base = (size_t)m * p.N + n0;
-        if (!p.out_f32 && p.N % 16 == 0 && n0 + COLS <= p.N) {
+        if (p.N % 16 == 0 && n0 + COLS <= p.N) {
 #pragma unroll
-          for (int c = 0; c < COLS; c += 16) put16(reinterpret_cast<__nv_bfloat16*>(p.C) + base + c, acc + c);
+          for (int c = 0; c < COLS; c += 16) put16(p.C, p.out_f32, base + c, acc + c);
         } else {
 #pragma unroll
           for (int c = 0; c < COLS; ++c)
@@ -448,17 +445,11 @@ __device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {     /
 __device__ __forceinline__ void arrive_in(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+__device__ __forceinline__ void tma_load_pair(uint32_t one, void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(s32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
-}
-// The warp that issues products stays together, and one lane of it issues (`one`): what the instructions take from registers common to the
-// warp is then at hand.  Issued from a branch of a single lane they take some 200 clocks each.
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one;
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(s32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(one) : "memory");
 }
 __device__ __forceinline__ void commit_pair(uint32_t one, uint64_t* bar) {
   asm volatile(
@@ -525,25 +516,24 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int st = 0;
-      uint32_t phase = 0u;
-      bool ok = true;
-      for (long long t = pair; t < tiles && ok; t += pairs) {
-        const int m0 = (int)(t % p.tiles_m) * 256 + (int)rank * TILE_ROWS, n0 = (int)(t / p.tiles_m) * PAIR_BN + (int)rank * (PAIR_BN / 2);
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (!(ok = mbar_wait(empty + st, phase ^ 1u, abort_flag, p.status, 121))) break;
-          if (rank == 0) mbar_expect_tx(full + st, 2 * PAIR_STAGE);
-          const uint32_t bar = in_cta(full + st, 0);
-          unsigned char* at = smem + st * PAIR_STAGE;
-          tma_load_pair(at, &map_x, bar, kb * KBYTES, m0);
-          tma_load_pair(at + PAIR_X, &map_w, bar, kb * KBYTES, n0);
-          if (++st == PAIR_STAGES) { st = 0; phase ^= 1u; }
-        }
+    const uint32_t one = elect_one();
+    int st = 0;
+    uint32_t phase = 0u;
+    bool ok = true;
+    for (long long t = pair; t < tiles && ok; t += pairs) {
+      const int m0 = (int)(t % p.tiles_m) * 256 + (int)rank * TILE_ROWS, n0 = (int)(t / p.tiles_m) * PAIR_BN + (int)rank * (PAIR_BN / 2);
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!(ok = warp_wait(empty + st, phase ^ 1u, abort_flag, p.status, 121))) break;
+        if (rank == 0) mbar_expect_tx_by(one, full + st, 2 * PAIR_STAGE);
+        const uint32_t bar = in_cta(full + st, 0);
+        unsigned char* at = smem + st * PAIR_STAGE;
+        tma_load_pair(one, at, &map_x, bar, kb * KBYTES, m0);
+        tma_load_pair(one, at + PAIR_X, &map_w, bar, kb * KBYTES, n0);
+        if (++st == PAIR_STAGES) { st = 0; phase ^= 1u; }
       }
-      if (*abort_flag)                       // copies in flight land (they take microseconds) before the CTA ends
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     }
+    if (*abort_flag)                         // copies in flight land (they take microseconds) before the CTA ends
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t one = elect_one();
@@ -655,9 +645,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       if (++b == 2) { b = 0; phase ^= 1u; }
       if (m < p.M) {
         const size_t base = (size_t)m * p.N + n0;
-        if (!p.out_f32 && p.N % 16 == 0 && n0 + COLS <= p.N) {
+        if (p.N % 16 == 0 && n0 + COLS <= p.N) {
 #pragma unroll
-          for (int c = 0; c < COLS; c += 16) put16(reinterpret_cast<__nv_bfloat16*>(p.C) + base + c, acc + c);
+          for (int c = 0; c < COLS; c += 16) put16(p.C, p.out_f32, base + c, acc + c);
         } else {
 #pragma unroll
           for (int c = 0; c < COLS; ++c)
@@ -689,15 +679,38 @@ bool make_map_bytes(CUtensorMap* map, const void* base, long long rows, int K, l
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// slices of k of the arrangement for few tokens: two CTAs share an SM, and K is cut so that the CTAs about fill those slots, at least 4 blocks
+// to a slice, clusters of a power of two
+int few_splits(long long tiles, int nkb, int sms) {
+  long long splits = 2ll * sms / tiles;
+  if (splits > nkb / 4) splits = nkb / 4;
+  return splits >= 8 ? 8 : (splits >= 4 ? 4 : (splits >= 2 ? 2 : 1));
+}
+
+// The arrangement that an estimate of its time takes: a start, and rounds of the tiles over the SMs of so many blocks of k each.  The numbers
+// (us) are fits to times on B200: 48 to 1,536 tokens by 4,096 x 4,096, 28,672 x 4,096, 4,096 x 14,336, 2,048 x 2,048 and 1,040 x 720.
+// E.g. 4,096 x 14,336, few / many / pairs: 64 tokens 19 / 48 / 42, 256 tokens 51 / 50 / 46, 1,024 tokens - / 98 / 77;
+// 4,096 x 4,096: 128 tokens 13 / 17 / 23, 512 tokens 29 / 18 / 24.
+enum Form { FEW, MANY, PAIR };
+Form choose(int M, int N, int K, bool powers, int sms) {
+  const int nkb = (K + KBYTES - 1) / KBYTES;
+  const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
+  const long long few_tiles = ((long long)N + TILE_ROWS - 1) / TILE_ROWS * (((long long)M + bn - 1) / bn);
+  const int splits = few_splits(few_tiles, nkb, sms);
+  auto rounds = [](long long tiles, long long at_once) { return (double)((tiles + at_once - 1) / at_once); };
+  const double few = 5.5 + rounds(few_tiles * splits, 2 * sms) * ((nkb + splits - 1) / splits) * (bn == 16 ? 0.45 : (bn == 32 ? 0.6 : 0.87));
+  const double many = 6 + rounds(((long long)M + 127) / 128 * (((long long)N + MANY_BN - 1) / MANY_BN), sms) * (0.35 * nkb + 2);
+  const double pair = 7 + rounds(((long long)M + 255) / 256 * (((long long)N + PAIR_BN - 1) / PAIR_BN), sms / 2) * (0.27 * nkb + 4);
+  if (few <= many && (!powers || few <= pair)) return FEW;
+  return powers && pair < many ? PAIR : MANY;
+}
+
 template <int BN>
 int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, Fp8Params p, int sms, cudaStream_t stream) {
   const int kb_total = (p.K + KBYTES - 1) / KBYTES;
   const int tiles_n = (p.N + TILE_ROWS - 1) / TILE_ROWS, tiles_t = (p.M + BN - 1) / BN;
-  // Two CTAs share an SM: K is cut so that the CTAs about fill those slots, at least 4 blocks to a slice, clusters of a power of two.
-  long long splits = 2ll * sms / ((long long)tiles_n * tiles_t);
-  if (splits > kb_total / 4) splits = kb_total / 4;
-  splits = splits >= 8 ? 8 : (splits >= 4 ? 4 : (splits >= 2 ? 2 : 1));
-  p.kblocks_per_split = (kb_total + (int)splits - 1) / (int)splits;
+  const int splits = few_splits((long long)tiles_n * tiles_t, kb_total, sms);
+  p.kblocks_per_split = (kb_total + splits - 1) / splits;
   p.splits = (kb_total + p.kblocks_per_split - 1) / p.kblocks_per_split;       // no empty slice
   constexpr int STAGE = (TILE_ROWS + BN) * KBYTES;
   constexpr int FIXED = 1024 + FEW_WINDOW * BN * 4 + 256;
@@ -737,18 +750,12 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, Fp8Params p, 
   return BSPEC_LAUNCH_CHECK();
 }
 
-template <int BN>
-int launch_many(const CUtensorMap& map_x, const CUtensorMap& map_w, const Fp8Params& p, int sms, cudaStream_t stream) {
-  const size_t smem = 1024 + (size_t)many_stages(BN) * (TILE_ROWS + BN) * KBYTES + 256;
-  static bool set_dev[bspec::kMaxDevices] = {};
-  bool& set = set_dev[bspec::current_device()];
-  if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_many_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
-  const long long tiles = (long long)p.tiles_m * p.tiles_n;
-  BSPEC_LAUNCH((gemm_fp8_many_kernel<BN>), (unsigned)(tiles < sms ? tiles : sms), many_threads(BN), smem, stream, map_x, map_w, p);
+typedef void (*WholeKernel)(CUtensorMap, CUtensorMap, Fp8Params);
+int launch_whole(WholeKernel kernel, const CUtensorMap& map_x, const CUtensorMap& map_w, const Fp8Params& p, long long grid, int threads,
+                 size_t smem, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  (void)bspec::launch(kernel, dim3((unsigned)grid), dim3(threads), smem, stream, map_x, map_w, p);
   return BSPEC_LAUNCH_CHECK();
 }
 
@@ -769,40 +776,27 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
   p.ws = {ws, ldws, ws_e8m0};
   p.M = M; p.N = N; p.K = K; p.out_f32 = out_f32; p.w_ahead = w_ahead;
   const int sms = bspec::sm_count();
-  if (xs_e8m0 && ws_e8m0 && M > 128) {
-    CUtensorMap map_x, map_w;
-    if (!make_map_bytes(&map_x, X, M, K, ldx, TILE_ROWS) || !make_map_bytes(&map_w, W, N, K, ldw, PAIR_BN / 2)) return (int)cudaErrorInvalidValue;
-    p.tiles_m = (M + 255) / 256;
-    p.tiles_n = (N + PAIR_BN - 1) / PAIR_BN;
-    const size_t smem = 1024 + (size_t)PAIR_STAGES * PAIR_STAGE + PAIR_SF_SLOTS * PAIR_SF;
-    static bool set_dev[bspec::kMaxDevices] = {};
-    bool& set = set_dev[bspec::current_device()];
-    if (!set) {
-      const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return (int)e;
-      set = true;
-    }
-    const long long tiles = (long long)p.tiles_m * p.tiles_n, pairs = sms / 2;
-    BSPEC_LAUNCH((gemm_fp8_pair_kernel), (unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, smem, stream, map_x, map_w, p);
-    return BSPEC_LAUNCH_CHECK();
-  }
-  const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS;
-  const int wide = FORCE_WIDE;
-  const int many_bn = wide ? 192 : 128;
-  const long long tiles_n = (N + many_bn - 1) / many_bn;
-  const bool many = M > 64 && tiles_m * tiles_n * 4 >= 3ll * sms;
+  const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + MANY_BN - 1) / MANY_BN;
+  const long long pairs_m = (M + 255) / 256, pairs_n = (N + PAIR_BN - 1) / PAIR_BN;
+  const Form form = choose(M, N, K, xs_e8m0 && ws_e8m0, sms);
   CUtensorMap map_x, map_w;
-  const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-  if (!make_map_bytes(&map_x, X, M, K, ldx, many ? TILE_ROWS : bn) || !make_map_bytes(&map_w, W, N, K, ldw, many ? many_bn : TILE_ROWS))
+  const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
+  if (!make_map_bytes(&map_x, X, M, K, ldx, form == FEW ? bn : TILE_ROWS) ||
+      !make_map_bytes(&map_w, W, N, K, ldw, form == PAIR ? PAIR_BN / 2 : (form == MANY ? MANY_BN : TILE_ROWS)))
     return (int)cudaErrorInvalidValue;
-  if (!many) {
+  if (form == FEW) {
     if (bn == 16) return launch_few<16>(map_w, map_x, p, sms, stream);
     if (bn == 32) return launch_few<32>(map_w, map_x, p, sms, stream);
-    if (bn == 64) return launch_few<64>(map_w, map_x, p, sms, stream);
-    return launch_few<128>(map_w, map_x, p, sms, stream);
+    return launch_few<64>(map_w, map_x, p, sms, stream);
   }
-  p.tiles_m = (int)tiles_m; p.tiles_n = (int)tiles_n;
-  return wide ? launch_many<192>(map_x, map_w, p, sms, stream) : launch_many<128>(map_x, map_w, p, sms, stream);
+  if (form == MANY) {
+    p.tiles_m = (int)tiles_m; p.tiles_n = (int)tiles_n;
+    return launch_whole(gemm_fp8_many_kernel, map_x, map_w, p, tiles_m * tiles_n < sms ? tiles_m * tiles_n : sms, MANY_THREADS,
+                        1024 + (size_t)MANY_STAGES * (TILE_ROWS + MANY_BN) * KBYTES + 256, stream);
+  }
+  p.tiles_m = (int)pairs_m; p.tiles_n = (int)pairs_n;
+  return launch_whole(gemm_fp8_pair_kernel, map_x, map_w, p, 2 * (pairs_m * pairs_n < sms / 2 ? pairs_m * pairs_n : sms / 2), PAIR_THREADS,
+                      1024 + (size_t)PAIR_STAGES * PAIR_STAGE + PAIR_SF_SLOTS * PAIR_SF, stream);
 }
 
 BSPEC_DEFINE_TRACE_SETTER(bspec_trace_set_gemm_fp8)

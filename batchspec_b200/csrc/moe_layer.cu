@@ -172,13 +172,6 @@ struct Piece {
   int a, tile, s0, s1, split;                // place in the list of chosen experts, 128 rows, stages of k
 };
 
-__device__ __forceinline__ void mma_8bit(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
-}
 __device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ float block_scale(const float* p, int e8m0, size_t i) {
   return e8m0 ? scale_value(reinterpret_cast<const uint8_t*>(p)[i]) : p[i];
@@ -344,14 +337,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   const int entries = first[A];
 
   if (warp == 0) {
-    // Lane 0 and 1 copy the weights' two halves of a stage, the next lanes 16 rows of tokens each: a stage costs the warp one
-    // pass through this code, not one thread a pass per copy.
+    const uint32_t one = elect_one();
     int st = 0, np = 0;                                        // stage of the ring, pieces so far
     uint32_t phase = 0u;
     bool ok = true;
     auto push = [&](const Piece& piece) {
       const int q = np % QUEUE;
-      if (ok) ok = mbar_wait(q_empty + q, ((uint32_t)(np / QUEUE) & 1u) ^ 1u, abort_flag, p.status, 113);
+      if (ok) ok = warp_wait(q_empty + q, ((uint32_t)(np / QUEUE) & 1u) ^ 1u, abort_flag, p.status, 113);
       if (lane == 0 && ok) {
         queue[q] = piece;
         mbar_arrive(q_full + q);
@@ -364,37 +356,36 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (lane == 0) t = atomicAdd(p.counters + counter, 1);
       return __shfl_sync(0xffffffffu, t, 0);
     };
-    // this lane's copy of a piece: map, row and place in a stage (`role` 0: none, 1: weights, 2: tokens)
-    const CUtensorMap* map = nullptr;
-    int y = 0, role = 0;
-    uint32_t dst = 0u, bytes = 0u;                             // bytes: of a whole stage
-    auto assign = [&](const CUtensorMap* weights, int y0, int y1, const CUtensorMap* tokens, int t0, int mid, int boxes) {
-      const int b = lane - 2;
-      role = lane < 2 ? 1 : (b < boxes * (FP8 ? 2 : 1) ? 2 : 0);
-      map = lane < 2 ? weights : tokens;
-      y = lane == 0 ? y0 : (lane == 1 ? y1 : (b < boxes ? t0 + 16 * b : mid + t0 + 16 * (b - boxes)));
-      dst = lane < 2 ? (uint32_t)lane * (A_BYTES / 2) : A_BYTES + (uint32_t)b * 2048u;
-      bytes = A_BYTES + (uint32_t)boxes * 2048u * (FP8 ? 2u : 1u);
+    // stage s of a piece: the weights' two halves, and its tokens; the first copies also say how many bytes will come
+    auto weights = [&](const CUtensorMap* map, int y0, int y1, int boxes, int s) {
+      if (ok) ok = warp_wait(empty + st, phase ^ 1u, abort_flag, p.status, 114);
+      if (!ok) return;
+      unsigned char* at = smem + (size_t)st * Lay::STAGE;
+      mbar_expect_tx_by(one, full + st, A_BYTES + (uint32_t)boxes * 2048u * (FP8 ? 2u : 1u));
+      tma_load_2d_by(one, at, map, full + st, s * STAGE_K, y0);
+      tma_load_2d_by(one, at + A_BYTES / 2, map, full + st, s * STAGE_K, y1);
+    };
+    auto tokens = [&](const CUtensorMap* map, int y, int mid, int boxes, int s) {
+      if (!ok) return;
+      unsigned char* at = smem + (size_t)st * Lay::STAGE + A_BYTES;
+      for (int b = 0; b < boxes; ++b) {
+        tma_load_2d_by(one, at + b * 2048, map, full + st, s * STAGE_K, y + 16 * b);
+        if (FP8) tma_load_2d_by(one, at + (boxes + b) * 2048, map, full + st, s * STAGE_K, mid + y + 16 * b);
+      }
     };
     auto step = [&]() {
       if (++st == p.stages) { st = 0; phase ^= 1u; }
-    };
-    // stage s of the piece, the copies of the roles in `mask`; the first ones also say how many bytes will come
-    auto copy = [&](int s, int mask) {
-      if (mask & 1) {
-        if (ok) ok = mbar_wait(empty + st, phase ^ 1u, abort_flag, p.status, 114);
-        if (lane == 0 && ok) mbar_expect_tx(full + st, bytes);
-      }
-      if (ok && (role & mask)) tma_load_2d(smem + (size_t)st * Lay::STAGE + dst, map, full + st, s * STAGE_K, y);
-      __syncwarp();
     };
     // the up products
     int t = draw(0);
     while (ok && t < up_pieces) {
       const int a = t / up_tiles, i0 = (t - a * up_tiles) * OUT, e = active[a];
       push({0, a, t - a * up_tiles, 0, up_stages, 0});
-      assign(&map_up, e * ffu + i0, e * ffu + i0 + (GLU ? p.ff : 64), &map_h, 0, p.n, NB / 16);
-      for (int s = 0; s < up_stages && ok; ++s, step()) copy(s, 3);
+      const int y0 = e * ffu + i0, y1 = y0 + (GLU ? p.ff : 64);
+      for (int s = 0; s < up_stages && ok; ++s, step()) {
+        weights(&map_up, y0, y1, NB / 16, s);
+        tokens(&map_h, 0, p.n, NB / 16, s);
+      }
       t = draw(0);                                             // not earlier: a CTA that starts first would take the others' first pieces
     }
     // the down products
@@ -404,81 +395,84 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int split = t % splits, a = t / splits % A, dt = t / splits / A, e = active[a];
       const int s0 = split * down_per, s1 = min(down_stages, s0 + down_per), c0 = first[a];
       push({1, a, dt, s0, s1, split});
-      assign(&map_down, e * p.d + dt * TILE, e * p.d + dt * TILE + 64, &map_u, c0, slots, (first[a + 1] - c0 + 15) / 16);
+      const int y0 = e * p.d + dt * TILE, boxes = (first[a + 1] - c0 + 15) / 16;
       int s = s0;
       if (!waited) {
         // the first weights are asked for before the wait for the up products
         waited = true;
         const int ahead = min(s1 - s0, p.stages), st_from = st;
         const uint32_t phase_from = phase;
-        for (int i = 0; i < ahead && ok; ++i, step()) copy(s0 + i, 1);
+        for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, boxes, s0 + i);
         if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         __threadfence();
         fence_async_all();                                     // u was written through the generic proxy
         st = st_from;
         phase = phase_from;
-        for (int i = 0; i < ahead; ++i, step()) copy(s0 + i, 2);
+        for (int i = 0; i < ahead; ++i, step()) tokens(&map_u, c0, slots, boxes, s0 + i);
         s = s0 + ahead;
       }
-      for (; s < s1 && ok; ++s, step()) copy(s, 3);
+      for (; s < s1 && ok; ++s, step()) {
+        weights(&map_down, y0, y0 + 64, boxes, s);
+        tokens(&map_u, c0, slots, boxes, s);
+      }
       t = draw(2);
     }
     push({-1, 0, 0, 0, 0, 0});
     if (*abort_flag)                                           // copies in flight land (they take microseconds) before the CTA ends
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   } else if (warp == 1) {
-    if (lane == 0) {
-      int st = 0, slot = 0;
-      uint32_t phase = 0u, slot_phase = 0u;
-      bool ok = true;
-      const uint64_t desc0 = smem_desc(smem);
-      for (int np = 0; ok; ++np) {
-        const int q = np % QUEUE;
-        if (!(ok = mbar_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 115))) break;
-        const Piece piece = queue[q];
-        mbar_arrive(q_empty + q);
-        if (piece.down < 0) break;
-        const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
-        const int cols = boxes * 16 * (FP8 ? 2 : 1);
-        const uint32_t idesc = FP8 ? (1u << 4) | ((uint32_t)(cols >> 3) << 17) | (8u << 24) : instr_desc(cols);
-        auto next_slot = [&]() {
-          ok = ok && mbar_wait(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
-          tc_fence_after();
-        };
-        auto commit_slot = [&]() {
-          tc_commit(acc_full + slot);
-          if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
-        };
-        if (!FP8) next_slot();
-        for (int s = piece.s0; s < piece.s1 && ok; ++s) {
-          if (!(ok = mbar_wait(full + st, phase, abort_flag, p.status, 117))) break;
-          tc_fence_after();
-          const uint64_t wd = desc0 + (uint64_t)(st * (Lay::STAGE / 16)), xd = wd + A_BYTES / 16;      // addresses count 16 bytes
-          if (FP8) {
+    const uint32_t one = elect_one();
+    int st = 0, slot = 0;
+    uint32_t phase = 0u, slot_phase = 0u;
+    bool ok = true;
+    const uint64_t desc0 = smem_desc(smem);
+    for (int np = 0; ok; ++np) {
+      const int q = np % QUEUE;
+      if (!(ok = warp_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 115))) break;
+      const Piece piece = queue[q];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty + q);
+      if (piece.down < 0) break;
+      const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
+      const int cols = boxes * 16 * (FP8 ? 2 : 1);
+      const uint32_t idesc = FP8 ? instr_desc_e4m3(cols) : instr_desc(cols);
+      auto next_slot = [&]() {
+        ok = ok && warp_wait(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
+        tc_fence_after();
+      };
+      auto commit_slot = [&]() {
+        tc_commit_by(one, acc_full + slot);
+        if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+      };
+      if (!FP8) next_slot();
+      for (int s = piece.s0; s < piece.s1 && ok; ++s) {
+        if (!(ok = warp_wait(full + st, phase, abort_flag, p.status, 117))) break;
+        tc_fence_after();
+        const uint64_t wd = desc0 + (uint64_t)(st * (Lay::STAGE / 16)), xd = wd + A_BYTES / 16;      // addresses count 16 bytes
+        if (FP8) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool fresh = k == 0 || (k == 2 && piece.down);      // a stage has one accumulator, in the down products two
-              if (fresh) {
-                if (k > 0) commit_slot();
-                next_slot();
-                if (!ok) break;
-              }
-              mma_8bit(tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, fresh ? 0u : 1u);
+          for (int k = 0; k < 4; ++k) {
+            const bool fresh = k == 0 || (k == 2 && piece.down);      // a stage has one accumulator, in the down products two
+            if (fresh) {
+              if (k > 0) commit_slot();
+              next_slot();
+              if (!ok) break;
             }
-            if (!ok) break;
-            tc_commit(empty + st);
-            commit_slot();
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc_mma(tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, (s > piece.s0 || k > 0) ? 1u : 0u);
-            tc_commit(empty + st);
+            tc_mma_8bit_by(one, tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, fresh ? 0u : 1u);
           }
-          if (++st == p.stages) { st = 0; phase ^= 1u; }
+          if (!ok) break;
+          tc_commit_by(one, empty + st);
+          commit_slot();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_by(one, tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, (s > piece.s0 || k > 0) ? 1u : 0u);
+          tc_commit_by(one, empty + st);
         }
-        if (!FP8 && ok) commit_slot();
+        if (++st == p.stages) { st = 0; phase ^= 1u; }
       }
+      if (!FP8 && ok) commit_slot();
     }
   } else {
     const int et = threadIdx.x - 64, ew = warp - 2;
