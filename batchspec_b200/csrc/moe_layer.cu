@@ -17,7 +17,7 @@
 //
 //   route    one cluster of 8 CTAs per 8 tokens: 64 warps share the router's rows and k, partial sums meet in the first CTA's
 //            shared memory, whose warps choose for a token each.  It also clears the counters of the second kernel.
-//   experts  one CTA per SM: a TMA warp that draws pieces of work, an MMA warp, four epilogue warps.  First the pieces of the up products
+//   experts  one CTA per SM: a TMA warp that draws pieces of work, an MMA warp, two groups of epilogue warps that take the pieces in turn.  First the pieces of the up products
 //            (128 rows of one expert) are drawn from one counter, then those of the down products (128 output columns of one expert,
 //            perhaps a slice of its k).  A piece of the second kind waits until every piece of the first kind is done; those
 //            have all been drawn by CTAs that run and wait for nothing, so it ends however many CTAs the device can hold.
@@ -33,7 +33,7 @@ namespace {
 
 constexpr int LAYER_TOKENS = 64;             // most tokens of a step
 constexpr int ROUTE_CLUSTER = 8, ROUTE_WARPS = 8, ROUTE_TOKENS = 8;
-constexpr int LAYER_THREADS = 192;           // TMA warp, MMA warp, 4 epilogue warps
+constexpr int LAYER_THREADS = 320;           // TMA warp, MMA warp, two groups of 4 epilogue warps
 constexpr int SMEM_BUDGET = 225 * 1024;
 
 // ------------------------------------------------------------------------------------------------ the router
@@ -43,18 +43,18 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
                        const void* __restrict__ corr, int corr_dtype, int C, int G, int keep, int top, float scale, int rule,
                        int* __restrict__ ids, float* __restrict__ wts, float* __restrict__ gate, int* __restrict__ counters,
                        uint8_t* __restrict__ hq, float* __restrict__ hs) {
-  bspec::pdl_prologue(84);
-  extern __shared__ float sm[];
   const int tiles = (rows + 15) / 16, units = tiles * slices;
-  float* part = sm;                                            // [units][8][16]
   const int rank = blockIdx.x % ROUTE_CLUSTER, t0 = blockIdx.x / ROUTE_CLUSTER * ROUTE_TOKENS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int steps = (d + 31) / 32, per = (steps + slices - 1) / slices;
+  bspec::pdl_prologue(84);
+  extern __shared__ float sm[];
+  float* part = sm;                                            // [units][8][16]
   if (blockIdx.x == 0 && threadIdx.x < 4) counters[threadIdx.x] = 0;
   // every CTA of the cluster runs before another one writes to its memory
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   uint32_t first;                                              // the first CTA's partials
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(first) : "r"(s32(part)), "r"(0));
-  const int steps = (d + 31) / 32, per = (steps + slices - 1) / slices;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const bool token = t0 + g < n;
   for (int unit = rank * ROUTE_WARPS + warp; unit < units; unit += ROUTE_CLUSTER * ROUTE_WARPS) {
@@ -143,7 +143,7 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
 // ------------------------------------------------------------------------------------------------ the experts
 constexpr int TILE = 128;                    // weight rows of a piece
 constexpr int A_BYTES = TILE * 128;          // of a stage: 128 bytes of every row
-constexpr int QUEUE = 4, SLOTS = 4;          // pieces on their way through the roles; accumulators
+constexpr int QUEUE = 4;                     // pieces on their way through the roles
 constexpr int MAX_STAGES = 10;
 constexpr int MAX_SPLITS = 4;                // slices of k of the down products
 
@@ -208,9 +208,9 @@ template <bool FP8, int NB>
 struct Layout {
   static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
   __host__ __device__ static int blocks(int k) { return (k + 63) / 64; }
-  // tile [NB][128], scales of two pieces' u [ff / 64][NB], then the lists
+  // of each epilogue group: tile [NB][128], scales of a piece's u [ff / 64][NB]; then the lists
   __host__ __device__ static size_t fixed(int ff, int slots, int E) {
-    return (size_t)NB * TILE * 4 + (FP8 ? (size_t)2 * blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
+    return (size_t)2 * NB * TILE * 4 + (FP8 ? (size_t)2 * blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
   }
 };
 
@@ -221,21 +221,22 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   using Lay = Layout<FP8, NB>;
   constexpr int STAGE_K = FP8 ? 128 : 64;                      // k of a stage
   constexpr int WIDTH = FP8 ? 2 * NB : NB;                     // columns of an accumulator
-  constexpr uint32_t TMEM_COLS = SLOTS * WIDTH;                // 64 .. 512
+  constexpr int SLOTS = FP8 && NB == 64 ? 2 : 4;               // accumulators of each epilogue group
+  constexpr uint32_t TMEM_COLS = 2 * SLOTS * WIDTH;            // 128 .. 512
   constexpr int OUT = GLU ? 64 : 128;                          // numbers of u per up piece
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[SLOTS], acc_empty[SLOTS], q_full[QUEUE], q_empty[QUEUE], meet;
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2 * SLOTS], acc_empty[2 * SLOTS], q_full[QUEUE], q_empty[QUEUE], meet[2];
   __shared__ Piece queue[QUEUE];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, n_active;
   volatile int* abort_flag = &abort_word;
   const int slots = p.n * p.top, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* tile = reinterpret_cast<float*>(smem + (size_t)p.stages * Lay::STAGE);          // [NB][128]
-  float* ys = tile + NB * TILE;
+  float* tile = reinterpret_cast<float*>(smem + (size_t)p.stages * Lay::STAGE);          // [2][NB][128]
+  float* ys = tile + 2 * NB * TILE;
   int* pos = reinterpret_cast<int*>(ys + (FP8 ? 2 * Lay::blocks(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
   int* tok = pos + slots;                                                                // [slots] tokens by expert
-  int* active = tok + slots;                                                             // [E] chosen experts, ascending
+  int* active = tok + slots;                                                             // [E] chosen experts
   int* first = active + p.E;                                                             // [E + 1] where their entries begin
   int* count = first + p.E + 1;                                                          // [E]
 
@@ -248,15 +249,16 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
     }
-    for (int i = 0; i < SLOTS; ++i) {
+    for (int i = 0; i < 2 * SLOTS; ++i) {
       mbar_init(acc_full + i, 1);
       mbar_init(acc_empty + i, 4);
     }
     for (int i = 0; i < QUEUE; ++i) {
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, 5);
+      mbar_init(q_empty + i, 9);
     }
-    mbar_init(&meet, 4);
+    mbar_init(meet, 4);
+    mbar_init(meet + 1, 4);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -271,13 +273,47 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   const uint32_t tmem_base = tmem_slot;
   bspec::pdl_prologue(85);
 
-  // ---- the entries by expert: counted, then placed in the order of their numbers, so that every CTA has the same order
-  for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
-    const int e = p.ids[s];
-    if (e < p.E) atomicAdd(count + e, 1);
+  // this CTA's first up piece, drawn while the lists are made
+  int first_piece = 0;
+  if (threadIdx.x == 0) first_piece = atomicAdd(p.counters, 1);
+  // ---- the entries by expert, in an order that every CTA finds alike
+  if (slots > 32) {
+    for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
+      const int e = p.ids[s];
+      if (e < p.E) atomicAdd(count + e, 1);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (warp == 0) {
+  if (slots <= 32 && warp == 0) {
+    // one entry per lane: experts in the order of their first entries
+    const int e = lane < slots ? p.ids[lane] : p.E;
+    const unsigned same = __match_any_sync(0xffffffffu, e), before = (1u << lane) - 1u;
+    const int leader = __ffs(same) - 1;
+    const bool leads = lane == leader && e < p.E;
+    int upto = leads ? __popc(same) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const int start = __shfl_sync(0xffffffffu, upto, leader) - __popc(same);
+    const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+    if (leads) {
+      active[__popc(leaders & before)] = e;
+      first[__popc(leaders & before)] = start;
+    }
+    if (e < p.E) {
+      pos[lane] = start + __popc(same & before);
+      tok[start + __popc(same & before)] = lane / p.top;
+    } else if (lane < slots) {
+      pos[lane] = -1;
+    }
+    if (lane == 31) {
+      first[__popc(leaders)] = upto;
+      n_active = __popc(leaders);
+    }
+  } else if (warp == 0) {
+    // counted, then placed in the order of their numbers
     int found = 0, run = 0;
 #pragma unroll 1
     for (int e0 = 0; e0 < p.E; e0 += 32) {
@@ -377,7 +413,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (++st == p.stages) { st = 0; phase ^= 1u; }
     };
     // the up products
-    int t = draw(0);
+    int t = __shfl_sync(0xffffffffu, first_piece, 0);
     while (ok && t < up_pieces) {
       const int a = t / up_tiles, i0 = (t - a * up_tiles) * OUT, e = active[a];
       push({0, a, t - a * up_tiles, 0, up_stages, 0});
@@ -423,8 +459,8 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   } else if (warp == 1) {
     const uint32_t one = elect_one();
-    int st = 0, slot = 0;
-    uint32_t phase = 0u, slot_phase = 0u;
+    int st = 0, ring[2] = {0, 0};                              // the groups' running accumulators
+    uint32_t phase = 0u, ring_phase[2] = {0u, 0u};
     bool ok = true;
     const uint64_t desc0 = smem_desc(smem);
     for (int np = 0; ok; ++np) {
@@ -437,13 +473,16 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
       const int cols = boxes * 16 * (FP8 ? 2 : 1);
       const uint32_t idesc = FP8 ? instr_desc_e4m3(cols) : instr_desc(cols);
+      const int group = np & 1;
+      int slot = group ? SLOTS + ring[1] : ring[0];
+      uint32_t slot_phase = group ? ring_phase[1] : ring_phase[0];
       auto next_slot = [&]() {
         ok = ok && warp_wait(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
         tc_fence_after();
       };
       auto commit_slot = [&]() {
         tc_commit_by(one, acc_full + slot);
-        if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+        if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
       };
       if (!FP8) next_slot();
       for (int s = piece.s0; s < piece.s1 && ok; ++s) {
@@ -473,13 +512,17 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         if (++st == p.stages) { st = 0; phase ^= 1u; }
       }
       if (!FP8 && ok) commit_slot();
+      if (group) ring[1] = slot - SLOTS, ring_phase[1] = slot_phase;
+      else ring[0] = slot, ring_phase[0] = slot_phase;
     }
   } else {
-    const int et = threadIdx.x - 64, ew = warp - 2;
+    const int group = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, ew = (warp - 2) & 3;
+    tile += group * NB * TILE;
+    ys += FP8 ? group * Lay::blocks(p.ff) * NB : 0;
     const uint32_t quad = warp & 3;
     const int row = (int)quad * 32 + lane;
     const uint32_t lane_base = tmem_base + ((quad * 32u) << 16);
-    int slot = 0;
+    int slot = group * SLOTS;
     uint32_t slot_phase = 0u, meet_phase = 0u;
     bool ok = true, up_known = false;
     // one arrival per warp: those of 32 lanes on one barrier would come one after the other
@@ -487,10 +530,10 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    // the epilogue threads meet (a bounded wait, so that none is left behind when another one gives up)
+    // the threads of a group meet (a bounded wait, so that none is left behind when another one gives up)
     auto meet_all = [&]() {
-      arrive(&meet);
-      ok = ok && mbar_wait(&meet, meet_phase, abort_flag, p.status, 118);
+      arrive(meet + group);
+      ok = ok && mbar_wait(meet + group, meet_phase, abort_flag, p.status, 118);
       meet_phase ^= 1u;
     };
     for (int np = 0; ok; ++np) {
@@ -499,6 +542,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const Piece piece = queue[q];
       arrive(q_empty + q);
       if (piece.down < 0) break;
+      if ((np & 1) != group) continue;                         // the other group's
       const int c0 = first[piece.a], cnt = first[piece.a + 1] - c0, e = active[piece.a];
       const int cols = piece.down ? (cnt + 15) / 16 * 16 : NB;
       float acc[FP8 ? NB : 1];
@@ -506,11 +550,10 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
 #pragma unroll
         for (int c = 0; c < NB; ++c) acc[c] = 0.f;
         if (piece.down) {
-          // the scales of this expert's u, for the first such piece once its first product says that the up products are done; into the other
-          // one of two buffers: the last piece's may still be read
+          // the scales of this expert's u, for the first such piece once its first product says that the up products are done
           if (!up_known) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           up_known = true;
-          ys = tile + NB * TILE + (np & 1) * Lay::blocks(p.ff) * NB;
+          meet_all();                                          // nobody reads the last piece's any more
           const int blocks = Lay::blocks(p.ff);
           for (int i = et; i < blocks * NB; i += 128) {
             const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
@@ -529,7 +572,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         auto take = [&]() -> uint32_t {                        // the next accumulator
           if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
-          if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+          if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
           return from;
         };
         for (int s = piece.s0; s < piece.s1; ++s) {
@@ -682,38 +725,50 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (!FP8) {
         tc_fence_before();
         arrive(acc_empty + slot);
-        if (++slot == SLOTS) { slot = 0; slot_phase ^= 1u; }
+        if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
       }
     }
     // ---- when every down piece of every CTA is done: the sums over the choices, four columns of a token per thread
     if (et == 0 && ok && !wait_for(p.counters + 3, down_pieces, p.status, abort_flag)) ok = false;
     __threadfence();
     meet_all();
-    const int quads = p.d / 4, parts = p.top * splits;
-    for (long long i = (long long)blockIdx.x * 128 + et; ok && i < (long long)p.n * quads; i += (long long)gridDim.x * 128) {
-      const int t = (int)(i / quads), c4 = 4 * (int)(i - (long long)t * quads);
+    ok = __all_sync(0xffffffffu, ok);
+    // few of them: eight lanes share a thread's results
+    const int quads = p.d / 4, parts = p.top * splits, threads = (int)gridDim.x * 256, share = p.n * quads * 8 <= threads ? 8 : 1;
+    const int inverse = (65536 + splits - 1) / splits;         // i / splits = i * inverse >> 16 for the few there are
+    const int sub = (threadIdx.x - 64) % share;
+    for (int i = ((int)blockIdx.x * 256 + (int)threadIdx.x - 64) / share; ok && i < p.n * quads; i += threads / share) {
+      const int t = i / quads, c4 = 4 * (i - t * quads);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p.add != nullptr) sum = scaled(four_bf16(p.add + (size_t)t * p.d + c4), p.gate != nullptr ? 1.f / (1.f + expf(-p.gate[t])) : 1.f);
-      int k = 0, split = 0;
+      if (p.add != nullptr && sub == 0)
+        sum = scaled(four_bf16(p.add + (size_t)t * p.d + c4), p.gate != nullptr ? 1.f / (1.f + expf(-p.gate[t])) : 1.f);
 #pragma unroll 1
-      for (int i0 = 0; i0 < parts; i0 += 8) {                  // eight (choice, slice) results in flight
+      for (int i0 = sub; i0 < parts; i0 += 8 * share) {        // eight (choice, slice) results in flight
         float4 x[8];
         float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          const int part = i0 + j * share, k = part * inverse >> 16, split = part - k * splits;
           w[j] = 0.f;
           x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i0 + j < parts) {
+          if (part < parts) {
             const int at = pos[t * p.top + k];
             w[j] = p.wts[t * p.top + k];
             if (at >= 0) x[j] = __ldcg(reinterpret_cast<const float4*>(p.y + ((size_t)split * entries + at) * p.d + c4));
             else if (split == 0) x[j] = four_bf16(p.h + (size_t)t * p.d + c4);
           }
-          if (++split == splits) { split = 0; ++k; }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           sum = make_float4(fmaf(w[j], x[j].x, sum.x), fmaf(w[j], x[j].y, sum.y), fmaf(w[j], x[j].z, sum.z), fmaf(w[j], x[j].w, sum.w));
+      }
+      if (share == 8) {
+        const unsigned eight = 0xffu << (lane & 24);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1)
+          sum = make_float4(sum.x + __shfl_xor_sync(eight, sum.x, o), sum.y + __shfl_xor_sync(eight, sum.y, o),
+                            sum.z + __shfl_xor_sync(eight, sum.z, o), sum.w + __shfl_xor_sync(eight, sum.w, o));
+        if (sub != 0) continue;
       }
       const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
       *reinterpret_cast<uint2*>(p.out + (size_t)t * p.d + c4) =
@@ -799,7 +854,7 @@ BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, i
       top > C || G <= 0 || C % G || keep <= 0 || keep > G || (long long)keep * (C / G) < top || (fp8 && sd == nullptr) || (rows > C && add == nullptr) ||
       ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(wu) | reinterpret_cast<uintptr_t>(wd) |
         reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(add)) & 15) ||
-      (long long)E * ffu > 0x7fffffff - 256 || (long long)E * d > 0x7fffffff - 256)
+      (long long)E * ffu > 0x7fffffff - 256 || (long long)E * d > 0x7fffffff - 256 || (long long)top * MAX_SPLITS > 16384)
     return (int)cudaErrorInvalidValue;
   long long at[AT_PARTS];
   places(n, d, ff, top, fp8, at);
@@ -829,7 +884,9 @@ BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, i
     const cudaError_t e = cudaFuncSetAttribute(moe_layer_route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return (int)e;
   }
-  BSPEC_LAUNCH((moe_layer_route_kernel), ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS), 32 * ROUTE_WARPS, smem, stream,
+  // started when the kernel before has ended: launched early, its clusters go wherever that one's CTAs happen to end first (measured, 61 tokens:
+  // 151 us instead of 142)
+  BSPEC_LAUNCH_SERIALIZED((moe_layer_route_kernel), ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS), 32 * ROUTE_WARPS, smem, stream,
                (const __nv_bfloat16*)h, n, d, (const __nv_bfloat16*)router, rows, slices, corr, corr_dtype, C, G, keep, top, scale, rule,
                (int*)(base + at[AT_IDS]), (float*)(base + at[AT_WTS]), (float*)(base + at[AT_GATE]), counters,
                fp8 ? (uint8_t*)(base + at[AT_HQ]) : (uint8_t*)nullptr, (float*)(base + at[AT_HS]));

@@ -1483,17 +1483,18 @@ def _sgemm(x, w, out, M: int, N: int, K: int, lda: int, ldw: int, sa: int, sw: i
 FP8_BLOCK = 128                   # numbers of a row that share a scale; weights share one per 128 x 128
 
 
-def _stream_of(*tensors) -> int:
+def _stream_of(first: torch.Tensor, *others) -> int:
     """The current stream of the device that all tensors are on, which has to be the current device."""
-    dev = tensors[0].device
-    for t in tensors:
+    dev = first.device
+    for t in others:
         if t is not None and t.device != dev:
             raise KernelError(f"tensors on {dev} and {t.device}: one launch takes tensors of one device")
     if dev.type != "cuda":
         raise KernelError("batchspec_b200 kernels run on a CUDA device only; got a tensor on " + str(dev))
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != torch.cuda.current_device():
         raise KernelError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
-    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
@@ -1509,46 +1510,49 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
         raise KernelError(f"quantize_fp8 takes float32 or bfloat16, got {x.dtype}")
     if block_rows not in (1, FP8_BLOCK):
         raise KernelError(f"quantize_fp8: blocks of {block_rows} rows are not supported (1 or {FP8_BLOCK})")
-    if x.dim() < 2 or x.shape[-1] < 1:
-        raise KernelError(f"quantize_fp8 takes matrices of at least one column, got shape {tuple(x.shape)}")
-    R, K = x.shape[-2:]
-    if x.dim() == 2:
+    shape = x.shape
+    if len(shape) < 2 or shape[-1] < 1:
+        raise KernelError(f"quantize_fp8 takes matrices of at least one column, got shape {tuple(shape)}")
+    R, K = shape[-2], shape[-1]
+    pitch, RB, KB = (K + 15) // 16 * 16, (R + block_rows - 1) // block_rows, (K + FP8_BLOCK - 1) // FP8_BLOCK
+    if len(shape) == 2:
         if K > 1 and x.stride(1) != 1:
             raise KernelError("quantize_fp8: the numbers of a row have to be dense")
         batch, ldx = 1, (x.stride(0) if R > 1 else K)
+        q, scale = x.new_empty((R, pitch), dtype=torch.float8_e4m3fn), x.new_empty((RB, KB), dtype=torch.float8_e8m0fnu)
     else:
         if not x.is_contiguous():
             raise KernelError("quantize_fp8: a tensor of more than two dimensions has to be contiguous")
-        batch, ldx = x.shape[:-2].numel(), K
-    lib = load_library(features=("fp8",))
-    pitch, KB = (K + 15) // 16 * 16, (K + FP8_BLOCK - 1) // FP8_BLOCK
-    q = torch.empty(x.shape[:-1] + (pitch,), dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-2] + ((R + block_rows - 1) // block_rows, KB), dtype=torch.float8_e8m0fnu, device=x.device)
-    if batch * R:
-        _check(lib.bspec_quantize_fp8(x.data_ptr(), _dtype_code(x.dtype), ldx, R * ldx, q.data_ptr(), pitch, scale.data_ptr(), batch, R,
-                                      K, block_rows, stream), "quantize_fp8")
+        batch, ldx = shape[:-2].numel(), K
+        q, scale = x.new_empty(shape[:-1] + (pitch,), dtype=torch.float8_e4m3fn), x.new_empty(shape[:-2] + (RB, KB), dtype=torch.float8_e8m0fnu)
+    if batch and R:
+        _check(load_library(features=("fp8",)).bspec_quantize_fp8(
+            x.data_ptr(), _dtype_code(x.dtype), ldx, R * ldx, q.data_ptr(), pitch, scale.data_ptr(), batch, R, K, block_rows, stream),
+            "quantize_fp8")
     return (q if pitch == K else q[..., :K]), scale
 
 
 def _fp8_rows(t: torch.Tensor, name: str) -> int:
     """Bytes from row to row of an e4m3 matrix that a tensor map can describe."""
-    rows, K = t.shape
-    if t.dtype != torch.float8_e4m3fn or (K > 1 and t.stride(1) != 1):
+    (rows, K), (stride, step) = t.shape, t.stride()
+    if t.dtype != torch.float8_e4m3fn or (K > 1 and step != 1):
         raise KernelError(f"linear_fp8: {name} has to be float8_e4m3fn with dense rows, got {t.dtype} with strides {t.stride()}")
-    ld = t.stride(0) if rows > 1 else (K + 15) // 16 * 16
+    ld = stride if rows > 1 else (K + 15) // 16 * 16
     if ld % 16 or ld < K or t.data_ptr() % 16:
         raise KernelError(f"linear_fp8: the rows of {name} have to start on 16-byte boundaries (as quantize_fp8 lays them out), "
                           f"got a row stride of {ld} bytes")
     return ld
 
 
-def _fp8_scales(t: torch.Tensor, shape, name: str):
+def _fp8_scales(t: torch.Tensor, rows: int, cols: int, name: str):
     """(scales from row to row, whether they are 8-bit exponents) of a matrix of scales."""
-    if t.dtype not in (torch.float32, torch.float8_e8m0fnu) or tuple(t.shape) != tuple(shape):
-        raise KernelError(f"{name} has to be float32 or float8_e8m0fnu of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    e8m0 = t.dtype == torch.float8_e8m0fnu
+    if not (e8m0 or t.dtype == torch.float32) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise KernelError(f"{name} has to be float32 or float8_e8m0fnu of shape {(rows, cols)}, got {t.dtype} of {tuple(t.shape)}")
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
         raise KernelError(f"{name} has to have dense rows")
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1]), int(t.dtype == torch.float8_e8m0fnu)
+    return (ld if rows > 1 else cols), int(e8m0)
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -1564,9 +1568,9 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     (M, K), N = x.shape, w.shape[0]
     KB = (K + FP8_BLOCK - 1) // FP8_BLOCK
     ldx, ldw = _fp8_rows(x, "x"), _fp8_rows(w, "w")
-    ldxs, xe = _fp8_scales(x_scale, (M, KB), "linear_fp8: x_scale")
-    ldws, we = _fp8_scales(w_scale, ((N + FP8_BLOCK - 1) // FP8_BLOCK, KB), "linear_fp8: w_scale")
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    ldxs, xe = _fp8_scales(x_scale, M, KB, "linear_fp8: x_scale")
+    ldws, we = _fp8_scales(w_scale, (N + FP8_BLOCK - 1) // FP8_BLOCK, KB, "linear_fp8: w_scale")
+    out = x.new_empty((M, N), dtype=out_dtype)
     if M and N:
         _check(load_library(features=("fp8",)).bspec_gemm_fp8(
             x.data_ptr(), ldx, x_scale.data_ptr(), ldxs, xe, w.data_ptr(), ldw, w_scale.data_ptr(), ldws, we, out.data_ptr(),
@@ -1957,12 +1961,12 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
         e8m0 = int(up_scale.dtype == torch.float8_e8m0fnu)
     elif up_scale is not None or down_scale is not None:
         raise KernelError("moe_layer: bfloat16 experts take no scales")
-    out = torch.empty((n, d), dtype=h.dtype, device=h.device)
+    out = torch.empty_like(h)
     if n == 0:
         return out
     lib = load_library(features=("moe",))
     # everything between the two kernels, counters too: a buffer of its own, so that calls on other streams or in other graphs share nothing
-    scratch = torch.empty((lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8)),), dtype=torch.uint8, device=h.device)
+    scratch = h.new_empty((lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8)),), dtype=torch.uint8)
     rule = (1 if softmax_top else 2 if softmax else 0) + (4 if group_max else 0) + (8 if renormalise else 0)
     _check(lib.bspec_moe_layer(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),
                                _dtype_code(correction.dtype) if correction is not None else F32, many, int(n_groups), int(keep), int(top),
