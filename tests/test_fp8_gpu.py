@@ -162,6 +162,43 @@ def test_product(ops, M, N, K, scales, out_dtype):
     ops.check_status()
 
 
+@pytest.mark.parametrize("scales", ["", "w"])       # powers of two alone go to the pairs of CTAs, the others not
+@pytest.mark.parametrize("M,N,K", [(2048, 8192, 1024), (1500, 10001, 650), (513, 16800, 2000), (3000, 4480, 4200), (257, 20011, 129), (1025, 7168, 384),
+                                   (300, 33000, 640)])
+def test_product_of_many_tiles(ops, M, N, K, scales):
+    """Several tiles per CTA, ends inside tiles and inside groups of four blocks of k, rows of the result on odd places."""
+    x, xs, w, ws = product_case(ops, M, N, K, scales, M + N + K)
+    for out_dtype in (torch.bfloat16, torch.float32):
+        check_product(ops.linear_fp8(x, xs, w, ws, out_dtype=out_dtype), x, xs, w, ws)
+    ops.check_status()
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Matrices of more than 2^31 numbers: the last rows of a quantised one, of the weights and of a result."""
+    g = generator(41)
+    x = torch.zeros(70000, 40000, device=DEV, dtype=torch.bfloat16)
+    x[-200:] = torch.randn(200, 40000, device=DEV, generator=g).to(torch.bfloat16)
+    tail = x[-200:].clone()
+    for block_rows in (1, 128):
+        q, s = ops.quantize_fp8(x, block_rows)
+        top = 70000 // 128 * 128                                   # the last whole block row begins here
+        want_q, want_s = ops.quantize_fp8(x[top:] if block_rows == 128 else x[-3:], block_rows)
+        assert torch.equal(q[-3:].float(), want_q[-3:].float()) and torch.equal(s[-1:].float(), want_s[-1:].float())
+        assert int((q[:1000].float() != 0).sum()) == 0
+    del x
+    a, sa = ops.quantize_fp8(tail[:3])
+    out = ops.linear_fp8(a, sa, q, s, out_dtype=torch.float32)     # weights of 2.8 GB
+    check_product(out[:, top:], a, sa, q[top:], s[top // 128:])
+    del q, s, out
+    w, sw = ops.quantize_fp8(torch.randn(40000, 128, device=DEV, generator=g), 128)
+    y, sy = ops.quantize_fp8(torch.randn(70000, 128, device=DEV, generator=g))
+    for scales in (sy, sy.float()):                                # results of 5.6 GB
+        out = ops.linear_fp8(y, scales, w, sw)
+        check_product(out[-300:], y[-300:], scales[-300:], w, sw)
+        check_product(out[:3], y[:3], scales[:3], w, sw)
+        del out
+
+
 @pytest.mark.parametrize("M", [3, 40, 96, 2000])
 def test_product_of_views(ops, M):
     """Rows of wider matrices, scales of wider matrices, and neighbours of the result left alone."""

@@ -140,6 +140,11 @@ CASES = [
     (61, 64, 16, 6, 2048, 1408, True, "softmax", 8, 4, "gated", True),
     (64, 100, 0, 8, 176, 80, False, "softmax_top", 1, 1, None, True),
     (5, 1000, 24, 8, 64, 16, True, "sigmoid", 1, 1, None, True),
+    (4, 40, 0, 8, 4096, 1024, True, "softmax_top", 1, 1, None, True),
+    (5, 3, 0, 1, 1024, 4096, False, "sigmoid", 1, 1, "plain", False),
+    (33, 24, 8, 4, 1152, 896, True, "softmax", 1, 1, None, True),
+    (48, 2, 0, 1, 512, 2048, True, "softmax_top", 1, 1, "gated", True),
+    (64, 300, 0, 5, 2048, 160, True, "softmax_top", 1, 1, None, True),
 ]
 
 
@@ -176,9 +181,10 @@ def test_every_8bit_number(ops):
     check_layer(ops.moe_layer(*args, **kw), args, kw, up.double() * 2.0 ** -9, down.double() * 2.0 ** -9, "softmax_top")
 
 
-def test_a_token_of_nan_stays_in_its_row(ops):
+@pytest.mark.parametrize("weights", ["bfloat16", "float32"])
+def test_a_token_of_nan_stays_in_its_row(ops, weights):
     for n in (4, 30):
-        args, kw, upv, downv = layer_case(ops, n, 16, 0, 4, 256, 64, True, "bfloat16", "softmax_top", 1, 1, None, True)
+        args, kw, upv, downv = layer_case(ops, n, 16, 0, 4, 256, 64, True, weights, "softmax_top", 1, 1, None, True)
         want = ops.moe_layer(*args, **kw)
         args[0][1, 7] = math.nan
         out = ops.moe_layer(*args, **kw)
@@ -186,6 +192,54 @@ def test_a_token_of_nan_stays_in_its_row(ops):
         others = [t for t in range(n) if t != 1]
         check_layer(out, args, kw, upv, downv, "softmax_top", rows=others)
         assert not bool(torch.isnan(out[others].float()).any()) and out.shape == want.shape
+
+
+def test_steps_whose_choices_are_all_identity_experts(ops):
+    """No expert is read; tokens are weighted copies of themselves (and of ``add``)."""
+    for n, shared in ((1, None), (7, "gated"), (40, "plain")):
+        args, kw, upv, downv = layer_case(ops, n, 6, 10, 3, 144, 48, True, "bfloat16", "softmax", 1, 1, shared, True)
+        args[2][:] = 0
+        args[2][6:] = 4
+        check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax")
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e8m0"])
+def test_tokens_of_very_different_sizes(ops, weights):
+    """Tokens from 2^-100 to 2^60: a router that is zero for them makes the choice independent of the sizes."""
+    args, kw, upv, downv = layer_case(ops, 20, 8, 0, 2, 256, 128, False, weights, "softmax_top", 1, 1, None, True)
+    h, router = args[0], args[1]
+    router.zero_()
+    h *= torch.exp2(torch.linspace(-100, 60, 20, device=DEV).round())[:, None].to(torch.bfloat16)
+    check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax_top")
+
+
+def test_a_nan_among_the_weights_shows_in_its_column(ops):
+    for weights in ("bfloat16", "float32"):
+        args, kw, upv, downv = layer_case(ops, 3, 2, 0, 2, 256, 128, True, weights, "softmax_top", 1, 1, None, True)
+        down = args[8]
+        if weights == "bfloat16":
+            down[1, 77, 5] = math.nan
+        else:
+            down.view(torch.uint8)[1, 77, 5] = 0x7F
+        out = ops.moe_layer(*args, **kw).float()
+        assert bool(torch.isnan(out[:, 77]).all()) and int(torch.isnan(out).sum()) == 3
+
+
+def test_experts_beyond_32_bits(ops):
+    """Stacked weights of more than 2^31 numbers: the last experts."""
+    E, d, ff = 72, 2048, 8192
+    args, kw, _, _ = layer_case(ops, 3, 1, 0, 1, d, 64, True, "bfloat16", "softmax_top", 1, 1, None, False)
+    g = generator(3)
+    up, down = torch.zeros(E, 2 * ff, d, device=DEV, dtype=torch.bfloat16), torch.zeros(E, d, ff, device=DEV, dtype=torch.bfloat16)
+    up[-2:] = torch.randn(2, 2 * ff, d, device=DEV, generator=g) * d ** -0.5
+    down[-2:] = torch.randn(2, d, ff, device=DEV, generator=g) * ff ** -0.5
+    correction = torch.zeros(E, device=DEV)
+    correction[-2:] = torch.tensor([9.0, 8.5], device=DEV)
+    router = torch.zeros(E, d, device=DEV, dtype=torch.bfloat16)
+    args = (args[0], router, correction, 1, 1, 2, 1.0, up, down)
+    out = ops.moe_layer(*args, **kw)
+    small = (args[0], router[-2:].contiguous(), correction[-2:].contiguous(), 1, 1, 2, 1.0, up[-2:].contiguous(), down[-2:].contiguous())
+    check_layer(out, small, kw, up[-2:].double(), down[-2:].double(), "softmax_top")
 
 
 def test_agrees_with_the_separate_operators(ops):
