@@ -48,6 +48,42 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int steps = (d + 31) / 32, per = (steps + slices - 1) / slices;
   bspec::pdl_prologue(84);
+  const int chooses = ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS);      // CTAs
+  if ((int)blockIdx.x >= chooses) {
+    // 8-bit experts: the clusters behind those that choose bring a token per CTA into two 8-bit numbers for each of its own, with one scale
+    const int row = blockIdx.x - chooses;
+    if (row >= n) return;
+    __shared__ uint32_t warp_max[ROUTE_WARPS];
+    uint32_t m = 0u;
+    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUTE_WARPS; ++i) m = max(m, warp_max[i]);
+    const int code = scale_code(m);
+    const float inv = inverse_scale(code);
+    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float v[4] = {__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
+                            __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u)};
+        two_e4m3x4(v, inv, hi[i], lo[i]);
+      }
+      *reinterpret_cast<uint2*>(hq + (size_t)row * d + k) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(hq + (size_t)(n + row) * d + k) = make_uint2(lo[0], lo[1]);
+    }
+    if (threadIdx.x == 0) hs[row] = scale_value(code);
+    return;
+  }
   extern __shared__ float sm[];
   float* part = sm;                                            // [units][8][16]
   if (blockIdx.x == 0 && threadIdx.x < 4) counters[threadIdx.x] = 0;
@@ -89,39 +125,6 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   if (rank == 0)
     for (int e = threadIdx.x; e < C; e += 32 * ROUTE_WARPS) bias[e] = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  // 8-bit experts: CTA `rank` brings token t0 + rank into two 8-bit numbers for each of its own, with one scale
-  if (hq != nullptr && t0 + rank < n) {
-    const int row = t0 + rank;
-    __shared__ uint32_t warp_max[ROUTE_WARPS];
-    uint32_t m = 0u;
-    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) warp_max[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ROUTE_WARPS; ++i) m = max(m, warp_max[i]);
-    const int code = scale_code(m);
-    const float inv = inverse_scale(code);
-    for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t hi[2], lo[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float v[4] = {__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
-                            __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u)};
-        two_e4m3x4(v, inv, hi[i], lo[i]);
-      }
-      *reinterpret_cast<uint2*>(hq + (size_t)row * d + k) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(hq + (size_t)(n + row) * d + k) = make_uint2(lo[0], lo[1]);
-    }
-    if (threadIdx.x == 0) hs[row] = scale_value(code);
-  }
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int t = t0 + warp;
@@ -226,7 +229,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   constexpr int OUT = GLU ? 64 : 128;                          // numbers of u per up piece
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2 * SLOTS], acc_empty[2 * SLOTS], q_full[QUEUE], q_empty[QUEUE], meet[2];
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2 * SLOTS], acc_empty[2 * SLOTS], q_full[QUEUE], q_empty[QUEUE], meet[2], up_done;
   __shared__ Piece queue[QUEUE];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, n_active;
@@ -259,6 +262,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     }
     mbar_init(meet, 4);
     mbar_init(meet + 1, 4);
+    mbar_init(&up_done, 1);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -440,8 +444,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const uint32_t phase_from = phase;
         for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, boxes, s0 + i);
         if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
+        if (lane == 0 && ok) mbar_arrive(&up_done);            // the epilogue may read the scales of u
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        __threadfence();
+        __syncwarp();
         fence_async_all();                                     // u was written through the generic proxy
         st = st_from;
         phase = phase_from;
@@ -549,18 +554,6 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (FP8) {
 #pragma unroll
         for (int c = 0; c < NB; ++c) acc[c] = 0.f;
-        if (piece.down) {
-          // the scales of this expert's u, for the first such piece once its first product says that the up products are done
-          if (!up_known) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
-          up_known = true;
-          meet_all();                                          // nobody reads the last piece's any more
-          const int blocks = Lay::blocks(p.ff);
-          for (int i = et; i < blocks * NB; i += 128) {
-            const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
-            if (c < cols) ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
-          }
-          meet_all();
-        }
         // the weights' scale of this thread's row
         const int rows_all = piece.down ? p.d : ffu, K = piece.down ? p.ff : p.d, KB = (K + 127) / 128;
         const int w_row = piece.down ? piece.tile * TILE + row : (GLU && row >= 64 ? p.ff + piece.tile * 64 + row - 64 : piece.tile * OUT + row);
@@ -569,6 +562,26 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const size_t ws_at = (size_t)e * ((rows_all + 127) / 128);
         const float* ws = piece.down ? p.sd : p.su;
         float wa = 0.f, wb = 0.f;
+        auto weight_scales = [&](int s) {                      // asked for before the waits below
+          if (s + lane < piece.s1) {
+            wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + s + lane);
+            wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + s + lane);
+          }
+        };
+        weight_scales(piece.s0);
+        if (piece.down) {
+          // the scales of this expert's u, which arrive while its first copies do
+          if (!up_known) ok = mbar_wait(&up_done, 0u, abort_flag, p.status, 120);
+          up_known = true;
+          meet_all();                                          // nobody reads the last piece's any more
+          const int blocks = Lay::blocks(p.ff);
+#pragma unroll 4
+          for (int i = et; i < blocks * cols; i += 128) {
+            const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
+            ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
+          }
+          meet_all();
+        }
         auto take = [&]() -> uint32_t {                        // the next accumulator
           if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
@@ -577,10 +590,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         };
         for (int s = piece.s0; s < piece.s1; ++s) {
           const int ahead = (s - piece.s0) & 31;
-          if (ahead == 0 && s + lane < piece.s1) {
-            wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + s + lane);
-            wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + s + lane);
-          }
+          if (ahead == 0 && s > piece.s0) weight_scales(s);
           __syncwarp();
           const float w_a = __shfl_sync(0xffffffffu, wa, ahead), w_b = __shfl_sync(0xffffffffu, wb, ahead);
           const float w = w_block == block_a ? w_a : w_b;
@@ -886,7 +896,7 @@ BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, i
   }
   // started when the kernel before has ended: launched early, its clusters go wherever that one's CTAs happen to end first (measured, 61 tokens:
   // 151 us instead of 142)
-  BSPEC_LAUNCH_SERIALIZED((moe_layer_route_kernel), ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS), 32 * ROUTE_WARPS, smem, stream,
+  BSPEC_LAUNCH_SERIALIZED((moe_layer_route_kernel), ROUTE_CLUSTER * ((n + ROUTE_TOKENS - 1) / ROUTE_TOKENS) * (fp8 ? 2 : 1), 32 * ROUTE_WARPS, smem, stream,
                (const __nv_bfloat16*)h, n, d, (const __nv_bfloat16*)router, rows, slices, corr, corr_dtype, C, G, keep, top, scale, rule,
                (int*)(base + at[AT_IDS]), (float*)(base + at[AT_WTS]), (float*)(base + at[AT_GATE]), counters,
                fp8 ? (uint8_t*)(base + at[AT_HQ]) : (uint8_t*)nullptr, (float*)(base + at[AT_HS]));
