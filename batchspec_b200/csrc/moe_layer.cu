@@ -210,7 +210,7 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) { return make
 template <bool FP8, int NB>
 struct Layout {
   static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
-  __host__ __device__ static int blocks(int k) { return (k + 63) / 64; }
+  __host__ __device__ static int blocks(int k) { return (k + 127) / 128 * 2; }             // of 64, in whole stages
   // of each epilogue group: tile [NB][128], scales of a piece's u [ff / 64][NB]; then the lists
   __host__ __device__ static size_t fixed(int ff, int slots, int E) {
     return (size_t)2 * NB * TILE * 4 + (FP8 ? (size_t)2 * blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
@@ -555,129 +555,96 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
 #pragma unroll
         for (int c = 0; c < NB; ++c) acc[c] = 0.f;
         // the weights' scale of this thread's row
-        const int rows_all = piece.down ? p.d : ffu, K = piece.down ? p.ff : p.d, KB = (K + 127) / 128;
+        const int rows_all = piece.down ? p.d : ffu, KB = ((piece.down ? p.ff : p.d) + 127) / 128;
         const int w_row = piece.down ? piece.tile * TILE + row : (GLU && row >= 64 ? p.ff + piece.tile * 64 + row - 64 : piece.tile * OUT + row);
         // lane l holds those of stage l of the next 32, for the two row blocks that the warp's rows can lie in
         const int w_block = min(w_row, rows_all - 1) / 128, block_a = __shfl_sync(0xffffffffu, w_block, 0), block_b = __shfl_sync(0xffffffffu, w_block, 31);
         const size_t ws_at = (size_t)e * ((rows_all + 127) / 128);
         const float* ws = piece.down ? p.sd : p.su;
-        float wa = 0.f, wb = 0.f;
-        auto weight_scales = [&](int s) {                      // asked for before the waits below
-          if (s + lane < piece.s1) {
-            wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + s + lane);
-            wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + s + lane);
+        const int steps = (piece.s1 - piece.s0) << piece.down;          // accumulators: a stage has one, in the down products two
+        // the columns' scales (asked for with the first weights' scales, while the first copies are on their way)
+        if (piece.down && !up_known) ok = mbar_wait(&up_done, 0u, abort_flag, p.status, 120);
+        up_known = piece.down;
+        meet_all();                                            // nobody reads the last piece's any more
+        {
+          const int blocks = (p.ff + 63) / 64, rows = piece.down ? Lay::blocks(p.ff) : 1, some = piece.down ? cnt : p.n;
+          const float* from = piece.down ? p.us + (size_t)c0 * blocks : p.hs;
+          for (int i = et; i < rows * cols; i += 128) {
+            const int c = i / rows, b = i - c * rows;          // neighbours read neighbouring blocks of an entry
+            ys[b * NB + c] = c < some && b < blocks ? __ldcg(from + (piece.down ? c * blocks + b : c)) : 0.f;
           }
-        };
-        weight_scales(piece.s0);
-        if (piece.down) {
-          // the scales of this expert's u, which arrive while its first copies do
-          if (!up_known) ok = mbar_wait(&up_done, 0u, abort_flag, p.status, 120);
-          up_known = true;
-          meet_all();                                          // nobody reads the last piece's any more
-          const int blocks = Lay::blocks(p.ff);
-#pragma unroll 4
-          for (int i = et; i < blocks * cols; i += 128) {
-            const int c = i / blocks, b = i - c * blocks;      // neighbours read neighbouring blocks of an entry
-            ys[b * NB + c] = c < cnt ? __ldcg(p.us + (size_t)(c0 + c) * blocks + b) : 0.f;
-          }
-          meet_all();
         }
-        auto take = [&]() -> uint32_t {                        // the next accumulator
+        meet_all();
+        const float* f = ys + (piece.down ? 2 * piece.s0 * NB : 0);
+        float wa = 0.f, wb = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+          const int s = i >> piece.down;
+          if ((i & (32 << piece.down) - 1) == 0 && piece.s0 + s + lane < piece.s1) {
+            wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + piece.s0 + s + lane);
+            wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + piece.s0 + s + lane);
+          }
+          __syncwarp();
+          const float w_a = __shfl_sync(0xffffffffu, wa, s & 31), w_b = __shfl_sync(0xffffffffu, wb, s & 31);
+          const float w = w_block == block_a ? w_a : w_b;
           if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
-          if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
-          return from;
-        };
-        for (int s = piece.s0; s < piece.s1; ++s) {
-          const int ahead = (s - piece.s0) & 31;
-          if (ahead == 0 && s > piece.s0) weight_scales(s);
-          __syncwarp();
-          const float w_a = __shfl_sync(0xffffffffu, wa, ahead), w_b = __shfl_sync(0xffffffffu, wb, ahead);
-          const float w = w_block == block_a ? w_a : w_b;
-          const int slot_a = slot;
-          const uint32_t from = take();
-          if (!piece.down) {
-            tc_fence_after();
+          tc_fence_after();
 #pragma unroll
-            for (int cc = 0; cc < NB; cc += 16) {
+          for (int cc = 0; cc < NB; cc += 16)
+            if (cc < cols) {
               uint32_t hi[16], lo[16];
               tc_ld16(from + cc, hi);
-              tc_ld16(from + NB + cc, lo);
+              tc_ld16(from + cols + cc, lo);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                acc[cc + i] = fmaf(fmaf(__uint_as_float(lo[i]), 0.0625f, __uint_as_float(hi[i])), w, acc[cc + i]);
-            }
-            tc_fence_before();
-            arrive(acc_empty + slot_a);
-          } else {
-            const int slot_b = slot;
-            const uint32_t from_b = take();
-            tc_fence_after();
-            const bool two = s * 128 + 64 < K;                 // (a block behind the rows' ends has no scales)
-            const float4* fa = reinterpret_cast<const float4*>(ys + 2 * s * NB);
-            const float4* fb = reinterpret_cast<const float4*>(ys + (two ? 2 * s + 1 : 2 * s) * NB);
-            const float w2 = two ? w : 0.f;
+              for (int j = 0; j < 16; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(f + cc + j);
+                const float fx[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int cc = 0; cc < NB; cc += 16)
-              if (cc < cols) {
-                uint32_t hi[16], lo[16], hb[16], lb[16];
-                tc_ld16(from + cc, hi);
-                tc_ld16(from + cols + cc, lo);
-                tc_ld16(from_b + cc, hb);
-                tc_ld16(from_b + cols + cc, lb);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float4 x = fa[cc / 4 + i], z = fb[cc / 4 + i];
-                  const float fx[4] = {x.x, x.y, x.z, x.w}, fz[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const int c = 4 * i + j;
-                    const float va = fmaf(__uint_as_float(lo[c]), 0.0625f, __uint_as_float(hi[c]));
-                    const float vb = fmaf(__uint_as_float(lb[c]), 0.0625f, __uint_as_float(hb[c]));
-                    acc[cc + c] = fmaf(va * fx[j], w, fmaf(vb * fz[j], w2, acc[cc + c]));
-                  }
-                }
+                for (int k = 0; k < 4; ++k)
+                  acc[cc + j + k] = fmaf(fmaf(__uint_as_float(lo[j + k]), 0.0625f, __uint_as_float(hi[j + k])) * fx[k], w, acc[cc + j + k]);
               }
-            tc_fence_before();
-            arrive(acc_empty + slot_a);
-            arrive(acc_empty + slot_b);
-          }
+            }
+          tc_fence_before();
+          arrive(acc_empty + slot);
+          if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
+          f += piece.down ? NB : 0;
         }
       } else {
         ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
         tc_fence_after();
       }
-      if (!piece.down) {
-        // all columns to shared memory, then the activation, entry by entry
-        meet_all();                                            // the last piece's tile has been read
-        if (FP8) {
+      // to shared memory, from where a few instructions per entry take them on: what is executed once per piece costs the fetch of its
+      // code (most of it from DRAM, as a step's weights pass through the L2) more than its work
+      meet_all();                                              // the last piece's tile has been read
+      if (FP8) {
 #pragma unroll
-          for (int c = 0; c < NB; ++c) tile[c * TILE + row] = acc[FP8 ? c : 0];
-        } else if (ok) {
+        for (int c = 0; c < NB; ++c) tile[c * TILE + row] = acc[FP8 ? c : 0];
+      } else if (ok) {
+#pragma unroll 1
+        for (int cc = 0; cc < cols; cc += 16) {
+          uint32_t v[16];
+          tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
+          tc_wait_ld();
 #pragma unroll
-          for (int cc = 0; cc < NB; cc += 16) {
-            uint32_t v[16];
-            tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
-            tc_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 16; ++c) tile[(cc + c) * TILE + row] = __uint_as_float(v[c]);
-          }
+          for (int c = 0; c < 16; ++c) tile[(cc + c) * TILE + row] = __uint_as_float(v[c]);
         }
+      }
+      if (!piece.down) {
         meet_all();
-        const int blocks = Lay::blocks(p.ff);
+        const int blocks = (p.ff + 63) / 64;
+#pragma unroll 1
         for (int i = ew; i < cnt; i += 4) {
           const float* from = tile + tok[c0 + i] * TILE;
-          const float hs = FP8 ? p.hs[tok[c0 + i]] : 1.f;
-#pragma unroll
+#pragma unroll 1
           for (int b = 0; b < OUT / 64; ++b) {
             const int f0 = piece.tile * OUT + 64 * b;          // 64 numbers of u: two per lane
             float v[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float z = from[64 * b + 32 * j + lane] * hs;
-              v[j] = GLU ? z / (1.f + expf(-z)) * (from[64 + 32 * j + lane] * hs) : gelu_erf(z);
+              const float z = from[64 * b + 32 * j + lane];
+              v[j] = GLU ? z / (1.f + expf(-z)) * from[64 + 32 * j + lane] : gelu_erf(z);
             }
             if (FP8) {
               uint32_t m = 0u;
@@ -712,21 +679,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       } else {
         const int col = piece.tile * TILE + row;
         float* y = p.y + ((size_t)piece.split * entries + c0) * p.d + col;
-        if (FP8) {
-#pragma unroll
-          for (int c = 0; c < NB; ++c)
-            if (c < cnt && col < p.d) y[(size_t)c * p.d] = acc[FP8 ? c : 0];
-        } else if (ok) {
-#pragma unroll
-          for (int cc = 0; cc < NB; cc += 16)
-            if (cc < cols) {
-              uint32_t v[16];
-              tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
-              tc_wait_ld();
-#pragma unroll
-              for (int c = 0; c < 16; ++c)
-                if (cc + c < cnt && col < p.d) y[(size_t)(cc + c) * p.d] = __uint_as_float(v[c]);
-            }
+        if (col < p.d) {
+#pragma unroll 4
+          for (int c = 0; c < cnt; ++c) y[(size_t)c * p.d] = tile[c * TILE + row];
         }
         __threadfence();
         meet_all();
@@ -753,11 +708,11 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (p.add != nullptr && sub == 0)
         sum = scaled(four_bf16(p.add + (size_t)t * p.d + c4), p.gate != nullptr ? 1.f / (1.f + expf(-p.gate[t])) : 1.f);
 #pragma unroll 1
-      for (int i0 = sub; i0 < parts; i0 += 8 * share) {        // eight (choice, slice) results in flight
-        float4 x[8];
-        float w[8];
+      for (int i0 = sub; i0 < parts; i0 += 4 * share) {        // four (choice, slice) results in flight
+        float4 x[4];
+        float w[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           const int part = i0 + j * share, k = part * inverse >> 16, split = part - k * splits;
           w[j] = 0.f;
           x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -769,7 +724,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4; ++j)
           sum = make_float4(fmaf(w[j], x[j].x, sum.x), fmaf(w[j], x[j].y, sum.y), fmaf(w[j], x[j].z, sum.z), fmaf(w[j], x[j].w, sum.w));
       }
       if (share == 8) {
