@@ -46,11 +46,14 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
   const bool softmax_top = scores == ROUTE_SOFTMAX_TOP;
   if (scores == ROUTE_SOFTMAX) {
     float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
     for (int i = lane; i < E; i += 32) mx = fmaxf(mx, sc[i]);
     mx = warp_max(mx);
+#pragma unroll 1
     for (int i = lane; i < E; i += 32) sum += expf(sc[i] - mx);
     sum = warp_sum(sum);
     // without a correction the logits themselves choose (the softmax keeps their order)
+#pragma unroll 1
     for (int i = lane; i < E; i += 32) {
       sc[i] = expf(sc[i] - mx) / sum;
       if (corr != nullptr) ch[i] = sc[i] + load_as_f32(corr, corr_dtype, i);
@@ -59,8 +62,10 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
   }
   if (G > 1 && keep < G) {
     const int per = E / G;
+#pragma unroll 1
     for (int g = lane; g < G; g += 32) {          // group scores
       float a = -INFINITY, b = -INFINITY;         // the two largest
+#pragma unroll 1
       for (int j = 0; j < per; ++j) {
         const float v = ch[g * per + j];
         if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
@@ -74,6 +79,7 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
       if (lane == 0 && best != 0x7fffffff) hs[best] = NAN;      // NaN marks a kept group
       __syncwarp();
     }
+#pragma unroll 1
     for (int i = lane; i < E; i += 32)
       if (!isnan(hs[i / per])) ch[i] = -INFINITY;
     __syncwarp();
@@ -107,11 +113,13 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
     float v = s * scale;
     if (renormalise) {
       float sum = 0.f;
+#pragma unroll 1
       for (int k = 0; k < top; ++k) sum += __shfl_sync(0xffffffffu, s, k);
       v = s / (sum + 1e-20f) * scale;
     } else if (softmax_top) {                     // the weights: softmax over the chosen logits alone
       const float e = expf(s - warp_max(s));
       float sum = 0.f;
+#pragma unroll 1
       for (int k = 0; k < top; ++k) sum += __shfl_sync(0xffffffffu, e, k);
       v = e / sum * scale;
     }
@@ -120,13 +128,18 @@ __device__ __forceinline__ void choose_experts(float* sc, float* ch, float* hs, 
   }
   if (renormalise && lane == 0) {
     float sum = 0.f;
+#pragma unroll 1
     for (int k = 0; k < top; ++k) sum += sc[ids[k]];
+#pragma unroll 1
     for (int k = 0; k < top; ++k) w[k] = sc[ids[k]] / (sum + 1e-20f) * scale;
   }
   if (softmax_top && lane == 0) {
     float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
     for (int k = 0; k < top; ++k) mx = fmaxf(mx, sc[ids[k]]);
+#pragma unroll 1
     for (int k = 0; k < top; ++k) sum += expf(sc[ids[k]] - mx);
+#pragma unroll 1
     for (int k = 0; k < top; ++k) w[k] = expf(sc[ids[k]] - mx) / sum * scale;
   }
 }

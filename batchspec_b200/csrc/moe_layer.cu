@@ -55,6 +55,7 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
     if (row >= n) return;
     __shared__ uint32_t warp_max[ROUTE_WARPS];
     uint32_t m = 0u;
+#pragma unroll 1
     for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
       const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
       const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -68,6 +69,7 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
     for (int i = 0; i < ROUTE_WARPS; ++i) m = max(m, warp_max[i]);
     const int code = scale_code(m);
     const float inv = inverse_scale(code);
+#pragma unroll 1
     for (int k = 8 * threadIdx.x; k < d; k += 8 * 32 * ROUTE_WARPS) {
       const uint4 raw = *reinterpret_cast<const uint4*>(h + (size_t)row * d + k);
       const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -93,12 +95,14 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(first) : "r"(s32(part)), "r"(0));
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const bool token = t0 + g < n;
+#pragma unroll 1
   for (int unit = rank * ROUTE_WARPS + warp; unit < units; unit += ROUTE_CLUSTER * ROUTE_WARPS) {
     const int r0 = unit / slices * 16, s0 = unit % slices * per, s1 = min(steps, s0 + per);
     const __nv_bfloat16* lo = wr + (size_t)min(r0 + g, rows - 1) * d + 8 * q;
     const __nv_bfloat16* hi = wr + (size_t)min(r0 + g + 8, rows - 1) * d + 8 * q;
     const __nv_bfloat16* x = h + (size_t)min(t0 + g, n - 1) * d + 8 * q;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
     for (int s = s0; s < s1; s += 4) {
       uint4 a[4], b[4], c[4];
 #pragma unroll
@@ -123,6 +127,7 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   }
   float* bias = part + (size_t)units * 16 * ROUTE_TOKENS;      // [C]
   if (rank == 0)
+#pragma unroll 1
     for (int e = threadIdx.x; e < C; e += 32 * ROUTE_WARPS) bias[e] = corr != nullptr ? load_as_f32(corr, corr_dtype, e) : 0.f;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   __syncwarp();
@@ -131,10 +136,11 @@ moe_layer_route_kernel(const __nv_bfloat16* __restrict__ h, int n, int d, const 
   if (rank != 0 || t >= n) return;
   float* sc = bias + C + (size_t)warp * 3 * C;
   float* ch = sc + C;
+#pragma unroll 1
   for (int e = lane; e < rows; e += 32) {
     const float* from = part + ((size_t)(e / 16 * slices) * ROUTE_TOKENS + warp) * 16 + e % 16;
     float z = 0.f;
-#pragma unroll 8
+#pragma unroll 4
     for (int s = 0; s < slices; ++s) z += from[s * ROUTE_TOKENS * 16];
     if (e < C) route_score(rule, z, bias[e], sc + e, ch + e);
     else gate[t] = z;                                          // the row behind the experts' rows
@@ -183,6 +189,7 @@ __device__ __forceinline__ float block_scale(const float* p, int e8m0, size_t i)
 // Waits until *counter reaches `target` (a bounded wait, as every other one).
 __device__ __forceinline__ bool wait_for(const int* counter, int target, int* status, volatile int* abort_flag) {
   unsigned long long t_from = 0ull;
+#pragma unroll 1
   for (uint32_t i = 0;; ++i) {
     int v;
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
@@ -248,6 +255,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < MAX_STAGES; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
@@ -270,6 +278,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+#pragma unroll 1
   for (int e = threadIdx.x; e < p.E; e += LAYER_THREADS) count[e] = 0;
   tc_fence_before();
   __syncthreads();
@@ -282,6 +291,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   if (threadIdx.x == 0) first_piece = atomicAdd(p.counters, 1);
   // ---- the entries by expert, in an order that every CTA finds alike
   if (slots > 32) {
+#pragma unroll 1
     for (int s = threadIdx.x; s < slots; s += LAYER_THREADS) {
       const int e = p.ids[s];
       if (e < p.E) atomicAdd(count + e, 1);
@@ -368,6 +378,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   {
     const int whole = A * down_tiles, G = gridDim.x;
     int best = (whole + G - 1) / G;                            // rounds, each of 1 / splits
+#pragma unroll 1
     for (int s = 2; s <= MAX_SPLITS && down_stages >= 4 * s; ++s) {
       const int rounds = (whole * s + G - 1) / G;
       if (rounds * splits * 7 <= best * s * 6) { best = rounds; splits = s; }
@@ -383,7 +394,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     bool ok = true;
     auto push = [&](const Piece& piece) {
       const int q = np % QUEUE;
-      if (ok) ok = warp_wait(q_empty + q, ((uint32_t)(np / QUEUE) & 1u) ^ 1u, abort_flag, p.status, 113);
+      if (ok) ok = warp_wait_short(q_empty + q, ((uint32_t)(np / QUEUE) & 1u) ^ 1u, abort_flag, p.status, 113);
       if (lane == 0 && ok) {
         queue[q] = piece;
         mbar_arrive(q_full + q);
@@ -398,7 +409,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     };
     // stage s of a piece: the weights' two halves, and its tokens; the first copies also say how many bytes will come
     auto weights = [&](const CUtensorMap* map, int y0, int y1, int boxes, int s) {
-      if (ok) ok = warp_wait(empty + st, phase ^ 1u, abort_flag, p.status, 114);
+      if (ok) ok = warp_wait_short(empty + st, phase ^ 1u, abort_flag, p.status, 114);
       if (!ok) return;
       unsigned char* at = smem + (size_t)st * Lay::STAGE;
       mbar_expect_tx_by(one, full + st, A_BYTES + (uint32_t)boxes * 2048u * (FP8 ? 2u : 1u));
@@ -408,7 +419,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     auto tokens = [&](const CUtensorMap* map, int y, int mid, int boxes, int s) {
       if (!ok) return;
       unsigned char* at = smem + (size_t)st * Lay::STAGE + A_BYTES;
-      for (int b = 0; b < boxes; ++b) {
+#pragma unroll
+      for (int b = 0; b < NB / 16; ++b) {
+        if (b >= boxes) break;
         tma_load_2d_by(one, at + b * 2048, map, full + st, s * STAGE_K, y + 16 * b);
         if (FP8) tma_load_2d_by(one, at + (boxes + b) * 2048, map, full + st, s * STAGE_K, mid + y + 16 * b);
       }
@@ -422,6 +435,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int a = t / up_tiles, i0 = (t - a * up_tiles) * OUT, e = active[a];
       push({0, a, t - a * up_tiles, 0, up_stages, 0});
       const int y0 = e * ffu + i0, y1 = y0 + (GLU ? p.ff : 64);
+#pragma unroll 1
       for (int s = 0; s < up_stages && ok; ++s, step()) {
         weights(&map_up, y0, y1, NB / 16, s);
         tokens(&map_h, 0, p.n, NB / 16, s);
@@ -442,6 +456,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         waited = true;
         const int ahead = min(s1 - s0, p.stages), st_from = st;
         const uint32_t phase_from = phase;
+#pragma unroll 1
         for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, boxes, s0 + i);
         if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
         if (lane == 0 && ok) mbar_arrive(&up_done);            // the epilogue may read the scales of u
@@ -450,9 +465,11 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         fence_async_all();                                     // u was written through the generic proxy
         st = st_from;
         phase = phase_from;
+#pragma unroll 1
         for (int i = 0; i < ahead; ++i, step()) tokens(&map_u, c0, slots, boxes, s0 + i);
         s = s0 + ahead;
       }
+#pragma unroll 1
       for (; s < s1 && ok; ++s, step()) {
         weights(&map_down, y0, y0 + 64, boxes, s);
         tokens(&map_u, c0, slots, boxes, s);
@@ -468,9 +485,10 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     uint32_t phase = 0u, ring_phase[2] = {0u, 0u};
     bool ok = true;
     const uint64_t desc0 = smem_desc(smem);
+#pragma unroll 1
     for (int np = 0; ok; ++np) {
       const int q = np % QUEUE;
-      if (!(ok = warp_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 115))) break;
+      if (!(ok = warp_wait_short(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 115))) break;
       const Piece piece = queue[q];
       __syncwarp();
       if (lane == 0) mbar_arrive(q_empty + q);
@@ -482,7 +500,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       int slot = group ? SLOTS + ring[1] : ring[0];
       uint32_t slot_phase = group ? ring_phase[1] : ring_phase[0];
       auto next_slot = [&]() {
-        ok = ok && warp_wait(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
+        ok = ok && warp_wait_short(acc_empty + slot, slot_phase ^ 1u, abort_flag, p.status, 116);
         tc_fence_after();
       };
       auto commit_slot = [&]() {
@@ -490,8 +508,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         if (++slot == SLOTS * (group + 1)) { slot = SLOTS * group; slot_phase ^= 1u; }
       };
       if (!FP8) next_slot();
+#pragma unroll 1
       for (int s = piece.s0; s < piece.s1 && ok; ++s) {
-        if (!(ok = warp_wait(full + st, phase, abort_flag, p.status, 117))) break;
+        if (!(ok = warp_wait_short(full + st, phase, abort_flag, p.status, 117))) break;
         tc_fence_after();
         const uint64_t wd = desc0 + (uint64_t)(st * (Lay::STAGE / 16)), xd = wd + A_BYTES / 16;      // addresses count 16 bytes
         if (FP8) {
@@ -538,12 +557,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     // the threads of a group meet (a bounded wait, so that none is left behind when another one gives up)
     auto meet_all = [&]() {
       arrive(meet + group);
-      ok = ok && mbar_wait(meet + group, meet_phase, abort_flag, p.status, 118);
+      ok = ok && mbar_wait_short(meet + group, meet_phase, abort_flag, p.status, 118);
       meet_phase ^= 1u;
     };
+#pragma unroll 1
     for (int np = 0; ok; ++np) {
       const int q = np % QUEUE;
-      if (!(ok = mbar_wait(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
+      if (!(ok = mbar_wait_short(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
       const Piece piece = queue[q];
       arrive(q_empty + q);
       if (piece.down < 0) break;
@@ -563,12 +583,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const float* ws = piece.down ? p.sd : p.su;
         const int steps = (piece.s1 - piece.s0) << piece.down;          // accumulators: a stage has one, in the down products two
         // the columns' scales (asked for with the first weights' scales, while the first copies are on their way)
-        if (piece.down && !up_known) ok = mbar_wait(&up_done, 0u, abort_flag, p.status, 120);
+        if (piece.down && !up_known) ok = mbar_wait_short(&up_done, 0u, abort_flag, p.status, 120);
         up_known = piece.down;
         meet_all();                                            // nobody reads the last piece's any more
         {
           const int blocks = (p.ff + 63) / 64, rows = piece.down ? Lay::blocks(p.ff) : 1, some = piece.down ? cnt : p.n;
           const float* from = piece.down ? p.us + (size_t)c0 * blocks : p.hs;
+#pragma unroll 2
           for (int i = et; i < rows * cols; i += 128) {
             const int c = i / rows, b = i - c * rows;          // neighbours read neighbouring blocks of an entry
             ys[b * NB + c] = c < some && b < blocks ? __ldcg(from + (piece.down ? c * blocks + b : c)) : 0.f;
@@ -587,7 +608,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           __syncwarp();
           const float w_a = __shfl_sync(0xffffffffu, wa, s & 31), w_b = __shfl_sync(0xffffffffu, wb, s & 31);
           const float w = w_block == block_a ? w_a : w_b;
-          if (ok) ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+          if (ok) ok = mbar_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
           tc_fence_after();
 #pragma unroll
@@ -612,7 +633,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           f += piece.down ? NB : 0;
         }
       } else {
-        ok = mbar_wait(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+        ok = mbar_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
         tc_fence_after();
       }
       // to shared memory, from where a few instructions per entry take them on: what is executed once per piece costs the fetch of its
@@ -702,6 +723,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     const int quads = p.d / 4, parts = p.top * splits, threads = (int)gridDim.x * 256, share = p.n * quads * 8 <= threads ? 8 : 1;
     const int inverse = (65536 + splits - 1) / splits;         // i / splits = i * inverse >> 16 for the few there are
     const int sub = (threadIdx.x - 64) % share;
+#pragma unroll 1
     for (int i = ((int)blockIdx.x * 256 + (int)threadIdx.x - 64) / share; ok && i < p.n * quads; i += threads / share) {
       const int t = i / quads, c4 = 4 * (i - t * quads);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);

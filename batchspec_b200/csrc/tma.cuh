@@ -53,6 +53,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   auto done = [&]() { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
   if (done()) return true;
   uint64_t t0 = 0;
+#pragma unroll 1
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
     if (done()) return true;
     if (*abort_flag) return false;
@@ -95,9 +96,20 @@ __device__ __forceinline__ void mbar_expect_tx_by(uint32_t one, uint64_t* bar, u
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
                ::"r"(s32(bar)), "r"(bytes), "r"(one) : "memory");
 }
-// mbar_wait by a whole warp, which learns one answer
+// mbar_wait whose polls are a call: for kernels with many waits in code that is executed a few times only, where the fetch of what lies between
+// costs more than the call
+static __device__ __noinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_wait(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_try_wait(bar, parity) || mbar_poll(bar, parity, abort_flag, status, code);
+}
+// by a whole warp, which learns one answer
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+__device__ __forceinline__ bool warp_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_short(bar, parity, abort_flag, status, code));
 }
 
 // Ask for a tile to be brought into the L2 (no shared-memory destination, no completion to wait for).
