@@ -223,17 +223,16 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         acc[c + 3] = fmaf(__uint_as_float(v[c + 3]), g.w, acc[c + 3]);
       }
     }
+    // every product of this slice has completed and every stage has been read: the sums take their place, where few instructions, the same for
+    // each token, find them (what is executed once costs the fetch of its code more than its work)
     const int row = (int)quad * 32 + lane, n = tile_n * TILE_ROWS + row;
-    if (p.splits == 1) {
-      if (ok && n < p.N) {
 #pragma unroll
-        for (int c = 0; c < BN; ++c)
-          if (tok0 + c < p.M) put(p.C, p.out_f32, (size_t)(tok0 + c) * p.N + n, acc[c]);
-      }
-    } else {
-      // every product of this slice has completed and every stage has been read: the sums take their place
-#pragma unroll
-      for (int c = 0; c < BN; ++c) part[c * TILE_ROWS + row] = acc[c];
+    for (int c = 0; c < BN; ++c) part[c * TILE_ROWS + row] = acc[c];
+    if (p.splits == 1 && ok && n < p.N) {
+      const int some = min(BN, p.M - tok0);
+      size_t at = (size_t)tok0 * p.N + n;
+#pragma unroll 4
+      for (int c = 0; c < some; ++c, at += p.N) put(p.C, p.out_f32, at, part[c * TILE_ROWS + row]);
     }
   }
   if (p.splits > 1) {
