@@ -12,12 +12,14 @@
 //                 may be cut into `splits` slices run by the CTAs of one cluster, whose partial tiles are joined in slice order through
 //                 distributed shared memory.
 //   many tokens   tokens on the rows, 128 rows of W on the columns: one persistent CTA per SM; eight epilogue warps hold the 128 x 128 sums.
-//                 The way back from tensor memory bounds it: 512 bytes a clock are asked for by 128 x 128 numbers per 128 k.
+//                 What bounds it is that way back: without the additions the product of 1,537 rows below takes 103 to 108 us, with them 119; its products
+//                 alone would take 55.  Tiles 192 wide, two CTAs per SM and other splits of the columns came no nearer.
 //   pairs         many tokens where both scales are powers of two: the tensor cores multiply by the scales and keep the sums of a whole
 //                 row, two CTAs share a tile (below).
 //
-// Measured on B200: 8 x 28,672 x 4,096 in 20 us (5.8 TB/s), 1,537 x 4,096 x 14,336 with float32 scales in 120 us (1.5 PFLOP/s), 2,048 x 28,672 x
-// 4,096 with e8m0 scales in 182 us (2.65 PFLOP/s; all zeros, which the power limit does not slow down, run at 4.1).
+// Measured on B200: 8 x 28,672 x 4,096 in 20.5 us (5.7 TB/s), 61 x 32,000 x 2,048 into float32 in 18.7 us (3.9 TB/s), 1,537 x 4,096 x 14,336 with
+// float32 scales in 119 us (1.5 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 174 to 178 us (2.7 PFLOP/s; 190 once the power limit holds;
+// all zeros, which it does not slow down, run at 4.1).
 #include "e4m3.cuh"
 #include "umma.cuh"
 
@@ -700,7 +702,8 @@ Form choose(int M, int N, int K, bool powers, int sms) {
   const double few = 5.5 + rounds(few_tiles * splits, 2 * sms) * ((nkb + splits - 1) / splits) * (bn == 16 ? 0.45 : (bn == 32 ? 0.6 : 0.87));
   const double many = 6 + rounds(((long long)M + 127) / 128 * (((long long)N + MANY_BN - 1) / MANY_BN), sms) * (0.35 * nkb + 2);
   const double pair = 7 + rounds(((long long)M + 255) / 256 * (((long long)N + PAIR_BN - 1) / PAIR_BN), sms / 2) * (0.27 * nkb + 4);
-  if (few <= many && (!powers || few <= pair)) return FEW;
+  const bool fits = ((long long)M + bn - 1) / bn <= 65535;      // a grid's second dimension
+  if (fits && few <= many && (!powers || few <= pair)) return FEW;
   return powers && pair < many ? PAIR : MANY;
 }
 
@@ -729,7 +732,6 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, Fp8Params p, 
     if (e != cudaSuccess) return (int)e;
     set = smem;
   }
-  if (tiles_t > 65535) return (int)cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles_n, tiles_t, p.splits);
   cfg.blockDim = dim3(FEW_THREADS);

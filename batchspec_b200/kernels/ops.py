@@ -1525,6 +1525,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
             raise KernelError("quantize_fp8: a tensor of more than two dimensions has to be contiguous")
         batch, ldx = shape[:-2].numel(), K
         q, scale = x.new_empty(shape[:-1] + (pitch,), dtype=torch.float8_e4m3fn), x.new_empty(shape[:-2] + (RB, KB), dtype=torch.float8_e8m0fnu)
+    if block_rows > 1 and RB > 65535:
+        raise KernelError(f"quantize_fp8: blocks of 128 rows of a matrix of {R} rows are not supported (65,535 blocks at most)")
     if batch and R:
         _check(load_library(features=("fp8",)).bspec_quantize_fp8(
             x.data_ptr(), _dtype_code(x.dtype), ldx, R * ldx, q.data_ptr(), pitch, scale.data_ptr(), batch, R, K, block_rows, stream),

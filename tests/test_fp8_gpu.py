@@ -173,6 +173,20 @@ def test_product_of_many_tiles(ops, M, N, K, scales):
     ops.check_status()
 
 
+def test_millions_of_rows_by_a_narrow_matrix(ops):
+    """More tiles of tokens than a grid's second dimension takes."""
+    M = 65536 * 64 + 70
+    x = torch.zeros(M, 32, device=DEV, dtype=torch.bfloat16)
+    x[-5:] = torch.randn(5, 32, device=DEV, generator=generator(5)).to(torch.bfloat16)
+    w, ws = ops.quantize_fp8(torch.randn(16, 32, device=DEV, generator=generator(6)), 128)
+    q, s = ops.quantize_fp8(x)
+    for scales in (s, s.float()):
+        out = ops.linear_fp8(q, scales, w, ws)
+        check_product(out[-70:], q[-70:], scales[-70:], w, ws)
+        assert not bool(out[:-70].any())
+    ops.check_status()
+
+
 def test_offsets_beyond_32_bits(ops):
     """Matrices of more than 2^31 numbers: the last rows of a quantised one, of the weights and of a result."""
     g = generator(41)
