@@ -291,6 +291,22 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  // Where a step chooses so often that nearly every expert is taken (of evenly chosen ones 1 in 20 is not), and weights enough follow, the first pieces'
+  // weights are asked into the L2 while the router runs.  Measured: 61 tokens of 64 experts, 4.8 rounds of pieces, 137.2 -> 133.8 us; with 1.6
+  // rounds, 23 tokens of 20 small experts, 35.1 -> 36.1.
+  const int tiles = (p.ff + OUT - 1) / OUT;
+  if (warp == 0 && slots >= 3 * p.E && p.E * tiles >= 3 * (int)gridDim.x) {
+    const uint32_t one = elect_one();
+    const int e = (int)blockIdx.x / tiles, i0 = ((int)blockIdx.x - e * tiles) * OUT;
+    if (e < p.E && one) {
+      const int y0 = e * (GLU ? 2 * p.ff : p.ff) + i0, y1 = y0 + (GLU ? p.ff : 64), stages = (p.d + STAGE_K - 1) / STAGE_K;
+#pragma unroll 1
+      for (int s = 0; s < stages; ++s) {
+        tma_prefetch_2d(&map_up, s * STAGE_K, y0);
+        tma_prefetch_2d(&map_up, s * STAGE_K, y1);
+      }
+    }
+  }
   bspec::pdl_prologue(85);
 
   // this CTA's first up piece, drawn while the lists are made
