@@ -161,7 +161,19 @@ constexpr int TILE = 128;                    // weight rows of a piece
 constexpr int A_BYTES = TILE * 128;          // of a stage: 128 bytes of every row
 constexpr int QUEUE = 4;                     // pieces on their way through the roles
 constexpr int MAX_STAGES = 10;
-constexpr int MAX_SPLITS = 4;                // slices of k of the down products
+constexpr int MAX_SPLITS = 4;                // slices of k of the down products: 1, 2 or 4
+
+// Division by a number that the host knows: the product with its reciprocal is at most one too small.
+struct Divide {
+  uint32_t by, inverse;
+  __host__ __device__ static Divide of(int n) { return {(uint32_t)n, 0xffffffffu / (uint32_t)n}; }
+  __device__ __forceinline__ int operator()(int n, int& rest) const {
+    uint32_t q = __umulhi((uint32_t)n, inverse), left = (uint32_t)n - q * by;
+    if (left >= by) { ++q; left -= by; }
+    rest = (int)left;
+    return (int)q;
+  }
+};
 
 struct LayerParams {
   const float* su;                           // scales of 128 x 128 blocks: float32, or 8-bit exponents (e8m0)
@@ -181,6 +193,7 @@ struct LayerParams {
   int* status;
   int n, d, ff, E, top;
   int stages;
+  Divide up_tiles, down_tiles, quads;         // tiles of an expert's products, groups of four numbers of a token
 };
 
 struct Piece {
@@ -294,12 +307,12 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   // Where a step chooses so often that nearly every expert is taken (of evenly chosen ones 1 in 20 is not), and weights enough follow, the first pieces'
   // weights are asked into the L2 while the router runs.  Measured: 61 tokens of 64 experts, 4.8 rounds of pieces, 137.2 -> 133.8 us; with 1.6
   // rounds, 23 tokens of 20 small experts, 35.1 -> 36.1.
-  const int tiles = (p.ff + OUT - 1) / OUT;
-  if (warp == 0 && slots >= 3 * p.E && p.E * tiles >= 3 * (int)gridDim.x) {
+  if (warp == 0 && slots >= 3 * p.E && p.E * (int)p.up_tiles.by >= 3 * (int)gridDim.x) {
     const uint32_t one = elect_one();
-    const int e = (int)blockIdx.x / tiles, i0 = ((int)blockIdx.x - e * tiles) * OUT;
+    int i0;
+    const int e = p.up_tiles((int)blockIdx.x, i0);
     if (e < p.E && one) {
-      const int y0 = e * (GLU ? 2 * p.ff : p.ff) + i0, y1 = y0 + (GLU ? p.ff : 64), stages = (p.d + STAGE_K - 1) / STAGE_K;
+      const int y0 = e * (GLU ? 2 * p.ff : p.ff) + i0 * OUT, y1 = y0 + (GLU ? p.ff : 64), stages = (p.d + STAGE_K - 1) / STAGE_K;
 #pragma unroll 1
       for (int s = 0; s < stages; ++s) {
         tma_prefetch_2d(&map_up, s * STAGE_K, y0);
@@ -394,20 +407,19 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   __syncthreads();
 
   const int A = n_active, ffu = GLU ? 2 * p.ff : p.ff;
-  const int up_tiles = (p.ff + OUT - 1) / OUT, up_pieces = A * up_tiles, up_stages = (p.d + STAGE_K - 1) / STAGE_K;
-  const int down_tiles = (p.d + TILE - 1) / TILE, down_stages = (p.ff + STAGE_K - 1) / STAGE_K;
+  const int up_pieces = A * (int)p.up_tiles.by, up_stages = (p.d + STAGE_K - 1) / STAGE_K;
+  const int down_tiles = (int)p.down_tiles.by, down_stages = (p.ff + STAGE_K - 1) / STAGE_K;
   // slices of the down products' k, four stages each at least: more of them only where that fills the CTAs' rounds by a seventh better
-  int splits = 1;
+  int shift = 0;
   {
-    const int whole = A * down_tiles, G = gridDim.x;
-    int best = (whole + G - 1) / G;                            // rounds, each of 1 / splits
-#pragma unroll 1
-    for (int s = 2; s <= MAX_SPLITS && down_stages >= 4 * s; ++s) {
-      const int rounds = (whole * s + G - 1) / G;
-      if (rounds * splits * 7 <= best * s * 6) { best = rounds; splits = s; }
+    const float whole = (float)(A * down_tiles) / (float)gridDim.x;
+    float best = ceilf(whole);                                 // rounds of whole pieces
+    for (int i = 1; (1 << i) <= MAX_SPLITS && down_stages >= (4 << i); ++i) {
+      const float rounds = ceilf(whole * (1 << i)) / (1 << i);
+      if (rounds * 7.f <= best * 6.f) { best = rounds; shift = i; }
     }
   }
-  const int down_per = (down_stages + splits - 1) / splits, down_pieces = A * down_tiles * splits;
+  const int splits = 1 << shift, down_per = (down_stages + splits - 1) >> shift, down_pieces = (A * down_tiles) << shift;
   const int entries = first[A];
 
   if (warp == 0) {
@@ -455,8 +467,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     // the up products
     int t = __shfl_sync(0xffffffffu, first_piece, 0);
     while (ok && t < up_pieces) {
-      const int a = t / up_tiles, i0 = (t - a * up_tiles) * OUT, e = active[a];
-      push({0, a, t - a * up_tiles, 0, up_stages, 0});
+      int tile_at;
+      const int a = p.up_tiles(t, tile_at), i0 = tile_at * OUT, e = active[a];
+      push({0, a, tile_at, 0, up_stages, 0});
       const int y0 = e * ffu + i0, y1 = y0 + (GLU ? p.ff : 64);
 #pragma unroll 1
       for (int s = 0; s < up_stages && ok; ++s, step()) {
@@ -469,7 +482,8 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     t = draw(2);
     bool waited = false;
     while (ok && t < down_pieces) {
-      const int split = t % splits, a = t / splits % A, dt = t / splits / A, e = active[a];
+      int dt;
+      const int split = t & (splits - 1), a = p.down_tiles(t >> shift, dt), e = active[a];
       const int s0 = split * down_per, s1 = min(down_stages, s0 + down_per), c0 = first[a];
       push({1, a, dt, s0, s1, split});
       const int y0 = e * p.d + dt * TILE, boxes = (first[a + 1] - c0 + 15) / 16;
@@ -743,12 +757,12 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     meet_all();
     ok = __all_sync(0xffffffffu, ok);
     // few of them: eight lanes share a thread's results
-    const int quads = p.d / 4, parts = p.top * splits, threads = (int)gridDim.x * 256, share = p.n * quads * 8 <= threads ? 8 : 1;
-    const int inverse = (65536 + splits - 1) / splits;         // i / splits = i * inverse >> 16 for the few there are
+    const int quads = (int)p.quads.by, parts = p.top * splits, threads = (int)gridDim.x * 256, share = p.n * quads * 8 <= threads ? 8 : 1;
     const int sub = (threadIdx.x - 64) % share;
 #pragma unroll 1
     for (int i = ((int)blockIdx.x * 256 + (int)threadIdx.x - 64) / share; ok && i < p.n * quads; i += threads / share) {
-      const int t = i / quads, c4 = 4 * (i - t * quads);
+      int rest;
+      const int t = p.quads(i, rest), c4 = 4 * rest;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (p.add != nullptr && sub == 0)
         sum = scaled(four_bf16(p.add + (size_t)t * p.d + c4), p.gate != nullptr ? 1.f / (1.f + expf(-p.gate[t])) : 1.f);
@@ -758,7 +772,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int part = i0 + j * share, k = part * inverse >> 16, split = part - k * splits;
+          const int part = i0 + j * share, k = part >> shift, split = part & (splits - 1);
           w[j] = 0.f;
           x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (part < parts) {
@@ -813,6 +827,9 @@ int launch_experts(const CUtensorMap* maps, LayerParams p, cudaStream_t stream) 
   if (fixed + 3 * (size_t)Lay::STAGE > SMEM_BUDGET) return (int)cudaErrorInvalidValue;
   const size_t room = (SMEM_BUDGET - fixed) / Lay::STAGE;
   p.stages = room > MAX_STAGES ? MAX_STAGES : (int)room;
+  p.up_tiles = Divide::of((p.ff + (GLU ? 63 : 127)) / (GLU ? 64 : 128));
+  p.down_tiles = Divide::of((p.d + TILE - 1) / TILE);
+  p.quads = Divide::of(p.d / 4);
   static bool set_dev[bspec::kMaxDevices] = {};
   bool& set = set_dev[bspec::current_device()];
   if (!set) {
