@@ -12,13 +12,14 @@
 //                 may be cut into `splits` slices run by the CTAs of one cluster, whose partial tiles are joined in slice order through
 //                 distributed shared memory.
 //   many tokens   tokens on the rows, 128 rows of W on the columns: one persistent CTA per SM; eight epilogue warps hold the 128 x 128 sums.
-//                 What bounds it is that way back: without the additions the product of 1,537 rows below takes 103 to 108 us, with them 119; its products
-//                 alone would take 55.  Tiles 192 wide, two CTAs per SM and other splits of the columns came no nearer.
+//                 What bounds it: a tile asks for 32 KB per 128 k, 512 of the clocks that the L2 (64 bytes a clock) and shared memory have; the
+//                 additions are a tenth of the time.  Tiles 192 wide, two CTAs per SM, and pairs of CTAs with rows of W on the accumulator's rows
+//                 (whose columns' scales have to be read for every block: 184 us for 118) came no nearer.
 //   pairs         many tokens where both scales are powers of two: the tensor cores multiply by the scales and keep the sums of a whole
 //                 row, two CTAs share a tile (below).
 //
 // Measured on B200: 8 x 28,672 x 4,096 in 20.5 us (5.7 TB/s), 61 x 32,000 x 2,048 into float32 in 18.7 us (3.9 TB/s), 1,537 x 4,096 x 14,336 with
-// float32 scales in 119 us (1.5 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 174 to 178 us (2.7 PFLOP/s; 190 once the power limit holds;
+// float32 scales in 118 us (1.5 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 174 us (2.75 PFLOP/s; 190 and more once the power limit holds;
 // all zeros, which it does not slow down, run at 4.1).
 #include "e4m3.cuh"
 #include "umma.cuh"

@@ -26,8 +26,9 @@
 // With few tokens what bounds a step are the phases that wait for each other: router 7 to 8 us, start and lists 3, first weights 4, then the
 // weights, then u through the L2 4, the last pieces and the sum over choices 3.  A good part of each is the fetch of its code, which the
 // weights have pushed out of the L2 since the last step: loops are kept as loops, and the polls of a wait are a call (1 token 38.4 -> 35.9 us,
-// 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code).
-// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 36 us; 8 tokens, gated, 8-bit, 53; 61 tokens, GELU, 139 (5.3 TB/s);
+// 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code),
+// and pieces are numbered without divisions by numbers of the step (61 tokens 133.8 -> 130.5).
+// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 53; 61 tokens, GELU, 130.5 (5.6 TB/s);
 // 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.
 #include "moe_choose.cuh"
 #include "e4m3.cuh"
