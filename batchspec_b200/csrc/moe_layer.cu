@@ -28,7 +28,7 @@
 // weights have pushed out of the L2 since the last step: loops are kept as loops, and the polls of a wait are a call (1 token 38.4 -> 35.9 us,
 // 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code),
 // and pieces are numbered without divisions by numbers of the step (61 tokens 133.8 -> 130.5).
-// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 53; 61 tokens, GELU, 130.5 (5.6 TB/s);
+// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 54; 61 tokens, GELU, 131 (5.6 TB/s);
 // 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.
 #include "moe_choose.cuh"
 #include "e4m3.cuh"
@@ -162,6 +162,7 @@ constexpr int TILE = 128;                    // weight rows of a piece
 constexpr int A_BYTES = TILE * 128;          // of a stage: 128 bytes of every row
 constexpr int QUEUE = 4;                     // pieces on their way through the roles
 constexpr int MAX_STAGES = 10;
+constexpr int WINDOW = 64;                   // blocks of u whose scales wait in shared memory at a time
 constexpr int MAX_SPLITS = 4;                // slices of k of the down products: 1, 2 or 4
 
 // Division by a number that the host knows: the product with its reciprocal is at most one too small.
@@ -238,10 +239,18 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) { return make
 template <bool FP8, int NB>
 struct Layout {
   static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
-  __host__ __device__ static int blocks(int k) { return (k + 127) / 128 * 2; }             // of 64, in whole stages
-  // of each epilogue group: tile [NB][128], scales of a piece's u [ff / 64][NB]; then the lists
+  // rows of scales: blocks of 64 in whole stages, a window of them at most
+  __host__ __device__ static int rows(int ff) { return (ff + 127) / 128 * 2 < WINDOW ? (ff + 127) / 128 * 2 : WINDOW; }
+  // of each epilogue group: tile [NB][128], scales of a piece's u [rows][NB]; then the lists
   __host__ __device__ static size_t fixed(int ff, int slots, int E) {
-    return (size_t)2 * NB * TILE * 4 + (FP8 ? (size_t)2 * blocks(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
+    return (size_t)2 * NB * TILE * 4 + (FP8 ? (size_t)2 * rows(ff) * NB * 4 : 0) + ((size_t)2 * slots + 3 * (size_t)E + 1) * 4 + 1024;
+  }
+  // stages that fit beside them, three at least or none
+  static int stages(int ff, int slots, int E) {
+    const size_t taken = 1024 + fixed(ff, slots, E);
+    if (taken + 3 * (size_t)STAGE > SMEM_BUDGET) return 0;
+    const size_t room = (SMEM_BUDGET - taken) / STAGE;
+    return room > MAX_STAGES ? MAX_STAGES : (int)room;
   }
 };
 
@@ -265,7 +274,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   const int slots = p.n * p.top, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* tile = reinterpret_cast<float*>(smem + (size_t)p.stages * Lay::STAGE);          // [2][NB][128]
   float* ys = tile + 2 * NB * TILE;
-  int* pos = reinterpret_cast<int*>(ys + (FP8 ? 2 * Lay::blocks(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
+  int* pos = reinterpret_cast<int*>(ys + (FP8 ? 2 * Lay::rows(p.ff) * NB : 0));            // [slots] where a (token, choice) lies by expert, or -1
   int* tok = pos + slots;                                                                // [slots] tokens by expert
   int* active = tok + slots;                                                             // [E] chosen experts
   int* first = active + p.E;                                                             // [E + 1] where their entries begin
@@ -580,7 +589,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
   } else {
     const int group = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, ew = (warp - 2) & 3;
     tile += group * NB * TILE;
-    ys += FP8 ? group * Lay::blocks(p.ff) * NB : 0;
+    ys += FP8 ? group * Lay::rows(p.ff) * NB : 0;
     const uint32_t quad = warp & 3;
     const int row = (int)quad * 32 + lane;
     const uint32_t lane_base = tmem_base + ((quad * 32u) << 16);
@@ -620,21 +629,23 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const size_t ws_at = (size_t)e * ((rows_all + 127) / 128);
         const float* ws = piece.down ? p.sd : p.su;
         const int steps = (piece.s1 - piece.s0) << piece.down;          // accumulators: a stage has one, in the down products two
-        // the columns' scales (asked for with the first weights' scales, while the first copies are on their way)
-        if (piece.down && !up_known) ok = mbar_wait_short(&up_done, 0u, abort_flag, p.status, 120);
-        up_known = piece.down;
-        meet_all();                                            // nobody reads the last piece's any more
-        {
-          const int blocks = (p.ff + 63) / 64, rows = piece.down ? Lay::blocks(p.ff) : 1, some = piece.down ? cnt : p.n;
-          const float* from = piece.down ? p.us + (size_t)c0 * blocks : p.hs;
+        const float* f = ys;
+        // the columns' scales: of the tokens, or of a window of this expert's u (whose first copies are on their way)
+        auto column_scales = [&](int i) {
+          if (piece.down && !up_known) ok = mbar_wait_short(&up_done, 0u, abort_flag, p.status, 120);
+          up_known = piece.down;
+          meet_all();                                        // nobody reads the last ones any more
+          const int blocks = (p.ff + 63) / 64, b0 = 2 * piece.s0 + i, rows = piece.down ? min(steps - i, WINDOW) : 1, some = piece.down ? cnt : p.n;
+          const float* scales = piece.down ? p.us + (size_t)c0 * blocks + b0 : p.hs;
 #pragma unroll 2
-          for (int i = et; i < rows * cols; i += 128) {
-            const int c = i / rows, b = i - c * rows;          // neighbours read neighbouring blocks of an entry
-            ys[b * NB + c] = c < some && b < blocks ? __ldcg(from + (piece.down ? c * blocks + b : c)) : 0.f;
+          for (int j = et; j < rows * cols; j += 128) {
+            const int c = j / rows, b = j - c * rows;        // neighbours read neighbouring blocks of an entry
+            ys[b * NB + c] = c < some && (!piece.down || b0 + b < blocks) ? __ldcg(scales + (piece.down ? c * blocks + b : c)) : 0.f;
           }
-        }
-        meet_all();
-        const float* f = ys + (piece.down ? 2 * piece.s0 * NB : 0);
+          meet_all();
+          f = ys;
+        };
+        column_scales(0);
         float wa = 0.f, wb = 0.f;
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
@@ -643,6 +654,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
             wa = block_scale(ws, p.e8m0, (ws_at + block_a) * KB + piece.s0 + s + lane);
             wb = block_scale(ws, p.e8m0, (ws_at + block_b) * KB + piece.s0 + s + lane);
           }
+          if (piece.down && i > 0 && i % WINDOW == 0) column_scales(i);
           __syncwarp();
           const float w_a = __shfl_sync(0xffffffffu, wa, s & 31), w_b = __shfl_sync(0xffffffffu, wb, s & 31);
           const float w = w_block == block_a ? w_a : w_b;
@@ -824,10 +836,8 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, int K, int byt
 template <bool FP8, bool GLU, int NB>
 int launch_experts(const CUtensorMap* maps, LayerParams p, cudaStream_t stream) {
   using Lay = Layout<FP8, NB>;
-  const size_t fixed = 1024 + Lay::fixed(p.ff, p.n * p.top, p.E);
-  if (fixed + 3 * (size_t)Lay::STAGE > SMEM_BUDGET) return (int)cudaErrorInvalidValue;
-  const size_t room = (SMEM_BUDGET - fixed) / Lay::STAGE;
-  p.stages = room > MAX_STAGES ? MAX_STAGES : (int)room;
+  p.stages = Lay::stages(p.ff, p.n * p.top, p.E);
+  if (p.stages == 0) return (int)cudaErrorInvalidValue;
   p.up_tiles = Divide::of((p.ff + (GLU ? 63 : 127)) / (GLU ? 64 : 128));
   p.down_tiles = Divide::of((p.d + TILE - 1) / TILE);
   p.quads = Divide::of(p.d / 4);
@@ -838,7 +848,8 @@ int launch_experts(const CUtensorMap* maps, LayerParams p, cudaStream_t stream) 
     if (e != cudaSuccess) return (int)e;
     set = true;
   }
-  BSPEC_LAUNCH((moe_layer_experts_kernel<FP8, GLU, NB>), bspec::sm_count(), LAYER_THREADS, fixed + (size_t)p.stages * Lay::STAGE, stream,
+  BSPEC_LAUNCH((moe_layer_experts_kernel<FP8, GLU, NB>), bspec::sm_count(), LAYER_THREADS,
+               1024 + Lay::fixed(p.ff, p.n * p.top, p.E) + (size_t)p.stages * Lay::STAGE, stream,
                maps[0], maps[1], maps[2], maps[3], p);
   return BSPEC_LAUNCH_CHECK();
 }
@@ -862,10 +873,13 @@ long long places(int n, int d, int ff, int top, bool fp8, long long (&at)[AT_PAR
 }
 }  // namespace
 
-// Bytes of scratch of a call.
-BSPEC_API long long bspec_moe_layer_scratch(int n, int d, int ff, int top, int fp8) {
+// Bytes of scratch of a call; 0 where its lists do not fit into shared memory (hundreds of choices for tens of tokens).
+BSPEC_API long long bspec_moe_layer_scratch(int n, int d, int ff, int top, int fp8, int E) {
   long long at[AT_PARTS];
-  return places(n, d, ff, top, fp8 != 0, at);
+  const int slots = n * top;
+  const int stages = fp8 ? (n <= 16 ? Layout<true, 16>::stages(ff, slots, E) : n <= 32 ? Layout<true, 32>::stages(ff, slots, E) : Layout<true, 64>::stages(ff, slots, E))
+                         : (n <= 16 ? Layout<false, 16>::stages(ff, slots, E) : n <= 32 ? Layout<false, 32>::stages(ff, slots, E) : Layout<false, 64>::stages(ff, slots, E));
+  return stages == 0 ? 0 : places(n, d, ff, top, fp8 != 0, at);
 }
 
 // h, add (may be null), out: bfloat16 [n, d].  router: `rows` rows, C = experts and identity experts, then perhaps one (rows = C + 1) whose
@@ -884,6 +898,7 @@ BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, i
         reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(add)) & 15) ||
       (long long)E * ffu > 0x7fffffff - 256 || (long long)E * d > 0x7fffffff - 256 || (long long)top * MAX_SPLITS > 16384)
     return (int)cudaErrorInvalidValue;
+  if (bspec_moe_layer_scratch(n, d, ff, top, fp8, E) == 0) return (int)cudaErrorInvalidValue;       // before the first kernel
   long long at[AT_PARTS];
   places(n, d, ff, top, fp8, at);
   char* base = (char*)scratch;

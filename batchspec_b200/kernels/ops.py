@@ -132,7 +132,7 @@ _SIGNATURES = {
                            c_int, c_void_p],
     "bspec_gemm_fp8": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
-    "bspec_moe_layer_scratch": [c_int] * 5,
+    "bspec_moe_layer_scratch": [c_int] * 6,
     "bspec_moe_layer": [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "bspec_moe_route": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
@@ -1919,8 +1919,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     whose logit's sigmoid multiplies ``add``.  ``w_up`` [E, ff, d] (``glu``: [E, 2 ff, d], gates first), ``w_down`` [E, d, ff]: bfloat16,
     or float8_e4m3fn with ``up_scale`` / ``down_scale``, a float32 or float8_e8m0fnu scale per 128 x 128 block of every expert (both of one
     type; what ``quantize_fp8`` makes of the stacked matrices).  With 8-bit weights the activations keep
-    8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps: ``moe_route`` and
-    ``moe_experts``."""
+    8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps, and
+    hundreds of choices for tens of tokens, are refused: ``moe_route`` and ``moe_experts`` take them."""
     stream = _stream_of(h, router, correction, w_up, w_down, up_scale, down_scale, add)
     if h.dim() != 2 or w_up.dim() != 3 or w_down.dim() != 3 or router.dim() != 2:
         raise KernelError("moe_layer takes h and router as matrices, w_up and w_down as stacks of matrices")
@@ -1968,7 +1968,10 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
         return out
     lib = load_library(features=("moe",))
     # everything between the two kernels, counters too: a buffer of its own, so that calls on other streams or in other graphs share nothing
-    scratch = h.new_empty((lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8)),), dtype=torch.uint8)
+    size = lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8), E)
+    if size == 0:
+        raise KernelError(f"moe_layer: {top} choices for each of {n} tokens among {E} experts do not fit: moe_route and moe_experts take them")
+    scratch = h.new_empty((size,), dtype=torch.uint8)
     rule = (1 if softmax_top else 2 if softmax else 0) + (4 if group_max else 0) + (8 if renormalise else 0)
     _check(lib.bspec_moe_layer(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),
                                _dtype_code(correction.dtype) if correction is not None else F32, many, int(n_groups), int(keep), int(top),

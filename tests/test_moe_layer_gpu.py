@@ -145,6 +145,9 @@ CASES = [
     (33, 24, 8, 4, 1152, 896, True, "softmax", 1, 1, None, True),
     (48, 2, 0, 1, 512, 2048, True, "softmax_top", 1, 1, "gated", True),
     (64, 300, 0, 5, 2048, 160, True, "softmax_top", 1, 1, None, True),
+    (64, 2, 0, 1, 128, 14336, True, "softmax_top", 1, 1, None, True),
+    (20, 3, 0, 2, 256, 8336, False, "softmax_top", 1, 1, None, True),
+    (2, 2, 0, 2, 9232, 4112, True, "softmax", 1, 1, "plain", True),
 ]
 
 
@@ -299,6 +302,15 @@ def test_a_decode_step_of_8bit_products(ops):
     h = (y.float() * 8).round().clamp(-16, 16) / 8          # exact logits
     args = (h.to(torch.bfloat16),) + args[1:]
     check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax_top")
+
+
+def test_more_choices_than_fit_are_refused(ops):
+    h = torch.zeros(64, 64, device=DEV, dtype=torch.bfloat16)
+    router, w_up = torch.zeros(512, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(512, 32, 64, device=DEV, dtype=torch.bfloat16)
+    w_down = torch.zeros(512, 64, 32, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="do not fit"):
+        ops.moe_layer(h, router, None, 1, 1, 512, 1.0, w_up, w_down)
+    ops.check_status()
 
 
 def test_refusals(ops):
