@@ -28,8 +28,8 @@
 // weights have pushed out of the L2 since the last step: loops are kept as loops, and the polls of a wait are a call (1 token 38.4 -> 35.9 us,
 // 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code),
 // and pieces are numbered without divisions by numbers of the step (61 tokens 133.8 -> 130.5).
-// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 54; 61 tokens, GELU, 131 (5.6 TB/s);
-// 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.
+// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 54; 61 tokens, GELU, 127 (5.8 TB/s);
+// 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 35.
 #include "moe_choose.cuh"
 #include "e4m3.cuh"
 #include "umma.cuh"
@@ -373,7 +373,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       n_active = __popc(leaders);
     }
   } else if (warp == 0) {
-    // counted, then placed in the order of their numbers
+    // counted; they take their places below
     int found = 0, run = 0;
 #pragma unroll 1
     for (int e0 = 0; e0 < p.E; e0 += 32) {
@@ -396,22 +396,6 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     if (lane == 0) {
       first[found] = run;
       n_active = found;
-    }
-    __syncwarp();
-#pragma unroll 1
-    for (int s0 = 0; s0 < slots; s0 += 32) {
-      const int s = s0 + lane, e = s < slots ? p.ids[s] : p.E;
-      const unsigned same = __match_any_sync(0xffffffffu, e);
-      if (e < p.E) {
-        const int from = count[e], at = from + __popc(same & ((1u << lane) - 1u));
-        pos[s] = at;
-        tok[at] = s / p.top;
-        __syncwarp(same);
-        if (lane == __ffs(same) - 1) count[e] = from + __popc(same);
-      } else if (s < slots) {
-        pos[s] = -1;
-      }
-      __syncwarp();
     }
   }
   __syncthreads();
@@ -596,6 +580,27 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     int slot = group * SLOTS;
     uint32_t slot_phase = 0u, meet_phase = 0u;
     bool ok = true, up_known = false;
+    if (slots > 32) {
+      // the entries take their places while the first copies are on their way
+      if (warp == 2) {
+#pragma unroll 1
+        for (int s0 = 0; s0 < slots; s0 += 32) {
+          const int s = s0 + lane, e = s < slots ? p.ids[s] : p.E;
+          const unsigned same = __match_any_sync(0xffffffffu, e);
+          if (e < p.E) {
+            const int from = count[e], at = from + __popc(same & ((1u << lane) - 1u));
+            pos[s] = at;
+            tok[at] = s / p.top;
+            __syncwarp(same);
+            if (lane == __ffs(same) - 1) count[e] = from + __popc(same);
+          } else if (s < slots) {
+            pos[s] = -1;
+          }
+          __syncwarp();
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
     // one arrival per warp: those of 32 lanes on one barrier would come one after the other
     auto arrive = [&](uint64_t* bar) {
       __syncwarp();
