@@ -694,6 +694,9 @@ int few_splits(long long tiles, int nkb, int sms) {
 // E.g. 4,096 x 14,336, few / many / pairs: 64 tokens 19 / 48 / 42, 256 tokens 51 / 50 / 46, 1,024 tokens - / 98 / 77;
 // 4,096 x 4,096: 128 tokens 13 / 17 / 23, 512 tokens 29 / 18 / 24.
 enum Form { FEW, MANY, PAIR };
+// The pairs' sums stay in the tensor cores, which cut what an addition shifts out: 1.4e-6 of a result over 11,264 k, where sums in registers are
+// off by 1e-7.  A float32 result over more than PAIR_K numbers is therefore not theirs.
+constexpr int PAIR_K = 4096;
 Form choose(int M, int N, int K, bool powers, int sms) {
   const int nkb = (K + KBYTES - 1) / KBYTES;
   const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
@@ -780,7 +783,7 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
   const int sms = bspec::sm_count();
   const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + MANY_BN - 1) / MANY_BN;
   const long long pairs_m = (M + 255) / 256, pairs_n = (N + PAIR_BN - 1) / PAIR_BN;
-  const Form form = choose(M, N, K, xs_e8m0 && ws_e8m0, sms);
+  const Form form = choose(M, N, K, xs_e8m0 && ws_e8m0 && !(out_f32 && K > PAIR_K), sms);
   CUtensorMap map_x, map_w;
   const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
   if (!make_map_bytes(&map_x, X, M, K, ldx, form == FEW ? bn : TILE_ROWS) ||

@@ -9,8 +9,8 @@
 // a stage costs two copies of weights and a few instructions, and what the sums cost does not grow with the weights.
 //   up     all tokens of the step are columns of every expert (no gather: the columns that did not choose it are dropped)
 //   down   an expert's tokens are its columns: u lies sorted by expert, 16 rows to a copy
-// bfloat16 weights: u is rounded to bfloat16 between the products.  8-bit weights: the activations do not lose precision to the
-// weights' format.  Every activation is the sum of two e4m3 numbers, x = s (a + b / 16): a is x / s rounded to 4 bits, b what is
+// The activations do not lose precision to the weights' format.  bfloat16 weights: every number of u is the sum of two bfloat16 numbers, 16
+// bits, both columns of the same product.  8-bit weights:  Every activation is the sum of two e4m3 numbers, x = s (a + b / 16): a is x / s rounded to 4 bits, b what is
 // left, times 16; s is a power of two, one for a token's h and one for 64 numbers of u.  That is 8 bits, as many as bfloat16 has (h is met
 // exactly down to 2^-22 of the token's largest number); both are columns of the same product.  A block of 128 k (of 64 in the down
 // products, for the scales of u) gets an accumulator of its own, which the epilogue warps read back and add to float32 sums.
@@ -187,7 +187,7 @@ struct LayerParams {
   const __nv_bfloat16* h;                    // [n, d]
   const __nv_bfloat16* add;                  // [n, d] or null
   const float* hs;                           // [n] scales of the tokens' 8-bit numbers
-  unsigned char* u;                          // entries sorted by expert: [n top, ff] bfloat16, or e4m3 [2][n top, ff]
+  unsigned char* u;                          // entries sorted by expert, two numbers for each: [2][n top, ff] bfloat16 or e4m3
   float* us;                                 // [n top, blocks of 64] their scales
   float* y;                                  // [splits][n top, d] the experts' results
   __nv_bfloat16* out;                        // [n, d]
@@ -238,7 +238,7 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) { return make
 // Shared memory behind the stages.  NB: columns, 16, 32 or 64.
 template <bool FP8, int NB>
 struct Layout {
-  static constexpr int B_BYTES = NB * 128 * (FP8 ? 2 : 1), STAGE = A_BYTES + B_BYTES;
+  static constexpr int B_BYTES = 2 * NB * 128, STAGE = A_BYTES + B_BYTES;
   // rows of scales: blocks of 64 in whole stages, a window of them at most
   __host__ __device__ static int rows(int ff) { return (ff + 127) / 128 * 2 < WINDOW ? (ff + 127) / 128 * 2 : WINDOW; }
   // of each epilogue group: tile [NB][128], scales of a piece's u [rows][NB]; then the lists
@@ -260,9 +260,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
                          const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_u, LayerParams p) {
   using Lay = Layout<FP8, NB>;
   constexpr int STAGE_K = FP8 ? 128 : 64;                      // k of a stage
-  constexpr int WIDTH = FP8 ? 2 * NB : NB;                     // columns of an accumulator
-  constexpr int SLOTS = FP8 && NB == 64 ? 2 : 4;               // accumulators of each epilogue group
-  constexpr uint32_t TMEM_COLS = 2 * SLOTS * WIDTH;            // 128 .. 512
+  constexpr int WIDTH = 2 * NB;                                // columns of an accumulator
+  constexpr int SLOTS = NB == 64 ? 2 : 4;                      // accumulators of each epilogue group
+  constexpr uint32_t TMEM_COLS = 2 * SLOTS * WIDTH;            // 256 or 512
   constexpr int OUT = GLU ? 64 : 128;                          // numbers of u per up piece
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
@@ -441,18 +441,18 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (ok) ok = warp_wait_short(empty + st, phase ^ 1u, abort_flag, p.status, 114);
       if (!ok) return;
       unsigned char* at = smem + (size_t)st * Lay::STAGE;
-      mbar_expect_tx_by(one, full + st, A_BYTES + (uint32_t)boxes * 2048u * (FP8 ? 2u : 1u));
+      mbar_expect_tx_by(one, full + st, A_BYTES + (uint32_t)boxes * 2048u);
       tma_load_2d_by(one, at, map, full + st, s * STAGE_K, y0);
       tma_load_2d_by(one, at + A_BYTES / 2, map, full + st, s * STAGE_K, y1);
     };
-    auto tokens = [&](const CUtensorMap* map, int y, int mid, int boxes, int s) {
+    auto tokens = [&](const CUtensorMap* map, int y, int mid, int boxes, bool two, int s) {
       if (!ok) return;
       unsigned char* at = smem + (size_t)st * Lay::STAGE + A_BYTES;
 #pragma unroll
       for (int b = 0; b < NB / 16; ++b) {
         if (b >= boxes) break;
         tma_load_2d_by(one, at + b * 2048, map, full + st, s * STAGE_K, y + 16 * b);
-        if (FP8) tma_load_2d_by(one, at + (boxes + b) * 2048, map, full + st, s * STAGE_K, mid + y + 16 * b);
+        if (two) tma_load_2d_by(one, at + (boxes + b) * 2048, map, full + st, s * STAGE_K, mid + y + 16 * b);
       }
     };
     auto step = [&]() {
@@ -467,8 +467,8 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int y0 = e * ffu + i0, y1 = y0 + (GLU ? p.ff : 64);
 #pragma unroll 1
       for (int s = 0; s < up_stages && ok; ++s, step()) {
-        weights(&map_up, y0, y1, NB / 16, s);
-        tokens(&map_h, 0, p.n, NB / 16, s);
+        weights(&map_up, y0, y1, NB / 16 * (FP8 ? 2 : 1), s);
+        tokens(&map_h, 0, p.n, NB / 16, FP8, s);
       }
       t = draw(0);                                             // not earlier: a CTA that starts first would take the others' first pieces
     }
@@ -488,7 +488,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const int ahead = min(s1 - s0, p.stages), st_from = st;
         const uint32_t phase_from = phase;
 #pragma unroll 1
-        for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, boxes, s0 + i);
+        for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, 2 * boxes, s0 + i);
         if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
         if (lane == 0 && ok) mbar_arrive(&up_done);            // the epilogue may read the scales of u
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -497,13 +497,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         st = st_from;
         phase = phase_from;
 #pragma unroll 1
-        for (int i = 0; i < ahead; ++i, step()) tokens(&map_u, c0, slots, boxes, s0 + i);
+        for (int i = 0; i < ahead; ++i, step()) tokens(&map_u, c0, slots, boxes, true, s0 + i);
         s = s0 + ahead;
       }
 #pragma unroll 1
       for (; s < s1 && ok; ++s, step()) {
-        weights(&map_down, y0, y0 + 64, boxes, s);
-        tokens(&map_u, c0, slots, boxes, s);
+        weights(&map_down, y0, y0 + 64, 2 * boxes, s);
+        tokens(&map_u, c0, slots, boxes, true, s);
       }
       t = draw(2);
     }
@@ -525,7 +525,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (lane == 0) mbar_arrive(q_empty + q);
       if (piece.down < 0) break;
       const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
-      const int cols = boxes * 16 * (FP8 ? 2 : 1);
+      const int cols = boxes * 16 * (FP8 || piece.down ? 2 : 1);
       const uint32_t idesc = FP8 ? instr_desc_e4m3(cols) : instr_desc(cols);
       const int group = np & 1;
       int slot = group ? SLOTS + ring[1] : ring[0];
@@ -700,11 +700,12 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       } else if (ok) {
 #pragma unroll 1
         for (int cc = 0; cc < cols; cc += 16) {
-          uint32_t v[16];
+          uint32_t v[16], lo[16];
           tc_ld16(lane_base + (uint32_t)(slot * WIDTH + cc), v);
+          tc_ld16(lane_base + (uint32_t)(slot * WIDTH + (piece.down ? cols + cc : cc)), lo);
           tc_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 16; ++c) tile[(cc + c) * TILE + row] = __uint_as_float(v[c]);
+          for (int c = 0; c < 16; ++c) tile[(cc + c) * TILE + row] = __uint_as_float(v[c]) + (piece.down ? __uint_as_float(lo[c]) : 0.f);
         }
       }
       if (!piece.down) {
@@ -743,8 +744,12 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
             } else {
 #pragma unroll
               for (int j = 0; j < 2; ++j)
-                if (f0 + 32 * j + lane < p.ff)
-                  reinterpret_cast<__nv_bfloat16*>(p.u)[(size_t)(c0 + i) * p.ff + f0 + 32 * j + lane] = __float2bfloat16_rn(v[j]);
+                if (f0 + 32 * j + lane < p.ff) {
+                  __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(p.u) + (size_t)(c0 + i) * p.ff + f0 + 32 * j + lane;
+                  const __nv_bfloat16 hi = __float2bfloat16_rn(v[j]);
+                  to[0] = hi;
+                  to[(size_t)slots * p.ff] = __float2bfloat16_rn(isinf(__bfloat162float(hi)) ? 0.f : v[j] - __bfloat162float(hi));
+                }
             }
           }
         }
@@ -868,7 +873,7 @@ enum { AT_IDS, AT_WTS, AT_GATE, AT_HQ, AT_HS, AT_U, AT_US, AT_Y, AT_PARTS };
 long long places(int n, int d, int ff, int top, bool fp8, long long (&at)[AT_PARTS]) {
   const long long slots = (long long)n * top, blocks_ff = (ff + 63) / 64;
   const long long bytes[AT_PARTS] = {4 * slots, 4 * slots, 4ll * n, fp8 ? 2ll * n * d : 0, fp8 ? 4ll * n : 0,
-                                     2 * slots * ff, fp8 ? 4 * slots * blocks_ff : 0, 4 * MAX_SPLITS * slots * d};
+                                     (fp8 ? 2 : 4) * slots * ff, fp8 ? 4 * slots * blocks_ff : 0, 4 * MAX_SPLITS * slots * d};
   long long size = 16;
   for (int i = 0; i < AT_PARTS; ++i) {
     at[i] = (size + 127) / 128 * 128;
@@ -920,7 +925,7 @@ BSPEC_API int bspec_moe_layer(const void* h, int n, int d, const void* router, i
   CUtensorMap maps[4];
   if (!make_map(maps, wu, (long long)E * ffu, d, bytes, 64) || !make_map(maps + 1, wd, (long long)E * d, ff, bytes, 64) ||
       !make_map(maps + 2, fp8 ? (const void*)(base + at[AT_HQ]) : h, fp8 ? 2 * n : n, d, bytes, 16) ||
-      !make_map(maps + 3, p.u, (fp8 ? 2ll : 1ll) * n * top, ff, bytes, 16))
+      !make_map(maps + 3, p.u, 2ll * n * top, ff, bytes, 16))
     return (int)cudaErrorInvalidValue;
 
   const int tiles = (rows + 15) / 16, steps = (d + 31) / 32;
