@@ -28,8 +28,8 @@
 // weights have pushed out of the L2 since the last step: loops are kept as loops, and the polls of a wait are a call (1 token 38.4 -> 35.9 us,
 // 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code),
 // and pieces are numbered without divisions by numbers of the step (61 tokens 133.8 -> 130.5).
-// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 35 us; 8 tokens, gated, 8-bit, 54; 61 tokens, GELU, 127 (5.8 TB/s);
-// 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 35.
+// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 36 us; 8 tokens, gated, 8-bit, 55; 61 tokens, GELU, 128.5 (5.7 TB/s);
+// 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.
 #include "moe_choose.cuh"
 #include "e4m3.cuh"
 #include "umma.cuh"
@@ -238,7 +238,11 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) { return make
 // Shared memory behind the stages.  NB: columns, 16, 32 or 64.
 template <bool FP8, int NB>
 struct Layout {
-  static constexpr int B_BYTES = 2 * NB * 128, STAGE = A_BYTES + B_BYTES;
+  // room for two numbers per column; 64 columns of bfloat16: for one, as few experts have more than 32 tokens and
+  // stages are worth more (61 tokens: 4 stages 138 us, 6 stages 128.5)
+  static constexpr int B_BYTES = (!FP8 && NB == 64 ? 1 : 2) * NB * 128, STAGE = A_BYTES + B_BYTES;
+  // where an expert's tokens do not fit in twice, its stages come twice (the second time out of the L2)
+  __device__ static int twice(int boxes) { return boxes * 4096 > B_BYTES ? 1 : 0; }
   // rows of scales: blocks of 64 in whole stages, a window of them at most
   __host__ __device__ static int rows(int ff) { return (ff + 127) / 128 * 2 < WINDOW ? (ff + 127) / 128 * 2 : WINDOW; }
   // of each epilogue group: tile [NB][128], scales of a piece's u [rows][NB]; then the lists
@@ -481,14 +485,16 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       const int s0 = split * down_per, s1 = min(down_stages, s0 + down_per), c0 = first[a];
       push({1, a, dt, s0, s1, split});
       const int y0 = e * p.d + dt * TILE, boxes = (first[a + 1] - c0 + 15) / 16;
-      int s = s0;
+      const int twice = Lay::twice(boxes), end = s1 << twice, at_once = twice ? boxes : 2 * boxes;
+      auto down_tokens = [&](int s) { tokens(&map_u, c0 + (s & twice) * slots, slots, boxes, !twice, s >> twice); };
+      int s = s0 << twice;
       if (!waited) {
         // the first weights are asked for before the wait for the up products
         waited = true;
-        const int ahead = min(s1 - s0, p.stages), st_from = st;
+        const int ahead = min(end - s, p.stages), st_from = st;
         const uint32_t phase_from = phase;
 #pragma unroll 1
-        for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, 2 * boxes, s0 + i);
+        for (int i = 0; i < ahead && ok; ++i, step()) weights(&map_down, y0, y0 + 64, at_once, (s + i) >> twice);
         if (lane == 0 && ok) ok = wait_for(p.counters + 1, up_pieces, p.status, abort_flag);
         if (lane == 0 && ok) mbar_arrive(&up_done);            // the epilogue may read the scales of u
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -497,13 +503,13 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         st = st_from;
         phase = phase_from;
 #pragma unroll 1
-        for (int i = 0; i < ahead; ++i, step()) tokens(&map_u, c0, slots, boxes, true, s0 + i);
-        s = s0 + ahead;
+        for (int i = 0; i < ahead; ++i, step()) down_tokens(s + i);
+        s += ahead;
       }
 #pragma unroll 1
-      for (; s < s1 && ok; ++s, step()) {
-        weights(&map_down, y0, y0 + 64, 2 * boxes, s);
-        tokens(&map_u, c0, slots, boxes, true, s);
+      for (; s < end && ok; ++s, step()) {
+        weights(&map_down, y0, y0 + 64, at_once, s >> twice);
+        down_tokens(s);
       }
       t = draw(2);
     }
@@ -525,7 +531,8 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       if (lane == 0) mbar_arrive(q_empty + q);
       if (piece.down < 0) break;
       const int boxes = piece.down ? (first[piece.a + 1] - first[piece.a] + 15) / 16 : NB / 16;
-      const int cols = boxes * 16 * (FP8 || piece.down ? 2 : 1);
+      const int twice = piece.down ? Lay::twice(boxes) : 0;
+      const int cols = boxes * 16 * ((FP8 || piece.down) && !twice ? 2 : 1);
       const uint32_t idesc = FP8 ? instr_desc_e4m3(cols) : instr_desc(cols);
       const int group = np & 1;
       int slot = group ? SLOTS + ring[1] : ring[0];
@@ -540,7 +547,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       };
       if (!FP8) next_slot();
 #pragma unroll 1
-      for (int s = piece.s0; s < piece.s1 && ok; ++s) {
+      for (int s = piece.s0 << twice; s < piece.s1 << twice && ok; ++s) {
         if (!(ok = warp_wait_short(full + st, phase, abort_flag, p.status, 117))) break;
         tc_fence_after();
         const uint64_t wd = desc0 + (uint64_t)(st * (Lay::STAGE / 16)), xd = wd + A_BYTES / 16;      // addresses count 16 bytes
@@ -561,7 +568,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_by(one, tmem_base + slot * WIDTH, wd + 2 * k, xd + 2 * k, idesc, (s > piece.s0 || k > 0) ? 1u : 0u);
+            tc_mma_by(one, tmem_base + slot * WIDTH + (s & twice) * cols, wd + 2 * k, xd + 2 * k, idesc, ((s >> twice) > piece.s0 || k > 0) ? 1u : 0u);
           tc_commit_by(one, empty + st);
         }
         if (++st == p.stages) { st = 0; phase ^= 1u; }

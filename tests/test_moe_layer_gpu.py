@@ -91,7 +91,7 @@ def choice_of(z, rule, correction, groups, keep, top, scale):
 def check_layer(out, args, kw, upv, downv, rule, rows=None):
     h, router, correction, groups, keep, top, scale, _, _ = args
     E, ff, d, many = upv.shape[0], downv.shape[2], h.shape[1], upv.shape[0] + kw["identity"]
-    z = (h.double() @ router.double().t())
+    z, of_squares, all_squares = (h.double() @ router.double().t()), 0.0, 0.0
     corr = correction.double().tolist() if correction is not None else None
     assert out.dtype == torch.bfloat16 and out.shape == h.shape
     for t in rows if rows is not None else range(h.shape[0]):
@@ -121,6 +121,8 @@ def check_layer(out, args, kw, upv, downv, rule, rows=None):
         room += want.abs() * 2.0 ** -8 + 2.0 ** -126
         off = (out[t].double() - want).abs()
         assert bool((off <= room).all()), (t, float((off / room).max()))
+        of_squares, all_squares = of_squares + float((off ** 2).sum()), all_squares + float((want ** 2).sum())
+    return math.sqrt(of_squares / max(all_squares, 1e-300))
 
 
 CASES = [
@@ -302,6 +304,18 @@ def test_a_decode_step_of_8bit_products(ops):
     h = (y.float() * 8).round().clamp(-16, 16) / 8          # exact logits
     args = (h.to(torch.bfloat16),) + args[1:]
     check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax_top")
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e8m0", "float32"])
+@pytest.mark.parametrize("n,E,top", [(16, 8, 3), (32, 24, 2), (60, 2, 1), (60, 30, 4)])
+def test_activations_keep_their_precision(ops, weights, n, E, top):
+    """What is left of the error is the result's rounding: 2^-8 at most at a significand of 1, evenly spread, 2^-8 / sqrt(3) / significand over
+    significands of equal logarithms: 2^-8 sqrt(1/3) sqrt(3/8 / log 2) = 1.66e-3, over 8,192 numbers and more within 3 in 100.  8-bit experts: and two
+    e4m3 numbers for each of u, at most 2^-9 off at a significand of 1, so half of that: 1.86e-3 in all; 16 bits of u add nothing to see
+    (u rounded to bfloat16 would make it 2.3e-3)."""
+    args, kw, upv, downv = layer_case(ops, n, E, 0, top, 512, 256, True, weights, "softmax_top", 1, 1, None, True)
+    off = check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax_top")
+    assert off <= (1.66e-3 if weights == "bfloat16" else 1.86e-3) * 1.05
 
 
 def test_more_choices_than_fit_are_refused(ops):
