@@ -28,6 +28,21 @@ __device__ __forceinline__ uint32_t to_e4m3x4(const float* v, float inv) {
 __device__ __forceinline__ float scale_value(uint32_t code) {
   return __uint_as_float(code == 0u ? 0x00400000u : (code == 255u ? 0x7fc00000u : code << 23));
 }
+// Whether the product f of two scales leaves float32's normal range although neither is 0 or infinite: such a product keeps few bits or none
+// (a sum of 128 products of e4m3 numbers, up to 2^25, brings 2^-140 back into the range), or turns a sum of 0 into NaN.
+__device__ __forceinline__ bool leaves_range(float x, float w, float f) {
+  return (fabsf(f) < 1.17549435e-38f && x != 0.f && w != 0.f) || (isinf(f) && !isinf(x) && !isinf(w));
+}
+// whether f is a normal number: what leaves_range holds for is not
+__device__ __forceinline__ bool is_ordinary(float f) { return ((__float_as_uint(f) & 0x7fffffffu) - 0x00800000u) < 0x7f000000u; }
+// Such a product as two factors with half of its exponent each: a sum that meets one after the other stays in the range if the result does.
+__device__ __forceinline__ void split_scales(float x, float w, float& first, float& second) {
+  int ex, ew;
+  const float mx = frexpf(x, &ex), mw = frexpf(w, &ew);
+  const int half = (ex + ew) >> 1;
+  first = ldexpf(mx, half);
+  second = ldexpf(mw, ex + ew - half);
+}
 // Two e4m3 numbers for one: v * inv = a + b / 16, a the nearest e4m3 number, b what is left, times 16 (|b| <= |a| where a is not among
 // the smallest numbers; exact for a v of 8 bits).  Two values, and four, packed with the first in the low byte.
 __device__ __forceinline__ void two_e4m3x2(float v0, float v1, float inv, uint32_t& a, uint32_t& b) {

@@ -2,10 +2,11 @@
 //   C[m, n] = sum over blocks b of 128 k:  xs[m, b] * ws[n / 128, b] * sum over k in b of X[m, k] * W[n, k]
 // X [M, K] has a scale per row and block, W [N, K] one per 128 x 128; scales are float32 numbers or powers of two in 8 bits (e8m0).
 //
-// The products of one block are exact sums of the tensor core (tcgen05.mma kind::f8f6f4, float32 accumulator in tensor memory); the
+// The products of one block are sums of the tensor core (tcgen05.mma kind::f8f6f4, float32 accumulator in tensor memory); the
 // scales differ from block to block, so every block of 128 k gets an accumulator of its own (a ring of them in tensor memory), and
 // the epilogue warps read it back, multiply by its scales and add it to float32 sums in registers while the next blocks' products
-// run.  The sum over blocks is in ascending k.
+// run.  The sum over blocks is in ascending k.  Where the product of the two scales alone would leave float32's range, a sum meets them in two factors
+// with half of the exponent each, so that small results keep their bits and zeros stay zeros.
 //
 // Three arrangements, chosen by an estimate of their times (`choose`):
 //   few tokens    rows of W on the accumulator's 128 rows, tokens on its columns: every weight is streamed once at full tile efficiency.  K
@@ -31,7 +32,7 @@ namespace {
 constexpr int KBYTES = 128;            // k per stage: one scale block, one 128-byte swizzle span
 constexpr int TILE_ROWS = 128;
 constexpr int FEW_THREADS = 192;       // TMA warp, MMA warp, 4 epilogue warps
-constexpr int FEW_WINDOW = 32;         // k blocks whose scales wait in shared memory at a time
+constexpr int FEW_WINDOW = 16;         // k blocks whose scales wait in shared memory at a time
 constexpr int MANY_THREADS = 320;      // TMA warp, MMA warp, 8 epilogue warps
 constexpr int MANY_BN = 128, MANY_STAGES = 6;
 
@@ -98,8 +99,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   constexpr int W_BYTES = TILE_ROWS * KBYTES, X_BYTES = BN * KBYTES, STAGE = W_BYTES + X_BYTES;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
-  float* scales = reinterpret_cast<float*>(smem + (size_t)p.stages * STAGE);      // [FEW_WINDOW][BN], xs * ws
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + FEW_WINDOW * BN);
+  float* scales = reinterpret_cast<float*>(smem + (size_t)p.stages * STAGE);      // [FEW_WINDOW][BN], xs * ws; and again, what a sum meets before it
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 2 * FEW_WINDOW * BN);
   uint64_t* empty = full + p.stages;
   uint64_t* acc_full = empty + p.stages;
   uint64_t* acc_empty = acc_full + NB;
@@ -187,17 +188,35 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     const uint32_t quad = warp & 3;
     const int et = threadIdx.x - 64;                                   // 0 .. 127
     bspec::pdl_wait();
-    bool ok = true;
+    bool ok = true, apart = false;
+    // whether it holds for any epilogue thread; they meet here
+    auto any_of = [](bool mine) {
+      uint32_t any;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "=r"(any) : "r"((uint32_t)mine) : "memory");
+      return any != 0u;
+    };
     for (int i = 0; i < nkb; ++i) {
       if (i % FEW_WINDOW == 0) {
         // the scales of the next blocks; every epilogue thread comes here, whatever its waits said
         const int nw = min(FEW_WINDOW, nkb - i);
         asm volatile("bar.sync 1, 128;" ::: "memory");
+        bool leaves = false;
         for (int j = et; j < nw * BN; j += 128) {
           const int c = j / nw, b = j - c * nw, tok = tok0 + c;        // neighbours read neighbouring blocks of a token
-          scales[b * BN + c] = tok < p.M ? scale_at(p.xs, tok, kb0 + i + b) * scale_at(p.ws, tile_n, kb0 + i + b) : 0.f;
+          float f = 0.f, before = 1.f;
+          if (tok < p.M) {
+            const float x = scale_at(p.xs, tok, kb0 + i + b), w = scale_at(p.ws, tile_n, kb0 + i + b);
+            f = x * w;
+            if (leaves_range(x, w, f)) {
+              split_scales(x, w, before, f);
+              leaves = true;
+            }
+          }
+          scales[b * BN + c] = f;
+          scales[(FEW_WINDOW + b) * BN + c] = before;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        apart = any_of(leaves);
       }
       const int b = i % NB;
       if (ok) ok = mbar_wait(acc_full + b, (uint32_t)(i / NB) & 1u, abort_flag, p.status, 104);
@@ -217,6 +236,10 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       else tc_ld64(from, v);
       tc_wait_ld();
       release();
+      if (apart) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * reinterpret_cast<const float*>(f)[FEW_WINDOW * BN + c]);
+      }
 #pragma unroll
       for (int c = 0; c < BN; c += 4) {
         const float4 g = f[c / 4];
@@ -379,8 +402,11 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
       for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
       float x_next = scale_at(p.xs, srow, 0), w_next = scale_at(p.ws, wrow, 0);
+      // whether a row's product of scales is not a normal number: asked behind the additions, when the next scales have come (before the wait for
+      // an accumulator it cost 14 of 118 us of the product of 1,537 x 4,096 x 14,336, here nothing)
+      bool apart = __any_sync(0xffffffffu, !is_ordinary(x_next * w_next));
       for (int kb = 0; kb < nkb; ++kb) {
-        const float f = x_next * w_next;
+        const float x = x_next, w = w_next;
         if (kb + 1 < nkb) {
           x_next = scale_at(p.xs, srow, kb + 1);
           w_next = scale_at(p.ws, wrow, kb + 1);
@@ -395,12 +421,20 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + b);
         if (++b == NB) { b = 0; phase ^= 1u; }
+        float f = x * w;
+        if (apart) {
+          float before = 1.f;
+          if (leaves_range(x, w, f)) split_scales(x, w, before, f);
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * before);
+        }
         const uint64_t ff = pack2(f, f);
 #pragma unroll
         for (int c = 0; c < COLS; c += 2) {                             // two to an instruction: the loop's time is what it issues
           const uint64_t sum = fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), ff, pack2(acc[c], acc[c + 1]));
           unpack2(sum, acc[c], acc[c + 1]);
         }
+        apart = __any_sync(0xffffffffu, !is_ordinary(x_next * w_next));
       }
       if (ok && m < p.M) {
         const size_t base = (size_t)m * p.N + n0;
@@ -719,7 +753,7 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, Fp8Params p, 
   p.kblocks_per_split = (kb_total + splits - 1) / splits;
   p.splits = (kb_total + p.kblocks_per_split - 1) / p.kblocks_per_split;       // no empty slice
   constexpr int STAGE = (TILE_ROWS + BN) * KBYTES;
-  constexpr int FIXED = 1024 + FEW_WINDOW * BN * 4 + 256;
+  constexpr int FIXED = 1024 + 2 * FEW_WINDOW * BN * 4 + 256;
   int stages = (112 * 1024 - FIXED) / STAGE;
   if (stages > 6) stages = 6;
   // the join's partial tile takes the stages' place
