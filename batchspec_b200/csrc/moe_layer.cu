@@ -669,6 +669,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           if (piece.down && i > 0 && i % WINDOW == 0) column_scales(i);
           __syncwarp();
           const float w_a = __shfl_sync(0xffffffffu, wa, s & 31), w_b = __shfl_sync(0xffffffffu, wb, s & 31);
+          // the weights' scale first: what it makes of a sum (up to 2^25) stays in float32's range for scales up to 2^100, and tokens may be of any size
           const float w = w_block == block_a ? w_a : w_b;
           if (ok) ok = mbar_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
@@ -686,7 +687,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
                 const float fx[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  acc[cc + j + k] = fmaf(fmaf(__uint_as_float(lo[j + k]), 0.0625f, __uint_as_float(hi[j + k])) * fx[k], w, acc[cc + j + k]);
+                  acc[cc + j + k] = fmaf(fmaf(__uint_as_float(lo[j + k]), 0.0625f, __uint_as_float(hi[j + k])) * w, fx[k], acc[cc + j + k]);
               }
             }
           tc_fence_before();
