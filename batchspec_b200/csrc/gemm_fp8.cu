@@ -467,6 +467,12 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 //   scale warps   bring the scales of four stages into the form that is copied: 32 lanes x 16 bytes, rows l, l + 32, l + 64, l + 96, a byte per
 //                 stage (the products of a stage name its byte)
 //   epilogue      eight warps: 128 rows x half the columns, read at once, freed, converted and stored while the next tile's products run
+// The tensor cores cut what an addition shifts out, always towards 0: over K products of one sign a sum that stays in them is off by 8.5e-8 of it at
+// 512 numbers, 2.0e-7 at 1,024, 5.2e-7 at 2,048, 1.5e-6 at 4,096 (root mean square), where a float32 product in the usual order is off by 5e-8 to
+// 2.3e-7.  A bfloat16 result does not notice (its rounding is 2e-3).  For a float32 result (JOIN) the accumulators change every PAIR_JOIN blocks of k, and
+// the epilogue adds them up in registers: 1.9e-7 at any K.  2,048 x 28,672 x 4,096 then takes 229 us instead of 200 (every 6 blocks 1.0e-7 and 247 us,
+// every 4 blocks 8.5e-8 and 264 us: what counts is the way of an accumulator through the epilogue and back; sums in registers for every block 414).
+constexpr int PAIR_JOIN = 8;           // blocks of k
 constexpr int PAIR_BN = 224, PAIR_STAGES = 7, PAIR_SF_SLOTS = 4, PAIR_SF_BUFS = 5, PAIR_THREADS = 448;
 constexpr int PAIR_X = TILE_ROWS * KBYTES, PAIR_W = PAIR_BN / 2 * KBYTES, PAIR_STAGE = PAIR_X + PAIR_W;
 constexpr int PAIR_SF = 512 + 1024;          // the scales of four stages: 128 rows of X, 256 of W
@@ -509,6 +515,7 @@ __device__ __forceinline__ void mma_scaled(uint32_t one, uint32_t tmem_d, uint64
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accum), "r"(one) : "memory");
 }
 
+template <bool JOIN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Fp8Params p) {
   extern __shared__ unsigned char smem_dyn[];
@@ -579,10 +586,25 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       uint32_t phase = 0u, acc_phase = 0u, sf_phase = 0u;
       bool ok = true;
       for (long long t = pair; t < tiles && ok; t += pairs) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(acc_empty + b, acc_phase ^ 1u, abort_flag, p.status, 122)))) break;
-        tc_fence_after();
+        // an accumulator for the whole row or, JOIN, for every PAIR_JOIN blocks of it
+        auto next_acc = [&]() {
+          ok = __all_sync(0xffffffffu, mbar_wait<true>(acc_empty + b, acc_phase ^ 1u, abort_flag, p.status, 122));
+          tc_fence_after();
+        };
+        next_acc();
+        if (!ok) break;
         uint32_t sfa = 0u, sfb = 0u;
+        int done = 0;                        // blocks in this accumulator
         for (int kb = 0; kb < nkb; ++kb) {
+          if constexpr (JOIN) {
+            if (done == PAIR_JOIN) {
+              commit_pair(one, acc_full + b);
+              if (++b == 2) { b = 0; acc_phase ^= 1u; }
+              next_acc();
+              if (!ok) break;
+              done = 0;
+            }
+          }
           if ((kb & 3) == 0) {
             if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(sf_full + slot, sf_phase, abort_flag, p.status, 126)))) break;
             tc_fence_after();
@@ -601,9 +623,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           const uint64_t xd = smem_desc(smem + st * PAIR_STAGE), wd = smem_desc(smem + st * PAIR_STAGE + PAIR_X);
 #pragma unroll
           for (int k = 0; k < KBYTES / 32; ++k)
-            mma_scaled(one, tmem_base + b * PAIR_BN, xd + 2 * k, wd + 2 * k, desc, sfa, sfb, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_scaled(one, tmem_base + b * PAIR_BN, xd + 2 * k, wd + 2 * k, desc, sfa, sfb, ((JOIN ? done : kb) > 0 || k > 0) ? 1u : 0u);
           commit_pair(one, empty + st);
           if (++st == PAIR_STAGES) { st = 0; phase ^= 1u; }
+          ++done;
         }
         if (!ok) break;
         commit_pair(one, acc_full + b);
@@ -668,17 +691,40 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     bool ok = true;
     for (long long t = pair; t < tiles && ok; t += pairs) {
       const int m = (int)(t % p.tiles_m) * 256 + (int)rank * TILE_ROWS + row, n0 = (int)(t / p.tiles_m) * PAIR_BN + half * COLS;
-      if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 125))) break;
-      tc_fence_after();
       float acc[COLS];
+      // this thread's columns of an accumulator, which then is free; into the sums or, JOIN, onto them
+      auto take = [&]() {
+        if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 125))) return;
+        tc_fence_after();
+        const uint32_t from = tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * PAIR_BN + half * COLS);
+        if constexpr (JOIN) {
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16)
-        tc_ld16(tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * PAIR_BN + half * COLS + c), *reinterpret_cast<uint32_t(*)[16]>(acc + c));
-      tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_in(in_cta(acc_empty + b, 0));
-      if (++b == 2) { b = 0; phase ^= 1u; }
+          for (int c = 0; c < COLS; c += 16) {
+            uint32_t v[16];
+            tc_ld16(from + c, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(v[j]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < COLS; c += 16) tc_ld16(from + c, *reinterpret_cast<uint32_t(*)[16]>(acc + c));
+          tc_wait_ld();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_in(in_cta(acc_empty + b, 0));
+        if (++b == 2) { b = 0; phase ^= 1u; }
+      };
+      if constexpr (JOIN) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+#pragma unroll 1
+        for (int k0 = 0; k0 < nkb && ok; k0 += PAIR_JOIN) take();
+      } else {
+        take();
+      }
+      if (!ok) break;
       if (m < p.M) {
         const size_t base = (size_t)m * p.N + n0;
         if (p.N % 16 == 0 && n0 + COLS <= p.N) {
@@ -728,9 +774,6 @@ int few_splits(long long tiles, int nkb, int sms) {
 // E.g. 4,096 x 14,336, few / many / pairs: 64 tokens 19 / 48 / 42, 256 tokens 51 / 50 / 46, 1,024 tokens - / 98 / 77;
 // 4,096 x 4,096: 128 tokens 13 / 17 / 23, 512 tokens 29 / 18 / 24.
 enum Form { FEW, MANY, PAIR };
-// The pairs' sums stay in the tensor cores, which cut what an addition shifts out: 1.4e-6 of a result over 11,264 k, where sums in registers are
-// off by 1e-7.  A float32 result over more than PAIR_K numbers is therefore not theirs.
-constexpr int PAIR_K = 4096;
 Form choose(int M, int N, int K, bool powers, int sms) {
   const int nkb = (K + KBYTES - 1) / KBYTES;
   const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
@@ -817,7 +860,7 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
   const int sms = bspec::sm_count();
   const long long tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + MANY_BN - 1) / MANY_BN;
   const long long pairs_m = (M + 255) / 256, pairs_n = (N + PAIR_BN - 1) / PAIR_BN;
-  const Form form = choose(M, N, K, xs_e8m0 && ws_e8m0 && !(out_f32 && K > PAIR_K), sms);
+  const Form form = choose(M, N, K, xs_e8m0 && ws_e8m0, sms);
   CUtensorMap map_x, map_w;
   const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : 64);
   if (!make_map_bytes(&map_x, X, M, K, ldx, form == FEW ? bn : TILE_ROWS) ||
@@ -834,7 +877,7 @@ BSPEC_API int bspec_gemm_fp8(const void* X, long long ldx, const void* xs, long 
                         1024 + (size_t)MANY_STAGES * (TILE_ROWS + MANY_BN) * KBYTES + 256, stream);
   }
   p.tiles_m = (int)pairs_m; p.tiles_n = (int)pairs_n;
-  return launch_whole(gemm_fp8_pair_kernel, map_x, map_w, p, 2 * (pairs_m * pairs_n < sms / 2 ? pairs_m * pairs_n : sms / 2), PAIR_THREADS,
+  return launch_whole(out_f32 && (K + KBYTES - 1) / KBYTES > PAIR_JOIN ? gemm_fp8_pair_kernel<true> : gemm_fp8_pair_kernel<false>, map_x, map_w, p, 2 * (pairs_m * pairs_n < sms / 2 ? pairs_m * pairs_n : sms / 2), PAIR_THREADS,
                       1024 + (size_t)PAIR_STAGES * PAIR_STAGE + PAIR_SF_SLOTS * PAIR_SF, stream);
 }
 

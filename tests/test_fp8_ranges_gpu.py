@@ -84,3 +84,17 @@ def test_rows_with_ordinary_scales_beside_extreme_ones(ops, M, N, K):
     ws[:, 2:] *= 2.0 ** -70
     check_product(ops.linear_fp8(x, xs, w, ws, out_dtype=torch.float32), x, xs, w, ws)
     ops.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(2048, 8192, 4096), (1500, 7000, 2304), (2048, 8192, 512), (3000, 4480, 4200)])
+def test_float32_results_of_products_of_one_sign(ops, M, N, K):
+    """Cuts towards 0 add up where every product has one sign.  Sums of 128 products are cut by the tensor core four times at most, by up to two half
+    steps (2^-24 of the sum each), their scales are exact here, and K / 128 additions in float32 round evenly to either side: together, as a root
+    mean square over many results, below (8 + sqrt(K / 128)) half steps."""
+    x, xs, w, ws = product_case(ops, M, N, K, True, 0, 0)
+    for t in (x, w):
+        t.view(torch.uint8).bitwise_and_(0x7F)
+    out = ops.linear_fp8(x, xs, w, ws, out_dtype=torch.float32)
+    off = check_product(out, x, xs, w, ws)
+    assert off <= (8 + math.sqrt(K / 128)) * 2.0 ** -24
+    ops.check_status()
