@@ -1919,8 +1919,10 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     whose logit's sigmoid multiplies ``add``.  ``w_up`` [E, ff, d] (``glu``: [E, 2 ff, d], gates first), ``w_down`` [E, d, ff]: bfloat16,
     or float8_e4m3fn with ``up_scale`` / ``down_scale``, a float32 or float8_e8m0fnu scale per 128 x 128 block of every expert (both of one
     type; what ``quantize_fp8`` makes of the stacked matrices).  Scales are at most 2^100.  With 8-bit weights the activations
-    keep 8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.  Longer steps, and
-    hundreds of choices for tens of tokens, are refused: ``moe_route`` and ``moe_experts`` take them."""
+    keep 8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.
+
+    Longer steps are refused, and so are more choices than have room in shared memory: at 64 tokens of 8-bit experts with 4,096 numbers inside and
+    more, 60 of 64 experts each, 55 of 256 or 37 of 1,024 are taken, of bfloat16 experts 167 of 256 or 149 of 1,024; up to 15 tokens all are."""
     stream = _stream_of(h, router, correction, w_up, w_down, up_scale, down_scale, add)
     if h.dim() != 2 or w_up.dim() != 3 or w_down.dim() != 3 or router.dim() != 2:
         raise KernelError("moe_layer takes h and router as matrices, w_up and w_down as stacks of matrices")
