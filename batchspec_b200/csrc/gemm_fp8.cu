@@ -219,7 +219,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         apart = any_of(leaves);
       }
       const int b = i % NB;
-      if (ok) ok = mbar_wait(acc_full + b, (uint32_t)(i / NB) & 1u, abort_flag, p.status, 104);
+      if (ok) ok = warp_wait(acc_full + b, (uint32_t)(i / NB) & 1u, abort_flag, p.status, 104);
       if (!ok) continue;
       tc_fence_after();
       const float4* f = reinterpret_cast<const float4*>(scales + (i % FEW_WINDOW) * BN);
@@ -411,7 +411,7 @@ gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
           x_next = scale_at(p.xs, srow, kb + 1);
           w_next = scale_at(p.ws, wrow, kb + 1);
         }
-        if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 108))) break;
+        if (!(ok = warp_wait(acc_full + b, phase, abort_flag, p.status, 108))) break;
         tc_fence_after();
         // all columns in one load: what bounds this loop is the number of trips to the tensor memory, not their width
         uint32_t v[COLS];
@@ -672,7 +672,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       for (int i = 0; i < 3; ++i) w[i] = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
       g += 4;
       fetch();
-      if (!(ok = mbar_wait(sf_empty + slot, phase ^ 1u, abort_flag, p.status, 124))) break;
+      if (!(ok = warp_wait(sf_empty + slot, phase ^ 1u, abort_flag, p.status, 124))) break;
       unsigned char* to = sf + slot * PAIR_SF + lane * 16;
 #pragma unroll
       for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(to + 512 * i) = w[i];
@@ -694,7 +694,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
       float acc[COLS];
       // this thread's columns of an accumulator, which then is free; into the sums or, JOIN, onto them
       auto take = [&]() {
-        if (!(ok = mbar_wait(acc_full + b, phase, abort_flag, p.status, 125))) return;
+        if (!(ok = warp_wait(acc_full + b, phase, abort_flag, p.status, 125))) return;
         tc_fence_after();
         const uint32_t from = tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * PAIR_BN + half * COLS);
         if constexpr (JOIN) {

@@ -613,16 +613,17 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    // the threads of a group meet (a bounded wait, so that none is left behind when another one gives up)
+    // the threads of a group meet (a bounded wait, so that none is left behind when another one gives up).  Here as in every wait of a warp its lanes
+    // learn one answer: what follows is for whole warps.
     auto meet_all = [&]() {
       arrive(meet + group);
-      ok = ok && mbar_wait_short(meet + group, meet_phase, abort_flag, p.status, 118);
+      ok = ok && warp_wait_short(meet + group, meet_phase, abort_flag, p.status, 118);
       meet_phase ^= 1u;
     };
 #pragma unroll 1
     for (int np = 0; ok; ++np) {
       const int q = np % QUEUE;
-      if (!(ok = mbar_wait_short(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
+      if (!(ok = warp_wait_short(q_full + q, (uint32_t)(np / QUEUE) & 1u, abort_flag, p.status, 119))) break;
       const Piece piece = queue[q];
       arrive(q_empty + q);
       if (piece.down < 0) break;
@@ -644,7 +645,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
         const float* f = ys;
         // the columns' scales: of the tokens, or of a window of this expert's u (whose first copies are on their way)
         auto column_scales = [&](int i) {
-          if (piece.down && !up_known) ok = mbar_wait_short(&up_done, 0u, abort_flag, p.status, 120);
+          if (piece.down && !up_known) ok = ok && warp_wait_short(&up_done, 0u, abort_flag, p.status, 120);
           up_known = piece.down;
           meet_all();                                        // nobody reads the last ones any more
           const int blocks = (p.ff + 63) / 64, b0 = 2 * piece.s0 + i, rows = piece.down ? min(steps - i, WINDOW) : 1, some = piece.down ? cnt : p.n;
@@ -671,7 +672,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           const float w_a = __shfl_sync(0xffffffffu, wa, s & 31), w_b = __shfl_sync(0xffffffffu, wb, s & 31);
           // the weights' scale first: what it makes of a sum (up to 2^25) stays in float32's range for scales up to 2^100, and tokens may be of any size
           const float w = w_block == block_a ? w_a : w_b;
-          if (ok) ok = mbar_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+          if (ok) ok = warp_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
           const uint32_t from = lane_base + (uint32_t)(slot * WIDTH);
           tc_fence_after();
 #pragma unroll
@@ -696,7 +697,7 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
           f += piece.down ? NB : 0;
         }
       } else {
-        ok = mbar_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
+        ok = warp_wait_short(acc_full + slot, slot_phase, abort_flag, p.status, 120);
         tc_fence_after();
       }
       // to shared memory, from where a few instructions per entry take them on: what is executed once per piece costs the fetch of its
@@ -784,9 +785,9 @@ moe_layer_experts_kernel(const __grid_constant__ CUtensorMap map_up, const __gri
     }
     // ---- when every down piece of every CTA is done: the sums over the choices, four columns of a token per thread
     if (et == 0 && ok && !wait_for(p.counters + 3, down_pieces, p.status, abort_flag)) ok = false;
+    ok = __all_sync(0xffffffffu, ok);
     __threadfence();
     meet_all();
-    ok = __all_sync(0xffffffffu, ok);
     // few of them: eight lanes share a thread's results
     const int quads = (int)p.quads.by, parts = p.top * splits, threads = (int)gridDim.x * 256, share = p.n * quads * 8 <= threads ? 8 : 1;
     const int sub = (threadIdx.x - 64) % share;
