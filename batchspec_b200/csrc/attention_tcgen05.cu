@@ -157,7 +157,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_
   // look-up of the CTA's first item read nothing that the kernel before this one writes, so they run under its
   // tail; q, the new tokens' keys and `out` are touched only after the wait.
   const unsigned long long t_trace = bspec::g_trace_buf != nullptr ? bspec::global_timer() : 0ull;
-  bspec::pdl_launch_dependents();
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   __nv_bfloat16* Qs = reinterpret_cast<__nv_bfloat16*>(smem);                  // QT x [128][128]
@@ -210,6 +209,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // not before this CTA holds its tensor memory, a wait without a limit: a CTA of the next kernel that took it would keep it until this kernel's end
+  bspec::pdl_launch_dependents();
   bspec::pdl_wait();
   bspec::trace_record(30, t_trace);
   uint32_t item_no = 0;          // items this role has taken from the ring

@@ -109,7 +109,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   float* part = reinterpret_cast<float*>(smem);                        // [BN][128] sums of this K slice, over the stages
 
   const unsigned long long t_trace = bspec::g_trace_buf != nullptr ? bspec::global_timer() : 0ull;
-  bspec::pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile_n = blockIdx.x, tok0 = blockIdx.y * BN, split = blockIdx.z;
   const int kb_total = (p.K + KBYTES - 1) / KBYTES;
@@ -136,6 +135,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // Not before this CTA holds its tensor memory: that is a wait without a limit, and a CTA of the next kernel that took the columns first would keep
+  // them until this kernel has ended.  (Three CTAs of 256 columns fit an SM where K is short.)
+  bspec::pdl_launch_dependents();
 
   float acc[BN];
 #pragma unroll

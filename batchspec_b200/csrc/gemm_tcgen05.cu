@@ -109,7 +109,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   float* part = reinterpret_cast<float*>(smem);      // [bn][128] partial tile of this K slice (reuses the stages)
 
   const unsigned long long t_trace = bspec::g_trace_buf != nullptr ? bspec::global_timer() : 0ull;
-  bspec::pdl_launch_dependents();           // the next kernel may start its own prologue and weight prefetch
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile_a = blockIdx.x;            // 128-row tile of the operand on the accumulator rows
   const int tile_b = blockIdx.y;            // bn-row tile of the other operand
@@ -137,6 +136,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // the next kernel may start its own prologue and weight prefetch; not before this CTA holds its tensor memory, a wait without a limit
+  bspec::pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {

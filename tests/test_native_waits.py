@@ -21,3 +21,21 @@ def test_a_warp_learns_one_answer_from_a_wait(name):
     for short in ("", "_short"):
         body = re.search(r"bool warp_wait" + short + r"\([^{]*\{([^}]*)\}", helpers).group(1)
         assert body.strip().startswith("return " + WHOLE_WARP + "mbar_wait" + short + "(")
+
+
+def kernels_with_tensor_memory():
+    """(file, kernel, its text) of every kernel that takes tensor memory."""
+    found = []
+    for path in sorted(CSRC.glob("*.cu")):
+        for part in path.read_text().split("__global__")[1:]:
+            if "tcgen05.alloc" in part:
+                found.append(pytest.param(part, id=path.name + ":" + re.search(r"(\w+_kernel)\(", part).group(1)))
+    return found
+
+
+@pytest.mark.parametrize("text", kernels_with_tensor_memory())
+def test_tensor_memory_is_held_before_the_next_kernel_may_start(text):
+    """``tcgen05.alloc`` waits without a limit.  A kernel that lets its successor start before all of its own CTAs hold their columns could wait
+    for columns that a CTA of the successor holds, which waits for this kernel's end."""
+    starts = [m.start() for m in re.finditer(r"pdl_(?:launch_dependents|prologue|prologue_late)\(", text)]
+    assert not starts or min(starts) > text.index("tcgen05.alloc")
