@@ -764,7 +764,7 @@ bool make_map_bytes(CUtensorMap* map, const void* base, long long rows, int K, l
 }
 
 // slices of k of the arrangement for few tokens: two CTAs share an SM, and K is cut so that the CTAs about fill those slots, at least 4 blocks
-// to a slice, clusters of a power of two
+// to a slice; 1, 2, 4 or 8, and where the rounding of their lengths leaves the eighth empty (33 to 35, 41, 42 and 49 blocks), seven
 int few_splits(long long tiles, int nkb, int sms) {
   long long splits = 2ll * sms / tiles;
   if (splits > nkb / 4) splits = nkb / 4;
