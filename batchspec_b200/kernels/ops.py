@@ -1921,8 +1921,9 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     type; what ``quantize_fp8`` makes of the stacked matrices).  Scales are at most 2^100.  With 8-bit weights the activations
     keep 8 bits (each is the sum of two e4m3 numbers).  Both inner sizes are multiples of 8, with 8-bit weights of 16.
 
-    Longer steps are refused, and so are more choices than have room in shared memory: at 64 tokens of 8-bit experts with 4,096 numbers inside and
-    more, 60 of 64 experts each, 55 of 256 or 37 of 1,024 are taken, of bfloat16 experts 167 of 256 or 149 of 1,024; up to 15 tokens all are."""
+    Longer steps are refused (they go 64 tokens at a time, or with bfloat16 experts through ``moe_route`` and ``moe_experts``), and so are
+    more choices than have room in shared memory: at 64 tokens of 8-bit experts with 4,096 numbers inside and more, 60 of 64 experts each, 55 of
+    256 or 37 of 1,024 are taken, of bfloat16 experts 167 of 256 or 149 of 1,024; up to 15 tokens all are."""
     stream = _stream_of(h, router, correction, w_up, w_down, up_scale, down_scale, add)
     if h.dim() != 2 or w_up.dim() != 3 or w_down.dim() != 3 or router.dim() != 2:
         raise KernelError("moe_layer takes h and router as matrices, w_up and w_down as stacks of matrices")
@@ -1934,7 +1935,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
         raise KernelError(f"moe_layer takes bfloat16 tokens and router, experts in bfloat16 or float8_e4m3fn; got {h.dtype}, {router.dtype}, "
                           f"{w_up.dtype}, {w_down.dtype}")
     if n > MOE_LAYER_MAX:
-        raise KernelError(f"moe_layer takes at most {MOE_LAYER_MAX} tokens, got {n}: longer steps go through moe_route and moe_experts")
+        raise KernelError(f"moe_layer takes at most {MOE_LAYER_MAX} tokens, got {n}: longer steps go {MOE_LAYER_MAX} tokens at a time, or with "
+                          "bfloat16 experts through moe_route and moe_experts")
     unit = 16 if fp8 else 8
     if E < 1 or many > 1024 or identity < 0 or d < 1 or ff < 1 or d % unit or ff % unit or (glu and ff_up % 2):
         raise KernelError(f"moe_layer: {E} experts (+ {identity}) of {d} x {ff} are not supported: at most 1024, sizes multiples of {unit}")
@@ -1972,7 +1974,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     # everything between the two kernels, counters too: a buffer of its own, so that calls on other streams or in other graphs share nothing
     size = lib.bspec_moe_layer_scratch(n, d, ff, top, int(fp8), E)
     if size == 0:
-        raise KernelError(f"moe_layer: {top} choices for each of {n} tokens among {E} experts do not fit: moe_route and moe_experts take them")
+        raise KernelError(f"moe_layer: {top} choices for each of {n} tokens among {E} experts do not fit: take fewer tokens at a time, or with "
+                          "bfloat16 experts moe_route and moe_experts")
     scratch = h.new_empty((size,), dtype=torch.uint8)
     rule = (1 if softmax_top else 2 if softmax else 0) + (4 if group_max else 0) + (8 if renormalise else 0)
     _check(lib.bspec_moe_layer(h.data_ptr(), n, d, router.data_ptr(), router.shape[0], _ptr(correction),

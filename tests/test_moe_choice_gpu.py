@@ -116,3 +116,16 @@ def test_the_documented_numbers_of_choices(ops, fp8, E, most):  # noqa: F811
     for ff in (4096, 14336):
         assert size(64, 64, ff, most, fp8, E) > 0 and (most == E or size(64, 64, ff, most + 1, fp8, E) == 0)
         assert size(15, 64, ff, E, fp8, E) > 0
+
+
+@pytest.mark.parametrize("weights", ["bfloat16", "e8m0"])
+def test_a_longer_step_goes_as_its_refusal_says(ops, weights):  # noqa: F811
+    args, kw, upv, downv = layer_case(ops, 150, 16, 0, 3, 128, 64, True, weights, "softmax_top", 1, 1, "plain", True)
+    with pytest.raises(ops.KernelError, match="64 tokens at a time, or with bfloat16 experts through moe_route and moe_experts"):
+        ops.moe_layer(*args, **kw)
+    parts = [ops.moe_layer(args[0][i:i + 64], *args[1:], **dict(kw, add=kw["add"][i:i + 64])) for i in range(0, 150, 64)]
+    layer.check_layer(torch.cat(parts), args, kw, upv, downv, "softmax_top", rows=range(0, 150, 13))
+    with pytest.raises(ops.KernelError, match="fewer tokens at a time"):
+        wide = torch.zeros(64, 64, device=DEV, dtype=torch.bfloat16)
+        ops.moe_layer(wide, torch.zeros(512, 64, device=DEV, dtype=torch.bfloat16), None, 1, 1, 512, 1.0,
+                      torch.zeros(512, 32, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(512, 64, 32, device=DEV, dtype=torch.bfloat16))
