@@ -571,5 +571,13 @@ BSPEC_API int bspec_gemm_tc_qkv_rope(const void* X, const void* W, void* C, int 
 // Switch programmatic dependent launch on (default) or off for every kernel of this library.
 BSPEC_API void bspec_set_pdl(int on) { bspec::pdl_enabled() = on != 0; }
 
+// The calling thread's capture mode (0 global, 1 thread-local, 2 relaxed: calls that are no part of a capture are let through); returns the one
+// before, or a negative CUDA error.
+BSPEC_API int bspec_capture_mode(int mode) {
+  cudaStreamCaptureMode m = (cudaStreamCaptureMode)mode;
+  const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+  return e == cudaSuccess ? (int)m : -(int)e;
+}
+
 BSPEC_DEFINE_TRACE_SETTER(bspec_trace_set_gemm_tcgen05)
 BSPEC_DEFINE_BOUNDS_REPORT(bspec_bounds_report_gemm_tcgen05)

@@ -130,6 +130,7 @@ _SIGNATURES = {
     "bspec_gate_heads": [c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "bspec_quantize_fp8": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_int,
                            c_int, c_void_p],
+    "bspec_capture_mode": [c_int],
     "bspec_gemm_fp8": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "bspec_moe_layer_scratch": [c_int] * 6,
@@ -728,6 +729,24 @@ def sm_count(device=None) -> int:
     return _sm_counts[idx]
 
 
+def _kept_zeros(n: int, device) -> torch.Tensor:
+    """int32 zeros that calls share for as long as the process lives.  A first call inside a capture makes them on a stream that is not captured:
+    in the graph's memory they would hold what was there before until its first replay, and every replay would clear them."""
+    if not torch.cuda.is_current_stream_capturing():
+        return torch.zeros((n,), dtype=torch.int32, device=device)
+    mode = load_library().bspec_capture_mode(2)          # memory may be asked for beside the capture
+    if mode < 0:
+        raise KernelError(f"capture mode: CUDA error {-mode}")
+    try:
+        side = torch.cuda.Stream(device)
+        with torch.cuda.stream(side):
+            zeros = torch.zeros((n,), dtype=torch.int32, device=device)
+        side.synchronize()
+    finally:
+        load_library().bspec_capture_mode(mode)
+    return zeros
+
+
 _tile_counters = {}               # device -> zeroed int32 buffers kept alive (graphs hold their addresses)
 
 
@@ -763,14 +782,14 @@ _work_counters = {}               # device -> two zeroed ints: the prompt attent
 
 def _work_counter(device) -> torch.Tensor:
     if device not in _work_counters:
-        _work_counters[device] = torch.zeros((2,), dtype=torch.int32, device=device)
+        _work_counters[device] = _kept_zeros(2, device)
     return _work_counters[device]
 
 
 def _counters(device, n: int) -> torch.Tensor:
     bufs = _tile_counters.setdefault(device, [])
     if not bufs or bufs[-1].numel() < n:
-        bufs.append(torch.zeros(max(n, 1 << 16), dtype=torch.int32, device=device))
+        bufs.append(_kept_zeros(max(n, 1 << 16), device))
     return bufs[-1]
 
 
@@ -1237,7 +1256,7 @@ _status = {}
 
 def _status_word(device) -> torch.Tensor:
     if device not in _status:
-        _status[device] = torch.zeros((1,), dtype=torch.int32, device=device)
+        _status[device] = _kept_zeros(1, device)
     return _status[device]
 
 
