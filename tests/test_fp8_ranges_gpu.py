@@ -98,3 +98,56 @@ def test_float32_results_of_products_of_one_sign(ops, M, N, K):
     off = check_product(out, x, xs, w, ws)
     assert off <= (8 + math.sqrt(K / 128)) * 2.0 ** -24
     ops.check_status()
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "float32"])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_blocks_of_nan_show_in_their_rows_and_columns_alone(ops, M, N, K, kind):
+    """A token with an infinity, a block of weights with a NaN (as the quantiser marks them), and scales of zero."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    xf, wf = torch.randn(M, K, device=DEV, generator=g), torch.randn(N, K, device=DEV, generator=g)
+    xf[2, 300], wf[130 if N > 130 else 5, 200] = math.inf, math.nan
+    (x, xs), (w, ws) = ops.quantize_fp8(xf), ops.quantize_fp8(wf, 128)
+    if kind == "float32":
+        xs, ws = xs.float(), ws.float()
+        xs[0] = 0
+    out = ops.linear_fp8(x, xs, w, ws, out_dtype=torch.float32)
+    nan = torch.zeros(M, N, dtype=torch.bool, device=DEV)
+    nan[2] = True
+    first = 128 if N > 130 else 0
+    nan[:, first:first + 128] = True
+    assert torch.equal(torch.isnan(out), nan)
+    if kind == "float32":
+        assert bool((out[0, ~nan[0]] == 0).all())
+    keep = [i for i in range(M) if i != 2][:200]
+    cols = torch.nonzero(~nan[0])[:, 0]
+    if len(cols):
+        a = x[keep].double() * spread(xs[keep], 1, len(keep), K)
+        b = (w.double() * spread(ws, 128, N, K))[cols]
+        room = (a.abs() @ b.abs().t()) * (2 * K + 8) * 2.0 ** -24
+        assert bool(((out[keep][:, cols].double() - a @ b.t()).abs() <= room).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_the_smallest_and_largest_powers(ops, M, N, K):
+    """Scales of 2^-127, which is below float32's normal numbers, meet scales that bring the products back."""
+    for xe, we in ((0, 200), (190, 40)):
+        x, xs, w, ws = product_case(ops, M, N, K, True, 0, 0)
+        xs, ws = torch.full(xs.shape, xe, dtype=torch.uint8, device=DEV), torch.full(ws.shape, we, dtype=torch.uint8, device=DEV)
+        xs, ws = xs.view(torch.float8_e8m0fnu), ws.view(torch.float8_e8m0fnu)
+        check_product(ops.linear_fp8(x, xs, w, ws, out_dtype=torch.float32), x, xs, w, ws)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("batch,R,K", [(70001, 5, 8), (33000, 130, 8), (3, 1, 70000)])
+def test_quantising_more_matrices_than_a_grid_is_high(ops, batch, R, K, block_rows):
+    g = torch.Generator(device=DEV).manual_seed(batch)
+    x = torch.randn(batch, R, K, device=DEV, generator=g)
+    q, s = ops.quantize_fp8(x, block_rows)
+    for i in (0, 1, batch // 2, 65534 // -(-R // block_rows) if batch > 3 else 1, batch - 1):
+        i = min(i, batch - 1)
+        want_q, want_s = ops.quantize_fp8(x[i], block_rows)
+        assert torch.equal(q[i].float(), want_q.float()) and torch.equal(s[i].float(), want_s.float())
+    room = q.float() * s.float().repeat_interleave(block_rows, 1)[:, :R].repeat_interleave(128, 2)[:, :, :K] - x
+    assert bool((room.abs() <= x.abs() * 2.0 ** -4 + s.float().amax() * 2.0 ** -10).all())

@@ -41,3 +41,20 @@ def test_large_tokens_beside_ordinary_ones(ops, weights):  # noqa: F811
     args[0][15] = 0
     check_layer(ops.moe_layer(*args, **kw), args, kw, upv, downv, "softmax_top")
     ops.check_status()
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "float32"])
+def test_a_block_of_nan_among_the_experts_shows_where_it_is_taken(ops, kind):  # noqa: F811
+    for name in ("up_scale", "down_scale"):
+        args, kw, upv, downv = layer_case(ops, 24, 8, 0, 2, 256, 128, True, kind, "softmax_top", 1, 1, None, False)
+        ids, _ = ops.moe_route(args[0], args[1], args[2], 1, 1, 2, 1.0, softmax_top=True)
+        e = int(ids[0, 0])
+        if kind == "e8m0":
+            kw[name].view(torch.uint8)[e, 0, 0] = 255
+        else:
+            kw[name][e, 0, 0] = float("nan")
+        out = ops.moe_layer(*args, **kw)
+        taken = (ids == e).any(dim=1)
+        assert 0 < int(taken.sum()) < 24
+        assert bool(torch.isnan(out[taken][:, :128]).all()) and not bool(torch.isnan(out[~taken]).any())
+        check_layer(out, args, kw, upv, downv, "softmax_top", rows=torch.nonzero(~taken)[:, 0].tolist())
