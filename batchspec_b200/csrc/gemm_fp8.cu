@@ -19,9 +19,9 @@
 //   pairs         many tokens where both scales are powers of two: the tensor cores multiply by the scales and keep the sums of a whole
 //                 row, two CTAs share a tile (below).
 //
-// Measured on B200: 8 x 28,672 x 4,096 in 20.5 us (5.7 TB/s), 61 x 32,000 x 2,048 into float32 in 18.7 us (3.9 TB/s), 1,537 x 4,096 x 14,336 with
-// float32 scales in 118 us (1.5 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 174 us (2.75 PFLOP/s; 190 and more once the power limit holds;
-// all zeros, which it does not slow down, run at 4.1).
+// Measured on B200: 8 x 28,672 x 4,096 in 20.7 us (5.7 TB/s), 61 x 32,000 x 2,048 into float32 in 19.4 us (3.8 TB/s), 1,537 x 4,096 x 14,336 with
+// float32 scales in 115 us (1.6 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 177 us (2.7 PFLOP/s; 190 and more once the power limit holds;
+// all zeros, which it does not slow down, run at 4.1), into float32 in 229 us.
 #include "e4m3.cuh"
 #include "umma.cuh"
 

@@ -9,11 +9,12 @@
 // a stage costs two copies of weights and a few instructions, and what the sums cost does not grow with the weights.
 //   up     all tokens of the step are columns of every expert (no gather: the columns that did not choose it are dropped)
 //   down   an expert's tokens are its columns: u lies sorted by expert, 16 rows to a copy
-// The activations do not lose precision to the weights' format.  bfloat16 weights: every number of u is the sum of two bfloat16 numbers, 16
-// bits, both columns of the same product.  8-bit weights:  Every activation is the sum of two e4m3 numbers, x = s (a + b / 16): a is x / s rounded to 4 bits, b what is
-// left, times 16; s is a power of two, one for a token's h and one for 64 numbers of u.  That is 8 bits, as many as bfloat16 has (h is met
-// exactly down to 2^-22 of the token's largest number); both are columns of the same product.  A block of 128 k (of 64 in the down
-// products, for the scales of u) gets an accumulator of its own, which the epilogue warps read back and add to float32 sums.
+// Activations take two columns of the same product.  bfloat16 weights: every number of u is the sum of two bfloat16 numbers, 16 bits.
+// 8-bit weights: every activation is the sum of two e4m3 numbers, x = s (a + b / 16): a is x / s rounded to 4 bits, b what is left, times 16; s
+// is a power of two, one for a token's h and one for 64 numbers of u.  That is 8 bits, as many as bfloat16 has, for numbers of h down to 2^-14.8 of
+// the token's largest; below that they lose bits one by one (steps of 2^-22 of the largest).  The result's error goes from 1.66e-3 to 1.8e-3 by it.
+// A block of 128 k (of 64 in the down products, for the scales of u) gets an accumulator of its own, which the epilogue warps read back and add to
+// float32 sums.
 //
 //   route    one cluster of 8 CTAs per 8 tokens: 64 warps share the router's rows and k, partial sums meet in the first CTA's
 //            shared memory, whose warps choose for a token each.  It also clears the counters of the second kernel.
@@ -28,8 +29,10 @@
 // weights have pushed out of the L2 since the last step: loops are kept as loops, and the polls of a wait are a call (1 token 38.4 -> 35.9 us,
 // 8 tokens of 8-bit experts 59.7 -> 53.0; running the epilogue over made-up pieces while the router runs made it slower, 24 us of code),
 // and pieces are numbered without divisions by numbers of the step (61 tokens 133.8 -> 130.5).
-// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 36 us; 8 tokens, gated, 8-bit, 55; 61 tokens, GELU, 128.5 (5.7 TB/s);
-// 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.
+// Measured on B200, 64 experts of 2,048 x 1,408, 6 per token: 1 token, gated, 36 us; 8 tokens of which 12 experts are taken, gated, 8-bit, 55; 61 tokens,
+// GELU, 129.5 (5.7 TB/s); 23 tokens, 20 experts of 1,040 x 720, 8-bit with float32 scales, 36.  Gated, evenly chosen, bfloat16 / 8-bit: 8 tokens (34
+// experts) 110 / 90, 32 tokens 173 / 142, 61 tokens 184 / 201: there the epilogue's steps for 8-bit experts, an accumulator per 64 or 128 k, take longer
+// than the weights.
 #include "moe_choose.cuh"
 #include "e4m3.cuh"
 #include "umma.cuh"
