@@ -19,11 +19,12 @@
 //   pairs         many tokens where both scales are powers of two: the tensor cores multiply by the scales and keep the sums of a whole
 //                 row, two CTAs share a tile (below).
 //
-// Measured on B200: 8 x 28,672 x 4,096 in 20.7 us (5.7 TB/s), 61 x 32,000 x 2,048 into float32 in 19.4 us (3.8 TB/s), 1,537 x 4,096 x 14,336 with
+// Measured on B200: 8 x 28,672 x 4,096 in 20.1 us (5.9 TB/s), 61 x 32,000 x 2,048 into float32 in 18.7 us (3.9 TB/s), 1,537 x 4,096 x 14,336 with
 // float32 scales in 115 us (1.6 PFLOP/s), 2,048 x 28,672 x 4,096 with e8m0 scales in 177 us (2.7 PFLOP/s; 190 and more once the power limit holds;
 // all zeros, which it does not slow down, run at 4.1), into float32 in 229 us.
 #include "e4m3.cuh"
 #include "umma.cuh"
+#include <type_traits>
 
 using namespace bspec;
 
@@ -190,7 +191,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     const uint32_t quad = warp & 3;
     const int et = threadIdx.x - 64;                                   // 0 .. 127
     bspec::pdl_wait();
-    bool ok = true, apart = false;
+    bool ok = true;
     // whether it holds for any epilogue thread; they meet here
     auto any_of = [](bool mine) {
       uint32_t any;
@@ -198,57 +199,67 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                    : "=r"(any) : "r"((uint32_t)mine) : "memory");
       return any != 0u;
     };
-    for (int i = 0; i < nkb; ++i) {
-      if (i % FEW_WINDOW == 0) {
-        // the scales of the next blocks; every epilogue thread comes here, whatever its waits said
-        const int nw = min(FEW_WINDOW, nkb - i);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        bool leaves = false;
-        for (int j = et; j < nw * BN; j += 128) {
-          const int c = j / nw, b = j - c * nw, tok = tok0 + c;        // neighbours read neighbouring blocks of a token
-          float f = 0.f, before = 1.f;
-          if (tok < p.M) {
-            const float x = scale_at(p.xs, tok, kb0 + i + b), w = scale_at(p.ws, tile_n, kb0 + i + b);
-            f = x * w;
-            if (leaves_range(x, w, f)) {
-              split_scales(x, w, before, f);
-              leaves = true;
-            }
-          }
-          scales[b * BN + c] = f;
-          scales[(FEW_WINDOW + b) * BN + c] = before;
-        }
-        apart = any_of(leaves);
+    int b = 0;
+    uint32_t phase = 0u;
+    for (int i0 = 0; i0 < nkb; i0 += FEW_WINDOW) {
+      // the scales of the next blocks; every epilogue thread comes here, whatever its waits said
+      const int nw = min(FEW_WINDOW, nkb - i0);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      bool unusual = false;
+      for (int j = et; j < nw * BN; j += 128) {
+        const int c = j / nw, k = j - c * nw, tok = tok0 + c;          // neighbours read neighbouring blocks of a token
+        const float f = tok < p.M ? scale_at(p.xs, tok, kb0 + i0 + k) * scale_at(p.ws, tile_n, kb0 + i0 + k) : 0.f;
+        unusual |= tok < p.M && !is_ordinary(f);
+        scales[k * BN + c] = f;
       }
-      const int b = i % NB;
-      if (ok) ok = warp_wait(acc_full + b, (uint32_t)(i / NB) & 1u, abort_flag, p.status, 104);
-      if (!ok) continue;
-      tc_fence_after();
-      const float4* f = reinterpret_cast<const float4*>(scales + (i % FEW_WINDOW) * BN);
-      const uint32_t from = tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * BN);
-      auto release = [&]() {
+      const bool apart = any_of(unusual);
+      if (apart) {
+        for (int j = et; j < nw * BN; j += 128) {
+          const int c = j / nw, k = j - c * nw, tok = tok0 + c;
+          float f = scales[k * BN + c], before = 1.f;
+          if (tok < p.M) {
+            const float x = scale_at(p.xs, tok, kb0 + i0 + k), w = scale_at(p.ws, tile_n, kb0 + i0 + k);
+            if (leaves_range(x, w, f)) split_scales(x, w, before, f);
+          }
+          scales[k * BN + c] = f;
+          scales[(FEW_WINDOW + k) * BN + c] = before;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      auto block = [&](int i, auto in_two) {
+        ok = warp_wait(acc_full + b, phase, abort_flag, p.status, 104);
+        if (!ok) return;
+        tc_fence_after();
+        const float4* f = reinterpret_cast<const float4*>(scales + i * BN);
+        const uint32_t from = tmem_base + ((quad * 32u) << 16) + (uint32_t)(b * BN);
+        // an accumulator is read in one trip, and is free for the next products before its numbers are added
+        uint32_t v[BN];
+        if constexpr (BN == 16) tc_ld16(from, v);
+        else if constexpr (BN == 32) tc_ld32(from, v);
+        else tc_ld64(from, v);
+        tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + b);             // one arrival per warp: those of its lanes would come one after the other
+        if (++b == NB) { b = 0; phase ^= 1u; }
+        if constexpr (decltype(in_two)::value) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * reinterpret_cast<const float*>(f)[FEW_WINDOW * BN + c]);
+        }
+#pragma unroll
+        for (int c = 0; c < BN; c += 4) {
+          const float4 g = f[c / 4];
+          acc[c] = fmaf(__uint_as_float(v[c]), g.x, acc[c]);
+          acc[c + 1] = fmaf(__uint_as_float(v[c + 1]), g.y, acc[c + 1]);
+          acc[c + 2] = fmaf(__uint_as_float(v[c + 2]), g.z, acc[c + 2]);
+          acc[c + 3] = fmaf(__uint_as_float(v[c + 3]), g.w, acc[c + 3]);
+        }
       };
-      // an accumulator is read in one trip, and is free for the next products before its numbers are added
-      uint32_t v[BN];
-      if constexpr (BN == 16) tc_ld16(from, v);
-      else if constexpr (BN == 32) tc_ld32(from, v);
-      else tc_ld64(from, v);
-      tc_wait_ld();
-      release();
-      if (apart) {
-#pragma unroll
-        for (int c = 0; c < BN; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * reinterpret_cast<const float*>(f)[FEW_WINDOW * BN + c]);
-      }
-#pragma unroll
-      for (int c = 0; c < BN; c += 4) {
-        const float4 g = f[c / 4];
-        acc[c] = fmaf(__uint_as_float(v[c]), g.x, acc[c]);
-        acc[c + 1] = fmaf(__uint_as_float(v[c + 1]), g.y, acc[c + 1]);
-        acc[c + 2] = fmaf(__uint_as_float(v[c + 2]), g.z, acc[c + 2]);
-        acc[c + 3] = fmaf(__uint_as_float(v[c + 3]), g.w, acc[c + 3]);
+      // two loops, so that the ordinary one is no longer for the other's sake (61 x 32,000 x 2,048: 18.7 us, with a branch in one loop 19.3)
+      if (!apart) {
+        for (int i = 0; i < nw && ok; ++i) block(i, std::false_type{});
+      } else {
+        for (int i = 0; i < nw && ok; ++i) block(i, std::true_type{});
       }
     }
     // every product of this slice has completed and every stage has been read: the sums take their place, where few instructions, the same for
