@@ -1938,7 +1938,8 @@ def moe_layer(h: torch.Tensor, router: torch.Tensor, correction: Optional[torch.
     whose logit's sigmoid multiplies ``add``.  ``w_up`` [E, ff, d] (``glu``: [E, 2 ff, d], gates first), ``w_down`` [E, d, ff]: bfloat16,
     or float8_e4m3fn with ``up_scale`` / ``down_scale``, a float32 or float8_e8m0fnu scale per 128 x 128 block of every expert (both of one
     type; what ``quantize_fp8`` makes of the stacked matrices).  Scales are at most 2^100.  With 8-bit weights the activations
-    keep 8 bits (each is the sum of two e4m3 numbers; numbers of h below 2^-14 of a token's largest keep fewer).  Both inner sizes are multiples of 8, with 8-bit weights of 16.
+    keep 8 bits (each is the sum of two e4m3 numbers; numbers of h below 2^-14 of a token's largest keep fewer).  Both inner sizes are multiples
+    of 8, with 8-bit weights of 16.
 
     Longer steps are refused (they go 64 tokens at a time, or with bfloat16 experts through ``moe_route`` and ``moe_experts``), and so are
     more choices than have room in shared memory: at 64 tokens of 8-bit experts with 4,096 numbers inside and more, 60 of 64 experts each, 55 of
